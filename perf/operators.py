@@ -75,11 +75,10 @@ def draw(rng):
         K = 16 * _log(rng, 8, 896)
         N = _log(rng, 64, 14336)
         M = _log(rng, 1, max(1, min(4096, 4096 * 14336 * 4096 // (K * N))))
-        return {"op": op, "rows": M, "out": N, "in": K, "dtype": rng.choice(["bf16", "bf16", "bf16", "fp16", "fp32"]),
-                "scales": kind}
+        return {"op": op, "rows": M, "out": N, "in": K, "dtype": rng.choice(["bf16", "bf16", "fp16"]), "scales": kind}
     if op == "gather":
         return {"op": op, "rows": _log(rng, 1, 4096), "experts": _log(rng, 1, 128), "out": _log(rng, 64, 2048),
-                "in": 16 * _log(rng, 8, 128), "dtype": rng.choice(["bf16", "bf16", "fp16", "fp32"]), "scales": kind}
+                "in": 16 * _log(rng, 8, 128), "dtype": rng.choice(["bf16", "bf16", "fp16"]), "scales": kind}
     E = _log(rng, 4, 128)
     return {"op": op, "tokens": _log(rng, 1, 2048), "experts": E, "k": min(E, rng.choice([1, 2, 4, 6, 8, 8])),
             "hidden": 16 * _log(rng, 16, 128), "inter": 128 * rng.randint(1, 6), "scales": kind}
