@@ -275,6 +275,61 @@ int kmi_qmm_batched(const void* x, const int64_t* x_strides, const uint32_t* w, 
                     int64_t nx, float x_scale, void* y, int64_t ldy, void* workspace, size_t workspace_bytes,
                     void* stream);
 
+/*
+ * E4M3 with one scale per block of 128 x 128: the published form of weights in
+ * 8-bit floating point (a float8 weight beside its weight_scale_inv); no
+ * counterpart in the reference.
+ *
+ * kmi_quantize_fp8: w [batch, rows, cols] (dtype, 16-byte aligned, cols % 16 ==
+ * 0) -> wq, the E4M3 bytes (4 per uint32, 16-byte aligned), and scales [batch,
+ * ceil(rows/128), ceil(cols/128)], E8M0 bytes: 2^e with the smallest e >= -126
+ * such that the block's largest magnitude is at most 448 * 2^e; codes w / 2^e
+ * (exact) rounded to the nearest, ties to even.  A block with an infinity or a
+ * NaN: scale 255 (NaN), codes 0.  The last blocks may be partial.
+ * kmi_dequantize_fp8: out = T(code * scale), the product in float32.  scales:
+ * float32, or with e8m0 != 0 the bytes above.
+ */
+int kmi_quantize_fp8(const void* w, int dtype, int64_t batch, int64_t rows, int64_t cols, uint32_t* wq,
+                     uint8_t* scales, void* stream);
+int kmi_dequantize_fp8(const uint32_t* wq, const void* scales, int e8m0, int64_t batch, int64_t rows, int64_t cols,
+                       void* out, int out_dtype, void* stream);
+
+/*
+ * y[M, N] = xhat[M, K] @ What[N, K]^T over such weights, both operands in 8
+ * bits: xhat is x quantized per row and 128 inputs as kmi_quantize_fp8 does a
+ * block (power-of-two scales; a row with an infinity or a NaN gives NaN).
+ * fp32 accumulation (the matrix instruction lines up each run of 8 products with
+ * its largest and keeps 13 binary places below it), y rounded once to x's dtype
+ * (bfloat16 or float16).  K % 16 == 0; x and w 16-byte aligned; scales [ceil(N/128), ceil(K/128)] float32 (any
+ * values) or E8M0 bytes.  Each output row depends only on its own input row.
+ * `workspace` (kmi_qmm_fp8_workspace_bytes) may be NULL when that is 0.
+ */
+size_t kmi_qmm_fp8_workspace_bytes(int64_t M, int64_t K, int64_t N, int dtype);
+int kmi_qmm_fp8(const void* x, int64_t M, int64_t K, int64_t N, const uint32_t* w, const void* scales, int e8m0,
+                int dtype, void* y, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * kmi_gather_qmm over such weights: y[p, m] = xhat[lhs[p], m] @ What[rhs[p]]^T,
+ * x [X, M, K], w [E, N, K/4], scales [E, ceil(N/128), ceil(K/128)], E <= 4096.
+ * Rows are grouped by expert on the GPU.  An index out of range gives a zero row.
+ */
+size_t kmi_gather_qmm_fp8_workspace_bytes(int64_t P, int64_t M, int64_t E, int64_t K, int64_t N, int dtype);
+int kmi_gather_qmm_fp8(const void* x, int64_t X, int64_t M, int64_t K, const uint32_t* w, const void* scales,
+                       int e8m0, int64_t E, int64_t N, const int32_t* lhs, const int32_t* rhs, int64_t P, int dtype,
+                       void* y, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * kmi_switch_glu over such experts: w_gu [E, 2I, H/4] (gate rows, then up rows;
+ * I % 128 == 0), w_down [E, H, I/4], H % 16 == 0, k <= 64.  The activations
+ * round(round(silu(gate)) * up) are quantized per row and 128 of I on their
+ * way into the down product.  bf16.  out [T, k, H], or [T, H] with scores.
+ */
+size_t kmi_switch_glu_fp8_workspace_bytes(int64_t T, int64_t H, int64_t I, int k, int64_t E);
+int kmi_switch_glu_fp8(const void* x, int64_t T, int64_t H, int64_t I, int k, const int32_t* inds,
+                       const void* scores, const uint32_t* w_gu, const void* s_gu, const uint32_t* w_down,
+                       const void* s_down, int e8m0, int64_t E, int dtype, void* out, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
 /* mask kinds of kmi_masked_softmax */
 #define KMI_MASK_NONE 0
 #define KMI_MASK_BOOL 1   /* uint8, nonzero = visible; hidden scores become finfo(bf16).min */

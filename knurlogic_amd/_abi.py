@@ -69,6 +69,14 @@ SIGNATURES = {
                                   P, P, SZ, P]),
     "kmi_vq_packed_switch_glu": (I, [P, I64, I64, I64, I, P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I64, I,
                                      P, P, SZ, P]),
+    "kmi_quantize_fp8": (I, [P, I, I64, I64, I64, P, P, P]),
+    "kmi_dequantize_fp8": (I, [P, P, I, I64, I64, I64, P, I, P]),
+    "kmi_qmm_fp8": (I, [P, I64, I64, I64, P, P, I, I, P, P, SZ, P]),
+    "kmi_qmm_fp8_workspace_bytes": (SZ, [I64, I64, I64, I]),
+    "kmi_gather_qmm_fp8": (I, [P, I64, I64, I64, P, P, I, I64, I64, P, P, I64, I, P, P, SZ, P]),
+    "kmi_gather_qmm_fp8_workspace_bytes": (SZ, [I64, I64, I64, I64, I64, I]),
+    "kmi_switch_glu_fp8": (I, [P, I64, I64, I64, I, P, P, P, P, P, P, I, I64, I, P, P, SZ, P]),
+    "kmi_switch_glu_fp8_workspace_bytes": (SZ, [I64, I64, I64, I, I64]),
     "kmi_read_probe": (I, [P, I64, I, P, P]),
     "kmi_mfma_probe": (I, [P, I, I, P, P, P]),
 }

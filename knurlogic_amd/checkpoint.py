@@ -186,11 +186,39 @@ def _repack(codes: torch.Tensor, bits: int) -> torch.Tensor:
     return words.to(torch.int32).view(torch.uint32)
 
 
+def fp8_recipe(weights: dict, path: str) -> dict | None:
+    """{group_size, bits, mode} of a layer published in block-scaled 8-bit
+    floating point -- ``weight`` float8_e4m3fn [..., N, K] beside
+    ``weight_scale_inv`` [..., ceil(N/128), ceil(K/128)], which multiplies it
+    -- or None when ``path`` has no such scales."""
+    s = weights.get(f"{path}.weight_scale_inv")
+    if s is None:
+        return None
+    w = weights.get(f"{path}.weight")
+    if w is None or w.dtype != torch.float8_e4m3fn:
+        raise ValueError(f"{path}: weight_scale_inv beside a weight that is not float8_e4m3fn")
+    want = (*w.shape[:-2], -(-w.shape[-2] // 128), -(-w.shape[-1] // 128)) if w.dim() >= 2 else None
+    if want is None or tuple(s.shape) != want or w.shape[-1] % 16:
+        raise ValueError(f"{path}: weight_scale_inv {tuple(s.shape)} for weight {tuple(w.shape)}: one scale per "
+                         "block of 128 x 128, inputs in multiples of 16")
+    return {"group_size": 128, "bits": 8, "mode": "fp8"}
+
+
 def build(weights: dict, path: str, in_dims: int | None = None, quant: dict | None = None,
           device="cuda", prefix: str = ""):
     """This package's module for the packed (or VQ) layer ``path``: a
     QuantizedLinear (2-D weight), QuantizedSwitchLinear (3-D) or
-    VQSwitchLinear; None when ``path`` is stored unpacked."""
+    VQSwitchLinear; None when ``path`` is stored unpacked.  A float8 weight
+    with block scales (``fp8_recipe``) becomes a layer of mode fp8, its scales
+    in float32."""
+    fp8 = fp8_recipe(weights, path)
+    if fp8 is not None:
+        w = weights[f"{path}.weight"].contiguous().view(torch.uint8).view(torch.uint32).to(device)
+        s = weights[f"{path}.weight_scale_inv"].to(device=device, dtype=torch.float32)
+        bias = weights.get(f"{path}.bias")
+        bias = bias.to(device) if bias is not None else None
+        cls = QuantizedLinear if w.dim() == 2 else QuantizedSwitchLinear
+        return cls(w, s, None, bias, **fp8)
     vq = vq_recipe(weights, path, in_dims=in_dims)
     if vq is not None:
         codes = weights[f"{path}.codes"]
@@ -217,8 +245,10 @@ def build(weights: dict, path: str, in_dims: int | None = None, quant: dict | No
             raise ValueError(f"{path}: packed, but neither a module shape nor the config's quantization "
                              "block gives its input size")
     r = recipe(weights, path, in_dims, quant, prefix)
-    if r["mode"] not in ("affine", "mxfp4", "mxfp8"):
-        raise ValueError(f"{path}: mode {r['mode']!r} is not implemented (affine, mxfp4, mxfp8)")
+    if r["mode"] not in ("affine", "mxfp4", "mxfp8", "fp8"):
+        raise ValueError(f"{path}: mode {r['mode']!r} is not implemented (affine, mxfp4, mxfp8, fp8)")
+    if r["mode"] == "fp8":
+        r["group_size"] = 128                              # the last block of inputs may be partial
     w = _u32(weights[f"{path}.weight"]).to(device)
     s = weights[f"{path}.scales"].to(device)
     if r["mode"] == "affine":
@@ -233,7 +263,7 @@ def build(weights: dict, path: str, in_dims: int | None = None, quant: dict | No
 
 
 def load_quantized(model_path=None, files=None, shapes: dict | None = None, device="cuda") -> dict:
-    """Every packed or VQ layer of an mlx-format artifact (``model*.safetensors``
+    """Every packed, VQ or block-scaled float8 layer of an mlx-format artifact (``model*.safetensors``
     and config.json under ``model_path``, or explicit ``files``) as this
     package's modules, {path: module}.  ``shapes`` maps a layer path to its
     dense weight shape (the module skeleton's), else input sizes come from
@@ -247,7 +277,7 @@ def load_quantized(model_path=None, files=None, shapes: dict | None = None, devi
     quant = artifact_quantization(model_path) if model_path is not None else {}
     declared = json.loads(meta["vq_modules"]) if "vq_modules" in meta else {}
     paths = sorted({k.rsplit(".", 1)[0] for k in weights
-                    if k.endswith(".scales") or k.endswith(".codes") or k.endswith(".vq_scales")})
+                    if k.endswith((".scales", ".codes", ".vq_scales", ".weight_scale_inv"))})
     out = {}
     for p in paths:
         in_dims = None

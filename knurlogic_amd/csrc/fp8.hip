@@ -1,0 +1,142 @@
+// The C entries of the block-scaled E4M3 products: a dense projection, rows
+// against their own expert (mlx's gather_qmm), and an expert block's SwitchGLU
+// with the weighted combine.
+#include "fp8.hpp"
+#include "qgemv.hpp"
+#include "../../include/knurlogic_amd.h"
+
+namespace kmi {
+
+namespace {
+
+size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
+
+constexpr int64_t MAX_E = 4096;        // of the GPU sort
+
+int check_operands(const char* what, int dtype, int64_t K, int64_t N, const void* x, const void* w) {
+    KMI_CHECK_ARG(dtype == BF16 || dtype == F16, "%s: dtype %d (bfloat16 or float16)", what, dtype);
+    KMI_CHECK_ARG(K > 0 && K % 16 == 0 && K < (1 << 24), "%s: K=%lld (a multiple of 16 below 2^24)", what, (long long)K);
+    KMI_CHECK_ARG(N > 0 && N < (1LL << 31), "%s: N=%lld", what, (long long)N);
+    KMI_CHECK_ARG((((uintptr_t)x | (uintptr_t)w) & 15) == 0, "%s: x and w on 16 bytes", what);
+    return OK;
+}
+
+// rows per tile: 16, or 32 / 64 where an active expert has more
+int tile_rows(int64_t per) { return per <= 16 ? 16 : per <= 32 ? 32 : 64; }
+
+int64_t per_expert(int64_t P, int64_t M, int64_t E) { return ceil_div(P * M, P < E ? P : E); }
+
+}  // namespace
+
+}  // namespace kmi
+
+using namespace kmi;
+
+extern "C" {
+
+size_t kmi_qmm_fp8_workspace_bytes(int64_t M, int64_t K, int64_t N, int dtype) { return 0; }
+
+int kmi_qmm_fp8(const void* x, int64_t M, int64_t K, int64_t N, const uint32_t* w, const void* scales, int e8m0,
+                int dtype, void* y, void* workspace, size_t workspace_bytes, void* stream) {
+    clear_error();
+    const char* what = "qmm (fp8)";
+    int rc = check_operands(what, dtype, K, N, x, w);
+    if (rc) return rc;
+    KMI_CHECK_ARG(M >= 0 && M < (1 << 21), "%s: M=%lld", what, (long long)M);
+    if (M == 0) return OK;
+    KMI_CHECK_ARG(x && w && scales && y, "%s: null pointer", what);
+    F8Args a = {};
+    a.w = (const unsigned char*)w; a.s = scales; a.e8 = e8m0; a.E = 1; a.wrows = N; a.K = K; a.N = N;
+    a.x = x; a.xrows = M; a.y = y; a.rows = M; a.tm = tile_rows(M);
+    return launch_fp8_skinny(a, dtype, false, ceil_div(M, a.tm), (hipStream_t)stream);
+}
+
+size_t kmi_gather_qmm_fp8_workspace_bytes(int64_t P, int64_t M, int64_t E, int64_t K, int64_t N, int dtype) {
+    if (P <= 0 || M <= 0 || E <= 0 || K <= 0 || N <= 0) return 0;
+    return sort_index_bytes(P * M, E, tile_rows(per_expert(P, M, E)));
+}
+
+int kmi_gather_qmm_fp8(const void* x, int64_t X, int64_t M, int64_t K, const uint32_t* w, const void* scales,
+                       int e8m0, int64_t E, int64_t N, const int32_t* lhs, const int32_t* rhs, int64_t P, int dtype,
+                       void* y, void* workspace, size_t workspace_bytes, void* stream) {
+    clear_error();
+    const char* what = "gather_qmm (fp8)";
+    int rc = check_operands(what, dtype, K, N, x, w);
+    if (rc) return rc;
+    KMI_CHECK_ARG(E > 0 && E <= MAX_E, "%s: %lld experts (1..%lld)", what, (long long)E, (long long)MAX_E);
+    KMI_CHECK_ARG(X >= 1 && M >= 1 && P >= 0 && P < (1LL << 31) && M < (1LL << 31) && P * M < (1LL << 31) &&
+                  X < (1LL << 31) && X * M < (1LL << 31), "%s: too many rows", what);
+    if (P == 0) return OK;
+    KMI_CHECK_ARG(x && w && scales && lhs && rhs && y, "%s: null pointer", what);
+    const size_t need = kmi_gather_qmm_fp8_workspace_bytes(P, M, E, K, N, dtype);
+    if (!workspace || workspace_bytes < need) {
+        set_error("%s: workspace of %zu bytes needed, %zu given", what, need, workspace_bytes);
+        return EWORKSPACE;
+    }
+    const int tm = tile_rows(per_expert(P, M, E));
+    SortedRows sr;
+    hipStream_t st = (hipStream_t)stream;
+    rc = launch_sort_rows(rhs, P, M, (int)E, tm, workspace, (uint16_t*)y, N, st, &sr);
+    if (rc) return rc;
+    F8Args a = {};
+    a.w = (const unsigned char*)w; a.s = scales; a.e8 = e8m0; a.E = E; a.wrows = N; a.K = K; a.N = N;
+    a.x = x; a.xrows = X * M; a.y = y; a.rows = P * M; a.tm = tm;
+    a.tiles = sr.tiles; a.sorted = sr.sorted; a.lhs = lhs; a.lhs_div = 1; a.Mper = M;
+    return launch_fp8_skinny(a, dtype, false, sr.max_tiles, st);
+}
+
+size_t kmi_switch_glu_fp8_workspace_bytes(int64_t T, int64_t H, int64_t I, int k, int64_t E) {
+    if (T <= 0 || H <= 0 || I <= 0 || k <= 0 || E <= 0) return 0;
+    const int64_t P = T * k;
+    return align256((size_t)P * I * 2) + align256((size_t)P * H * 2) +
+           sort_index_bytes(P, E, tile_rows(per_expert(P, 1, E)));
+}
+
+int kmi_switch_glu_fp8(const void* x, int64_t T, int64_t H, int64_t I, int k, const int32_t* inds,
+                       const void* scores, const uint32_t* w_gu, const void* s_gu, const uint32_t* w_down,
+                       const void* s_down, int e8m0, int64_t E, int dtype, void* out, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+    clear_error();
+    const char* what = "switch_glu (fp8)";
+    KMI_CHECK_ARG(dtype == BF16, "%s: only bfloat16 activations are implemented", what);
+    int rc = check_operands(what, dtype, H, 2 * I, x, w_gu);
+    if (rc) return rc;
+    rc = check_operands(what, dtype, I, H, workspace, w_down);
+    if (rc) return rc;
+    KMI_CHECK_ARG(I % F8_BLOCK == 0, "%s: I=%lld (gate and up stack in whole blocks of 128)", what, (long long)I);
+    KMI_CHECK_ARG(k >= 1 && k <= 64 && E >= 1 && E <= MAX_E, "%s: top-%d of %lld experts", what, k, (long long)E);
+    KMI_CHECK_ARG(T >= 0 && T < (1LL << 31) && T * k < (1LL << 31), "%s: T=%lld", what, (long long)T);
+    if (T == 0) return OK;
+    KMI_CHECK_ARG(x && inds && w_gu && s_gu && w_down && s_down && out, "%s: null pointer", what);
+    const size_t need = kmi_switch_glu_fp8_workspace_bytes(T, H, I, k, E);
+    if (!workspace || workspace_bytes < need) {
+        set_error("%s: workspace of %zu bytes needed, %zu given", what, need, workspace_bytes);
+        return EWORKSPACE;
+    }
+    hipStream_t st = (hipStream_t)stream;
+    const int64_t P = T * k;
+    const int tm = tile_rows(per_expert(P, 1, E));
+    char* ws = (char*)workspace;
+    uint16_t* act = (uint16_t*)ws;
+    ws += align256((size_t)P * I * 2);
+    uint16_t* y = scores ? (uint16_t*)ws : (uint16_t*)out;
+    ws += align256((size_t)P * H * 2);
+    SortedRows sr;
+    rc = launch_sort_rows(inds, P, 1, (int)E, tm, ws, y, H, st, &sr);
+    if (rc) return rc;
+    F8Args g = {};
+    g.w = (const unsigned char*)w_gu; g.s = s_gu; g.e8 = e8m0; g.E = E; g.wrows = 2 * I; g.K = H; g.N = I;
+    g.x = x; g.xrows = T; g.y = act; g.rows = P; g.tm = tm;
+    g.tiles = sr.tiles; g.sorted = sr.sorted; g.lhs_div = k; g.Mper = 1;
+    rc = launch_fp8_skinny(g, dtype, true, sr.max_tiles, st);
+    if (rc) return rc;
+    F8Args d = g;
+    d.w = (const unsigned char*)w_down; d.s = s_down; d.wrows = H; d.K = I; d.N = H;
+    d.x = act; d.xrows = P; d.y = y; d.lhs_div = 1;
+    rc = launch_fp8_skinny(d, dtype, false, sr.max_tiles, st);
+    if (rc) return rc;
+    if (scores) return kmi_moe_combine(y, scores, dtype, T, k, H, out, stream);
+    return OK;
+}
+
+}  // extern "C"

@@ -24,9 +24,9 @@ import math
 
 import torch
 
-from .ops import (add_bias, gather_qmm, linear, moe_combine, moe_experts, moe_route,
-                  moe_shared_add, quantize, quantized_matmul, swiglu, switch_glu, switch_glu_mx, vq_gather_qmm,
-                  vq_experts, vq_glu, vq_packed_experts, vq_packed_gather_qmm, vq_packed_glu, vq_packed_switch_glu,
+from .ops import (FP8_BLOCK, _resolve, add_bias, gather_qmm, linear, moe_combine, moe_experts, moe_route,
+                  moe_shared_add, quantize, quantized_matmul, swiglu, switch_glu, switch_glu_fp8, switch_glu_mx,
+                  vq_gather_qmm, vq_experts, vq_glu, vq_packed_experts, vq_packed_gather_qmm, vq_packed_glu, vq_packed_switch_glu,
                   vq_switch_glu)
 
 
@@ -42,6 +42,20 @@ class Linear:
         return linear(x, self.weight, self.bias)
 
 
+def _from_float(cls, w, bias, group_size, bits, mode):
+    """cls over w quantized in ``mode`` (omitted group_size / bits: the mode's)."""
+    group_size, bits = _resolve(group_size, bits, mode)
+    wq, scales, *biases = quantize(w, group_size=group_size, bits=bits, mode=mode)
+    return cls(wq, scales, biases[0] if biases else None, bias, group_size, bits, mode)
+
+
+def _input_dims(layer):
+    # fp8's last block of inputs may be partial
+    if layer.mode == "fp8":
+        return layer.weight.shape[-1] * (1 if layer.weight.dtype == torch.float8_e4m3fn else 4)
+    return layer.scales.shape[-1] * layer.group_size
+
+
 class QuantizedLinear:
     """nn.QuantizedLinear: y = quantized_matmul(x, w, scales, biases) (+ bias)."""
 
@@ -51,12 +65,13 @@ class QuantizedLinear:
         self.group_size, self.bits, self.mode = group_size, bits, mode
 
     @classmethod
-    def from_float(cls, w: torch.Tensor, bias=None, group_size: int = 64, bits: int = 4):
-        return cls(*quantize(w, group_size=group_size, bits=bits), bias, group_size, bits)
+    def from_float(cls, w: torch.Tensor, bias=None, group_size: int | None = None, bits: int | None = None,
+                   mode: str = "affine"):
+        return _from_float(cls, w, bias, group_size, bits, mode)
 
     @property
     def input_dims(self):
-        return self.scales.shape[-1] * self.group_size
+        return _input_dims(self)
 
     @property
     def output_dims(self):
@@ -78,13 +93,14 @@ class QuantizedSwitchLinear:
         self.group_size, self.bits, self.mode = group_size, bits, mode
 
     @classmethod
-    def from_float(cls, w: torch.Tensor, bias=None, group_size: int = 64, bits: int = 4):
+    def from_float(cls, w: torch.Tensor, bias=None, group_size: int | None = None, bits: int | None = None,
+                   mode: str = "affine"):
         """w [E, N, K] -> the quantized layer (mx.quantize per expert row)."""
-        return cls(*quantize(w, group_size=group_size, bits=bits), bias, group_size, bits)
+        return _from_float(cls, w, bias, group_size, bits, mode)
 
     @property
     def input_dims(self):
-        return self.scales.shape[2] * self.group_size
+        return _input_dims(self)
 
     @property
     def output_dims(self):
@@ -104,6 +120,8 @@ class QuantizedSwitchLinear:
 
 
 def _stackable(a: QuantizedSwitchLinear, b: QuantizedSwitchLinear) -> bool:
+    if a.mode == "fp8" and a.output_dims % FP8_BLOCK:        # up's first block would straddle gate's last rows
+        return False
     return (a.weight.shape == b.weight.shape and a.scales.shape == b.scales.shape
             and a.group_size == b.group_size and a.bits == b.bits and a.bias is None
             and b.bias is None and a.weight.dtype == b.weight.dtype and a.scales.dtype == b.scales.dtype
@@ -133,20 +151,20 @@ class SwitchGLU:
                                                cat(gate_proj.scales, up_proj.scales),
                                                cat(gate_proj.biases, up_proj.biases),
                                                None, gate_proj.group_size, gate_proj.bits, mode)
-            I = gate_proj.output_dims
-            view = lambda t, lo: None if t is None else t[:, lo:lo + I]
-            self.gate_proj = QuantizedSwitchLinear(view(self.fused.weight, 0), view(self.fused.scales, 0),
-                                                   view(self.fused.biases, 0), None,
+            half = lambda t, up: None if t is None else t[:, t.shape[1] // 2:] if up else t[:, :t.shape[1] // 2]
+            self.gate_proj = QuantizedSwitchLinear(half(self.fused.weight, 0), half(self.fused.scales, 0),
+                                                   half(self.fused.biases, 0), None,
                                                    gate_proj.group_size, gate_proj.bits, mode)
-            self.up_proj = QuantizedSwitchLinear(view(self.fused.weight, I), view(self.fused.scales, I),
-                                                 view(self.fused.biases, I), None,
+            self.up_proj = QuantizedSwitchLinear(half(self.fused.weight, 1), half(self.fused.scales, 1),
+                                                 half(self.fused.biases, 1), None,
                                                  up_proj.group_size, up_proj.bits, mode)
         else:
             self.gate_proj, self.up_proj = gate_proj, up_proj
 
     @classmethod
-    def from_float(cls, gate_w, up_w, down_w, group_size: int = 64, bits: int = 4):
-        q = lambda w: QuantizedSwitchLinear.from_float(w, None, group_size, bits)
+    def from_float(cls, gate_w, up_w, down_w, group_size: int | None = None, bits: int | None = None,
+                   mode: str = "affine"):
+        q = lambda w: QuantizedSwitchLinear.from_float(w, None, group_size, bits, mode)
         return cls(q(gate_w), q(up_w), q(down_w))
 
     def _one_call(self, k: int) -> bool:
@@ -160,6 +178,12 @@ class SwitchGLU:
         return (f is not None and d.bias is None and k <= 8 and f.mode in ("mxfp4", "mxfp8")
                 and d.mode == f.mode and x.dtype == torch.bfloat16
                 and x.shape[-1] % 64 == 0 and (f.weight.shape[1] // 2) % 64 == 0)
+
+    def _one_call_fp8(self, x: torch.Tensor) -> bool:
+        """E4M3 experts in blocks of 128 in one call (kmi_switch_glu_fp8)."""
+        f, d = self.fused, self.down_proj
+        return (f is not None and d.bias is None and f.mode == "fp8" and d.mode == "fp8"
+                and d.scales.dtype == f.scales.dtype and x.dtype == torch.bfloat16)
 
     def __call__(self, x: torch.Tensor, indices: torch.Tensor) -> torch.Tensor:
         """x [..., H], indices [..., k] (int) -> [..., k, H]."""
@@ -178,6 +202,8 @@ class SwitchGLU:
                               scores, f.group_size, f.bits)
         if self._one_call_mx(x, k):
             return switch_glu_mx(x, indices, f.weight, f.scales, d.weight, d.scales, scores, f.mode)
+        if self._one_call_fp8(x):
+            return switch_glu_fp8(x, indices, f.weight, f.scales, d.weight, d.scales, scores)
         y = self.gathered(x, indices)
         return y if scores is None else moe_combine(y, scores)
 

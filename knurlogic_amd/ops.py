@@ -11,6 +11,7 @@ tensors' device and stream; nothing falls back to the CPU.
 """
 from __future__ import annotations
 
+import contextlib
 import math
 
 import torch
@@ -54,11 +55,15 @@ MODE_CODE = {"affine": 0, "mxfp4": 1, "mxfp8": 2}
 _MX_BITS = {"mxfp4": 4, "mxfp8": 8}
 
 
-def _check_mode(mode: str, allow_mx: bool = False):
-    if mode == "affine" or (allow_mx and mode in _MX_BITS):
+#: E4M3 weights with one scale per block of 128 x 128 (mode "fp8")
+FP8_BLOCK = 128
+
+
+def _check_mode(mode: str, allow_mx: bool = False, allow_fp8: bool = False):
+    if mode == "affine" or (allow_mx and mode in _MX_BITS) or (allow_fp8 and mode == "fp8"):
         return
     raise ValueError(f"mode {mode!r}: {'affine, mxfp4 and mxfp8 are' if allow_mx else 'only affine is'} "
-                     "implemented here")
+                     f"implemented here{' (and fp8)' if allow_fp8 else ''}")
 
 
 def _check_mx(what, scales, biases, group_size, bits, mode):
@@ -102,8 +107,10 @@ def _check_experts(what, H, E, w_gu, s_gu, b_gu, w_down, s_down, b_down, group_s
 
 
 def _resolve(group_size, bits, mode: str):
-    """mlx's mode-dependent defaults for an omitted group_size / bits: affine
-    64 and 4, mxfp4 32 and 4, mxfp8 32 and 8."""
+    """The mode's defaults for an omitted group_size / bits: affine 64 and 4,
+    mxfp4 32 and 4, mxfp8 32 and 8 (mlx's), fp8 128 and 8."""
+    if mode == "fp8":
+        return (FP8_BLOCK if group_size is None else int(group_size), 8 if bits is None else int(bits))
     if mode in _MX_BITS:
         return (32 if group_size is None else int(group_size),
                 _MX_BITS[mode] if bits is None else int(bits))
@@ -129,9 +136,12 @@ def quantize(w: torch.Tensor, group_size: int | None = None, bits: int | None = 
     [..., K/group_size]) in w's dtype, groups along the last axis (omitted
     group_size / bits: 64 and 4).  mxfp4 / mxfp8: (wq, scales uint8 E8M0),
     group 32 and 4 / 8 bits, which are also the only values taken (mlx
-    returns no biases)."""
-    _check_mode(mode, allow_mx=True)
+    returns no biases).  fp8: E4M3 codes and one uint8 E8M0 scale per block of
+    128 x 128 of w [..., N, K] (scales [..., ceil(N/128), ceil(K/128)])."""
+    _check_mode(mode, allow_mx=True, allow_fp8=True)
     group_size, bits = _resolve(group_size, bits, mode)
+    if mode == "fp8":
+        return _quantize_fp8(w, group_size, bits)
     if mode != "affine":
         if group_size != 32 or bits != _MX_BITS[mode]:
             raise ValueError(f"quantize: {mode} takes group_size 32 and {_MX_BITS[mode]} bits "
@@ -174,9 +184,13 @@ def dequantize(w: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor | Non
     """``mx.dequantize``: scale * q + bias in ``dtype`` (default: scales'
     dtype).  ``rounding`` picks the storage rounding order.  mxfp4 / mxfp8:
     element * 2^(scale - 127), uint8 E8M0 scales, no biases (default dtype
-    bfloat16).  Omitted group_size / bits take mlx's defaults for the mode."""
-    _check_mode(mode, allow_mx=True)
+    bfloat16).  fp8: element * its block's scale (float32, or uint8 E8M0),
+    in float32 and rounded to dtype (default bfloat16).  Omitted group_size /
+    bits take the mode's defaults."""
+    _check_mode(mode, allow_mx=True, allow_fp8=True)
     group_size, bits = _resolve(group_size, bits, mode)
+    if mode == "fp8":
+        return _dequantize_fp8(w, scales, biases, group_size, bits, dtype)
     if mode != "affine":
         _check_mx("dequantize", scales, biases, group_size, bits, mode)
         _on_gpu(w, scales)
@@ -259,9 +273,13 @@ def quantized_matmul(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor,
     What at 4 or 8 bits with transpose=True is the dense projection
     (kmi_qmm); a batched What (leading dimensions broadcast against x's),
     transpose=False or the 2, 3, 5 and 6-bit widths run kmi_qmm_batched.
-    Omitted group_size / bits take mlx's defaults for the mode."""
-    _check_mode(mode, allow_mx=True)
+    fp8 (kmi_qmm_fp8): What 2-D, transpose=True, x in bfloat16 or float16; x is
+    quantized to E4M3 as well, a power-of-two scale per row and 128 inputs.
+    Omitted group_size / bits take the mode's defaults."""
+    _check_mode(mode, allow_mx=True, allow_fp8=True)
     group_size, bits = _resolve(group_size, bits, mode)
+    if mode == "fp8":
+        return _qmm_fp8(x, w, scales, biases, transpose, group_size, bits)
     if transpose and w.ndim == 2 and mode != "affine":
         return _qmm_mx(x, w, scales, biases, group_size, bits, mode)
     if not transpose or w.ndim != 2 or bits not in (4, 8) or mode != "affine":
@@ -561,11 +579,14 @@ def gather_qmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor,
     Rows are grouped by expert on the GPU whatever ``sorted_indices`` says,
     so each routed expert's weights are read once.  The mxfp4 / mxfp8
     modes (uint8 E8M0 scales, no biases) run the batched kernel's gather
-    form, either orientation."""
-    _check_mode(mode, allow_mx=True)
+    form, either orientation.  fp8 (kmi_gather_qmm_fp8): transpose=True, x
+    quantized as in ``quantized_matmul``."""
+    _check_mode(mode, allow_mx=True, allow_fp8=True)
     group_size, bits = _resolve(group_size, bits, mode)
     if x.ndim < 2 or w.ndim < 3:
         raise ValueError("gather_qmm: x needs [..., M, K] and w [..., N, K*bits/32]")
+    if mode == "fp8":
+        return _gather_fp8(x, w, scales, biases, lhs_indices, rhs_indices, transpose, group_size, bits)
     if mode != "affine":
         _check_mx("gather_qmm", scales, biases, group_size, bits, mode)
         _on_gpu(x, w, scales)
@@ -837,6 +858,188 @@ def moe_experts(x: torch.Tensor, logits: torch.Tensor, k: int, w_gu, s_gu, b_gu,
                                  group_size, bits, _ptr(out), _ptr(inds), _ptr(scores), _ptr(ws), nbytes,
                                  _stream(x)), "moe_experts")
     return out, inds, scores
+
+
+# --- E4M3 weights with a scale per block of 128 x 128 -------------------------------
+
+def _one_device(what, *ts):
+    _on_gpu(*ts)
+    dev = ts[0].device
+    for t in ts[1:]:
+        if t is not None and t.device != dev:
+            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
+
+
+def _on(t: torch.Tensor):
+    """A context with t's device current (kernels launch on the current one)."""
+    return contextlib.nullcontext() if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _fp8_blocks(n: int) -> int:
+    return -(-n // FP8_BLOCK)
+
+
+def _fp8_codes(what, w):
+    """w [..., N, K/4] packed uint32 of an E4M3 weight given packed or as
+    float8_e4m3fn [..., N, K], contiguous on 16 bytes."""
+    if w.dtype == torch.float8_e4m3fn:
+        if w.ndim < 2 or w.shape[-1] % 16:
+            raise ValueError(f"{what}: w {tuple(w.shape)} needs inputs in multiples of 16")
+        return _aligned16(w.view(torch.uint8)).view(torch.uint32)
+    if w.dtype not in (torch.uint32, torch.int32):
+        raise ValueError(f"{what}: w must be packed uint32 or float8_e4m3fn (got {w.dtype})")
+    return _aligned16(w)
+
+
+def _check_fp8(what, w, scales, biases, group_size, bits):
+    """The format's rules; returns the packed codes, the scales and whether
+    they are E8M0 bytes."""
+    if biases is not None:
+        raise ValueError(f"{what}: fp8 has no biases")
+    if group_size != FP8_BLOCK or bits != 8:
+        raise ValueError(f"{what}: fp8 takes group_size {FP8_BLOCK} and 8 bits (got {group_size} and {bits})")
+    if scales.dtype not in (torch.float32, torch.uint8):
+        raise ValueError(f"{what}: fp8 scales are float32 or uint8 E8M0 exponents (got {scales.dtype})")
+    wq = _fp8_codes(what, w)
+    if wq.ndim < 2 or wq.shape[-1] % 4:
+        raise ValueError(f"{what}: w packs {tuple(wq.shape)} words; inputs come in multiples of 16")
+    want = (*wq.shape[:-2], _fp8_blocks(wq.shape[-2]), _fp8_blocks(wq.shape[-1] * 4))
+    if tuple(scales.shape) != want:
+        raise ValueError(f"{what}: scales {tuple(scales.shape)} for a [{wq.shape[-2]}, {wq.shape[-1] * 4}] fp8 "
+                         f"weight; expected {want}")
+    return wq, scales.contiguous(), int(scales.dtype == torch.uint8)
+
+
+def _quantize_fp8(w, group_size, bits):
+    if group_size != FP8_BLOCK or bits != 8:
+        raise ValueError(f"quantize: fp8 takes group_size {FP8_BLOCK} and 8 bits (got {group_size} and {bits})")
+    _on_gpu(w)
+    if w.dtype not in DTYPE_CODE or w.ndim < 2 or w.shape[-1] % 16:
+        raise ValueError("quantize: fp8 needs a bf16/fp16/fp32 tensor [..., N, K] with K a multiple of 16")
+    wc = _aligned16(w)
+    lead, (N, K) = tuple(w.shape[:-2]), w.shape[-2:]
+    wq = torch.empty(*lead, N, K // 4, dtype=torch.uint32, device=w.device)
+    sc = torch.empty(*lead, _fp8_blocks(N), _fp8_blocks(K), dtype=torch.uint8, device=w.device)
+    with _on(w):
+        _abi.check(_lib().kmi_quantize_fp8(_ptr(wc), DTYPE_CODE[w.dtype], math.prod(lead), N, K, _ptr(wq), _ptr(sc),
+                                           _stream(w)), "quantize")
+    return wq, sc
+
+
+def _dequantize_fp8(w, scales, biases, group_size, bits, dtype):
+    what = "dequantize"
+    wq, sc, e8 = _check_fp8(what, w, scales, biases, group_size, bits)
+    _one_device(what, wq, sc)
+    out_dtype = dtype or torch.bfloat16
+    if out_dtype not in DTYPE_CODE:
+        raise ValueError(f"{what}: dtype {out_dtype}")
+    lead, N, K = tuple(wq.shape[:-2]), wq.shape[-2], wq.shape[-1] * 4
+    out = torch.empty(*lead, N, K, dtype=out_dtype, device=wq.device)
+    with _on(wq):
+        _abi.check(_lib().kmi_dequantize_fp8(_ptr(wq), _ptr(sc), e8, math.prod(lead), N, K, _ptr(out),
+                                             DTYPE_CODE[out_dtype], _stream(wq)), what)
+    return out
+
+
+def _fp8_x(what, x, K):
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"{what}: fp8 products take bfloat16 or float16 x (got {x.dtype})")
+    if x.ndim < 1 or x.shape[-1] != K:
+        raise ValueError(f"{what}: x {tuple(x.shape)} for a weight of {K} inputs")
+    return _aligned16(x)
+
+
+def _qmm_fp8(x, w, scales, biases, transpose, group_size, bits):
+    what = "quantized_matmul"
+    if not transpose or w.ndim != 2:
+        raise ValueError(f"{what}: fp8 takes a 2-D weight with transpose=True (got {tuple(w.shape)}, "
+                         f"transpose={transpose})")
+    wq, sc, e8 = _check_fp8(what, w, scales, biases, group_size, bits)
+    N, K = wq.shape[0], wq.shape[1] * 4
+    _one_device(what, x, wq, sc)
+    xc = _fp8_x(what, x, K)
+    y = x.new_empty((*x.shape[:-1], N))
+    if y.numel() == 0:
+        return y
+    M = xc.numel() // K if K else 0
+    L = _lib()
+    code = DTYPE_CODE[x.dtype]
+    with _on(x):
+        nbytes = L.kmi_qmm_fp8_workspace_bytes(M, K, N, code)
+        ws = _workspace(nbytes, x.device)
+        _abi.check(L.kmi_qmm_fp8(_ptr(xc), M, K, N, _ptr(wq), _ptr(sc), e8, code, _ptr(y), _ptr(ws), nbytes,
+                                 _stream(x)), what)
+    return y
+
+
+def _gather_fp8(x, w, scales, biases, lhs_indices, rhs_indices, transpose, group_size, bits):
+    what = "gather_qmm"
+    if not transpose:
+        raise ValueError(f"{what}: fp8 weights are [..., N, K] (transpose=True)")
+    wq, sc, e8 = _check_fp8(what, w, scales, biases, group_size, bits)
+    N, K = wq.shape[-2], wq.shape[-1] * 4
+    _one_device(what, x, wq, sc)
+    xc = _fp8_x(what, x, K)
+    E, Xb, M = math.prod(wq.shape[:-2]), math.prod(x.shape[:-2]), x.shape[-2]
+    lhs, rhs, ishape = _flat_indices(x, wq, lhs_indices, rhs_indices)
+    P = lhs.numel()
+    y = torch.empty(*ishape, M, N, dtype=x.dtype, device=x.device)
+    if y.numel() == 0:
+        return y
+    L = _lib()
+    code = DTYPE_CODE[x.dtype]
+    with _on(x):
+        nbytes = L.kmi_gather_qmm_fp8_workspace_bytes(P, M, E, K, N, code)
+        ws = _workspace(nbytes, x.device)
+        _abi.check(L.kmi_gather_qmm_fp8(_ptr(xc), Xb, M, K, _ptr(wq), _ptr(sc), e8, E, N, _ptr(lhs), _ptr(rhs), P,
+                                        code, _ptr(y), _ptr(ws), nbytes, _stream(x)), what)
+    return y
+
+
+def switch_glu_fp8(x: torch.Tensor, indices: torch.Tensor, w_gu, s_gu, w_down, s_down,
+                   scores: torch.Tensor | None = None):
+    """``switch_glu`` for E4M3 experts with a scale per block of 128 x 128
+    (kmi_switch_glu_fp8): x [..., H] bf16 and the SwiGLU activations are
+    quantized to E4M3 (a power-of-two scale per row and 128 inputs) on their
+    way into the products; gate and up stacked per expert (w_gu [E, 2I, H/4],
+    s_gu [E, 2I/128, ceil(H/128)], I in multiples of 128), w_down [E, H, I/4].
+    The same results as ``gather_qmm``, ``swiglu``, ``gather_qmm`` and
+    ``moe_combine`` in turn."""
+    what = "switch_glu_fp8"
+    if x.dtype != torch.bfloat16:
+        raise ValueError(f"{what}: only bfloat16 activations are implemented")
+    wg, sg, e8 = _check_fp8(what, w_gu, s_gu, None, FP8_BLOCK, 8)
+    wd, sd, e8d = _check_fp8(what, w_down, s_down, None, FP8_BLOCK, 8)
+    if e8 != e8d:
+        raise ValueError(f"{what}: both weights' scales must be float32, or both uint8")
+    _one_device(what, x, indices, wg, sg, wd, sd, scores)
+    lead, H = tuple(x.shape[:-1]), x.shape[-1]
+    if indices.ndim < 1 or tuple(indices.shape[:-1]) != lead or indices.dtype.is_floating_point:
+        raise ValueError(f"{what}: integer indices [..., k] must match x [..., H]")
+    k = indices.shape[-1]
+    if wg.ndim != 3 or wd.ndim != 3:
+        raise ValueError(f"{what}: w_gu and w_down must be [E, rows, words]")
+    E, I = wg.shape[0], wd.shape[2] * 4
+    if tuple(wg.shape) != (E, 2 * I, H // 4) or tuple(wd.shape) != (E, H, I // 4) or H % 16 or I % FP8_BLOCK:
+        raise ValueError(f"{what}: w_gu {tuple(wg.shape)} and w_down {tuple(wd.shape)} for x of {H} features "
+                         f"(H in multiples of 16, I of {FP8_BLOCK})")
+    if scores is not None and (scores.shape != indices.shape or scores.dtype != x.dtype):
+        raise ValueError(f"{what}: scores must match indices in shape and x in dtype")
+    T = math.prod(lead)
+    out = torch.empty((*lead, H) if scores is not None else (*lead, k, H), dtype=x.dtype, device=x.device)
+    if T == 0 or k == 0:
+        return out.zero_()
+    xc = _aligned16(x)
+    ic = indices.reshape(T, k).to(torch.int32).contiguous()
+    kc = None if scores is None else scores.contiguous()
+    L = _lib()
+    with _on(x):
+        nbytes = L.kmi_switch_glu_fp8_workspace_bytes(T, H, I, k, E)
+        ws = _workspace(nbytes, x.device)
+        _abi.check(L.kmi_switch_glu_fp8(_ptr(xc), T, H, I, k, _ptr(ic), _ptr(kc), _ptr(wg), _ptr(sg), _ptr(wd),
+                                        _ptr(sd), e8, E, DTYPE_CODE[x.dtype], _ptr(out), _ptr(ws), nbytes,
+                                        _stream(x)), what)
+    return out
 
 
 # --- VQ codebook-decode experts ---------------------------------------------------
