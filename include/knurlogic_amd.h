@@ -313,7 +313,8 @@ int kmi_qmm_fp8(const void* x, int64_t M, int64_t K, int64_t N, const uint32_t* 
  * x [X, M, K], w [E, N, K/4], scales [E, ceil(N/128), ceil(K/128)], E <= 4096.
  * Rows are grouped by expert on the GPU.  An index out of range gives a zero row.
  */
-size_t kmi_gather_qmm_fp8_workspace_bytes(int64_t P, int64_t M, int64_t E, int64_t K, int64_t N, int dtype);
+size_t kmi_gather_qmm_fp8_workspace_bytes(int64_t P, int64_t X, int64_t M, int64_t E, int64_t K, int64_t N,
+                                          int dtype);
 int kmi_gather_qmm_fp8(const void* x, int64_t X, int64_t M, int64_t K, const uint32_t* w, const void* scales,
                        int e8m0, int64_t E, int64_t N, const int32_t* lhs, const int32_t* rhs, int64_t P, int dtype,
                        void* y, void* workspace, size_t workspace_bytes, void* stream);

@@ -74,7 +74,7 @@ SIGNATURES = {
     "kmi_qmm_fp8": (I, [P, I64, I64, I64, P, P, I, I, P, P, SZ, P]),
     "kmi_qmm_fp8_workspace_bytes": (SZ, [I64, I64, I64, I]),
     "kmi_gather_qmm_fp8": (I, [P, I64, I64, I64, P, P, I, I64, I64, P, P, I64, I, P, P, SZ, P]),
-    "kmi_gather_qmm_fp8_workspace_bytes": (SZ, [I64, I64, I64, I64, I64, I]),
+    "kmi_gather_qmm_fp8_workspace_bytes": (SZ, [I64, I64, I64, I64, I64, I64, I]),
     "kmi_switch_glu_fp8": (I, [P, I64, I64, I64, I, P, P, P, P, P, P, I, I64, I, P, P, SZ, P]),
     "kmi_switch_glu_fp8_workspace_bytes": (SZ, [I64, I64, I64, I, I64]),
     "kmi_read_probe": (I, [P, I64, I, P, P]),

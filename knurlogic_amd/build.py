@@ -25,7 +25,8 @@ FLAGS = [
 # (MoE 16 tokens 67.5 -> 64.9 us, 256 tokens 153.6 -> 148.2; KV8 64 rows at
 # D = 512 97.4 -> 80.2; the GEMMs and the VQ kernels measured even or slower
 # with it, and keep their accumulators in AGPRs).
-EXTRA = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for f in ("qgemv.hip", "qgemv_xs.hip", "qgemv_dl.hip", "kv8.hip")}
+EXTRA = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for f in ("qgemv.hip", "qgemv_xs.hip", "qgemv_dl.hip", "kv8.hip",
+                                                                  "fp8_skinny.hip", "fp8_gemm.hip")}
 
 
 # The compiler's per-kernel resource remarks (registers, scratch, occupancy),

@@ -21,10 +21,45 @@ int check_operands(const char* what, int dtype, int64_t K, int64_t N, const void
     return OK;
 }
 
-// rows per tile: 16, or 32 / 64 where an active expert has more
-int tile_rows(int64_t per) { return per <= 16 ? 16 : per <= 32 ? 32 : 64; }
+int check_workspace(const char* what, size_t need, const void* ws, size_t bytes) {
+    if (need && (!ws || bytes < need)) {
+        set_error("%s: workspace of %zu bytes needed, %zu given", what, need, bytes);
+        return EWORKSPACE;
+    }
+    KMI_CHECK_ARG(((uintptr_t)ws & 15) == 0, "%s: workspace on 16 bytes", what);
+    return OK;
+}
 
-int64_t per_expert(int64_t P, int64_t M, int64_t E) { return ceil_div(P * M, P < E ? P : E); }
+// How a call runs: on f8_skinny, which quantizes x itself, or with x quantized
+// ahead on f8_gemm's tiles; and the rows per tile.
+struct Plan {
+    bool gemm;
+    int tm;
+};
+
+Plan plan_dense(int64_t M, int64_t K) {
+    if (M <= 64 || K > FP8_GEMM_MAX_K) return {false, M <= 16 ? 16 : M <= 32 ? 32 : 64};
+    return {true, 128};
+}
+
+// rows grouped by expert: by the average rows of an active one
+Plan plan_grouped(int64_t rows, int64_t P, int64_t E, int64_t K, bool glu) {
+    const int64_t per = ceil_div(rows, P < E ? P : E);
+    if (per <= 16 || K > FP8_GEMM_MAX_K) return {false, per <= 16 ? 16 : per <= 32 ? 32 : 64};
+    return {true, glu || per <= 64 ? 64 : 128};
+}
+
+size_t rows_bytes(int64_t rows, int64_t K, bool half) {
+    return align256((size_t)rows * fp8_row_bytes(K, half)) + align256((size_t)rows * fp8_row_scales(K));
+}
+
+// x quantized at ws (rows_bytes), as a's x
+int quantize_rows(F8Args& a, const void* x, int dtype, int64_t rows, bool half, char* ws, hipStream_t st) {
+    unsigned char* q = (unsigned char*)ws;
+    unsigned char* s = q + align256((size_t)rows * fp8_row_bytes(a.K, half));
+    a.x = q; a.xrows = rows; a.xld = fp8_row_bytes(a.K, half); a.xs = s; a.xs_ld = fp8_row_scales(a.K);
+    return launch_fp8_rows(x, dtype, rows, a.K, half, q, s, st);
+}
 
 }  // namespace
 
@@ -34,7 +69,10 @@ using namespace kmi;
 
 extern "C" {
 
-size_t kmi_qmm_fp8_workspace_bytes(int64_t M, int64_t K, int64_t N, int dtype) { return 0; }
+size_t kmi_qmm_fp8_workspace_bytes(int64_t M, int64_t K, int64_t N, int dtype) {
+    if (M <= 0 || K <= 0 || N <= 0 || !plan_dense(M, K).gemm) return 0;
+    return rows_bytes(M, K, false);
+}
 
 int kmi_qmm_fp8(const void* x, int64_t M, int64_t K, int64_t N, const uint32_t* w, const void* scales, int e8m0,
                 int dtype, void* y, void* workspace, size_t workspace_bytes, void* stream) {
@@ -45,15 +83,23 @@ int kmi_qmm_fp8(const void* x, int64_t M, int64_t K, int64_t N, const uint32_t* 
     KMI_CHECK_ARG(M >= 0 && M < (1 << 21), "%s: M=%lld", what, (long long)M);
     if (M == 0) return OK;
     KMI_CHECK_ARG(x && w && scales && y, "%s: null pointer", what);
+    rc = check_workspace(what, kmi_qmm_fp8_workspace_bytes(M, K, N, dtype), workspace, workspace_bytes);
+    if (rc) return rc;
+    const Plan p = plan_dense(M, K);
+    hipStream_t st = (hipStream_t)stream;
     F8Args a = {};
     a.w = (const unsigned char*)w; a.s = scales; a.e8 = e8m0; a.E = 1; a.wrows = N; a.K = K; a.N = N;
-    a.x = x; a.xrows = M; a.y = y; a.rows = M; a.tm = tile_rows(M);
-    return launch_fp8_skinny(a, dtype, false, ceil_div(M, a.tm), (hipStream_t)stream);
+    a.x = x; a.xrows = M; a.y = y; a.rows = M; a.tm = p.tm; a.half = dtype == F16;
+    if (!p.gemm) return launch_fp8_skinny(a, dtype, false, ceil_div(M, a.tm), st);
+    rc = quantize_rows(a, x, dtype, M, false, (char*)workspace, st);
+    return rc ? rc : launch_fp8_gemm(a, false, ceil_div(M, a.tm), st);
 }
 
-size_t kmi_gather_qmm_fp8_workspace_bytes(int64_t P, int64_t M, int64_t E, int64_t K, int64_t N, int dtype) {
-    if (P <= 0 || M <= 0 || E <= 0 || K <= 0 || N <= 0) return 0;
-    return sort_index_bytes(P * M, E, tile_rows(per_expert(P, M, E)));
+size_t kmi_gather_qmm_fp8_workspace_bytes(int64_t P, int64_t X, int64_t M, int64_t E, int64_t K, int64_t N,
+                                          int dtype) {
+    if (P <= 0 || X <= 0 || M <= 0 || E <= 0 || K <= 0 || N <= 0) return 0;
+    const Plan p = plan_grouped(P * M, P, E, K, false);
+    return sort_index_bytes(P * M, E, p.tm) + (p.gemm ? rows_bytes(X * M, K, false) : 0);
 }
 
 int kmi_gather_qmm_fp8(const void* x, int64_t X, int64_t M, int64_t K, const uint32_t* w, const void* scales,
@@ -68,28 +114,30 @@ int kmi_gather_qmm_fp8(const void* x, int64_t X, int64_t M, int64_t K, const uin
                   X < (1LL << 31) && X * M < (1LL << 31), "%s: too many rows", what);
     if (P == 0) return OK;
     KMI_CHECK_ARG(x && w && scales && lhs && rhs && y, "%s: null pointer", what);
-    const size_t need = kmi_gather_qmm_fp8_workspace_bytes(P, M, E, K, N, dtype);
-    if (!workspace || workspace_bytes < need) {
-        set_error("%s: workspace of %zu bytes needed, %zu given", what, need, workspace_bytes);
-        return EWORKSPACE;
-    }
-    const int tm = tile_rows(per_expert(P, M, E));
+    const Plan p = plan_grouped(P * M, P, E, K, false);
+    KMI_CHECK_ARG(!p.gemm || X * M * fp8_row_bytes(K, false) < (1LL << 31), "%s: x past 2 GiB of codes", what);
+    rc = check_workspace(what, kmi_gather_qmm_fp8_workspace_bytes(P, X, M, E, K, N, dtype), workspace,
+                         workspace_bytes);
+    if (rc) return rc;
     SortedRows sr;
     hipStream_t st = (hipStream_t)stream;
-    rc = launch_sort_rows(rhs, P, M, (int)E, tm, workspace, (uint16_t*)y, N, st, &sr);
+    rc = launch_sort_rows(rhs, P, M, (int)E, p.tm, workspace, (uint16_t*)y, N, st, &sr);
     if (rc) return rc;
     F8Args a = {};
     a.w = (const unsigned char*)w; a.s = scales; a.e8 = e8m0; a.E = E; a.wrows = N; a.K = K; a.N = N;
-    a.x = x; a.xrows = X * M; a.y = y; a.rows = P * M; a.tm = tm;
+    a.x = x; a.xrows = X * M; a.y = y; a.rows = P * M; a.tm = p.tm; a.half = dtype == F16;
     a.tiles = sr.tiles; a.sorted = sr.sorted; a.lhs = lhs; a.lhs_div = 1; a.Mper = M;
-    return launch_fp8_skinny(a, dtype, false, sr.max_tiles, st);
+    if (!p.gemm) return launch_fp8_skinny(a, dtype, false, sr.max_tiles, st);
+    rc = quantize_rows(a, x, dtype, X * M, false, (char*)workspace + sort_index_bytes(P * M, E, p.tm), st);
+    return rc ? rc : launch_fp8_gemm(a, false, sr.max_tiles, st);
 }
 
 size_t kmi_switch_glu_fp8_workspace_bytes(int64_t T, int64_t H, int64_t I, int k, int64_t E) {
     if (T <= 0 || H <= 0 || I <= 0 || k <= 0 || E <= 0) return 0;
     const int64_t P = T * k;
-    return align256((size_t)P * I * 2) + align256((size_t)P * H * 2) +
-           sort_index_bytes(P, E, tile_rows(per_expert(P, 1, E)));
+    const Plan p = plan_grouped(P, P, E, H > I ? H : I, true);
+    return align256((size_t)P * H * 2) + sort_index_bytes(P, E, p.tm) +
+           (p.gemm ? rows_bytes(T, H, true) + rows_bytes(P, I, false) : align256((size_t)P * I * 2));
 }
 
 int kmi_switch_glu_fp8(const void* x, int64_t T, int64_t H, int64_t I, int k, const int32_t* inds,
@@ -108,32 +156,42 @@ int kmi_switch_glu_fp8(const void* x, int64_t T, int64_t H, int64_t I, int k, co
     KMI_CHECK_ARG(T >= 0 && T < (1LL << 31) && T * k < (1LL << 31), "%s: T=%lld", what, (long long)T);
     if (T == 0) return OK;
     KMI_CHECK_ARG(x && inds && w_gu && s_gu && w_down && s_down && out, "%s: null pointer", what);
-    const size_t need = kmi_switch_glu_fp8_workspace_bytes(T, H, I, k, E);
-    if (!workspace || workspace_bytes < need) {
-        set_error("%s: workspace of %zu bytes needed, %zu given", what, need, workspace_bytes);
-        return EWORKSPACE;
-    }
-    hipStream_t st = (hipStream_t)stream;
     const int64_t P = T * k;
-    const int tm = tile_rows(per_expert(P, 1, E));
+    const Plan p = plan_grouped(P, P, E, H > I ? H : I, true);
+    KMI_CHECK_ARG(!p.gemm || (T * fp8_row_bytes(H, true) < (1LL << 31) && P * I < (1LL << 31)),
+                  "%s: activations past 2 GiB", what);
+    rc = check_workspace(what, kmi_switch_glu_fp8_workspace_bytes(T, H, I, k, E), workspace, workspace_bytes);
+    if (rc) return rc;
+    hipStream_t st = (hipStream_t)stream;
     char* ws = (char*)workspace;
-    uint16_t* act = (uint16_t*)ws;
-    ws += align256((size_t)P * I * 2);
     uint16_t* y = scores ? (uint16_t*)ws : (uint16_t*)out;
     ws += align256((size_t)P * H * 2);
     SortedRows sr;
-    rc = launch_sort_rows(inds, P, 1, (int)E, tm, ws, y, H, st, &sr);
+    rc = launch_sort_rows(inds, P, 1, (int)E, p.tm, ws, y, H, st, &sr);
     if (rc) return rc;
+    ws += sort_index_bytes(P, E, p.tm);
     F8Args g = {};
     g.w = (const unsigned char*)w_gu; g.s = s_gu; g.e8 = e8m0; g.E = E; g.wrows = 2 * I; g.K = H; g.N = I;
-    g.x = x; g.xrows = T; g.y = act; g.rows = P; g.tm = tm;
+    g.x = x; g.xrows = T; g.rows = P; g.tm = p.tm;
     g.tiles = sr.tiles; g.sorted = sr.sorted; g.lhs_div = k; g.Mper = 1;
-    rc = launch_fp8_skinny(g, dtype, true, sr.max_tiles, st);
-    if (rc) return rc;
     F8Args d = g;
-    d.w = (const unsigned char*)w_down; d.s = s_down; d.wrows = H; d.K = I; d.N = H;
-    d.x = act; d.xrows = P; d.y = y; d.lhs_div = 1;
-    rc = launch_fp8_skinny(d, dtype, false, sr.max_tiles, st);
+    d.w = (const unsigned char*)w_down; d.s = s_down; d.wrows = H; d.K = I; d.N = H; d.xrows = P; d.y = y;
+    d.lhs_div = 1;
+    if (p.gemm) {
+        rc = quantize_rows(g, x, dtype, T, true, ws, st);
+        if (rc) return rc;
+        ws += rows_bytes(T, H, true);
+        d.x = g.y = ws; d.xld = I; d.xs_ld = g.ys_ld = fp8_row_scales(I);
+        d.xs = g.ys = (unsigned char*)ws + align256((size_t)P * I);
+        rc = launch_fp8_gemm(g, true, sr.max_tiles, st);
+        if (rc) return rc;
+        rc = launch_fp8_gemm(d, false, sr.max_tiles, st);
+    } else {
+        d.x = g.y = ws;
+        rc = launch_fp8_skinny(g, dtype, true, sr.max_tiles, st);
+        if (rc) return rc;
+        rc = launch_fp8_skinny(d, dtype, false, sr.max_tiles, st);
+    }
     if (rc) return rc;
     if (scores) return kmi_moe_combine(y, scores, dtype, T, k, H, out, stream);
     return OK;

@@ -35,10 +35,32 @@ struct F8Args {
     const int32_t* lhs;
     int64_t lhs_div, Mper;
     int tm;
+    // launch_fp8_gemm: x is rows of codes as launch_fp8_rows writes them (xld
+    // bytes each) with scale bytes xs [xrows, xs_ld]; gate|up writes codes y
+    // [rows, N] and scale bytes ys [rows, ys_ld] of the activations
+    int64_t xld;
+    const unsigned char* xs;
+    int64_t xs_ld;
+    unsigned char* ys;
+    int64_t ys_ld;
+    int half;                   // y is float16
 };
 
 // tiles of up to a.tm (16, 32 or 64) rows; dtype BF16 or F16
 int launch_fp8_skinny(const F8Args& a, int dtype, bool glu, int64_t tiles, hipStream_t st);
+
+// Rows quantized ahead: codes in rows of fp8_row_bytes (a multiple of 128, the
+// tail zero; half: the codes' values in float16) and scale bytes in rows of
+// fp8_row_scales.
+int64_t fp8_row_bytes(int64_t K, bool half);
+int64_t fp8_row_scales(int64_t K);
+int launch_fp8_rows(const void* x, int dtype, int64_t rows, int64_t K, bool half, unsigned char* q, unsigned char* s,
+                    hipStream_t st);
+// K past which the row scales of a tile (128 bytes a block) crowd the LDS
+constexpr int64_t FP8_GEMM_MAX_K = 65536;
+// tiles of up to a.tm (64 or 128; gate|up 64) rows over such rows; gate|up takes
+// its x in float16
+int launch_fp8_gemm(const F8Args& a, bool glu, int64_t tiles, hipStream_t st);
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef short s16x2 __attribute__((ext_vector_type(2)));
@@ -56,6 +78,18 @@ __device__ __forceinline__ uint32_t f8_scale_byte(uint32_t amax_bits) {
 
 __device__ __forceinline__ f32x4 f8_mfma(i32x8 a, i32x8 b, f32x4 c, uint32_t sa, uint32_t sb) {
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, (int)sa, 0, (int)sb);
+}
+
+__device__ __forceinline__ i32x8 f8_operand(u32x4 lo, u32x4 hi) {
+    return i32x8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
+}
+
+// the same with B's scale in byte `at` (a constant) of sb
+__device__ __forceinline__ f32x4 f8_mfma_at(i32x8 a, i32x8 b, f32x4 c, uint32_t sa, uint32_t sb, int at) {
+    if (at == 0) return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, (int)sa, 0, (int)sb);
+    if (at == 1) return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, (int)sa, 1, (int)sb);
+    if (at == 2) return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, (int)sa, 2, (int)sb);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, (int)sa, 3, (int)sb);
 }
 
 // max over the four lanes l, l ^ 16, l ^ 32, l ^ 48

@@ -989,7 +989,7 @@ def _gather_fp8(x, w, scales, biases, lhs_indices, rhs_indices, transpose, group
     L = _lib()
     code = DTYPE_CODE[x.dtype]
     with _on(x):
-        nbytes = L.kmi_gather_qmm_fp8_workspace_bytes(P, M, E, K, N, code)
+        nbytes = L.kmi_gather_qmm_fp8_workspace_bytes(P, Xb, M, E, K, N, code)
         ws = _workspace(nbytes, x.device)
         _abi.check(L.kmi_gather_qmm_fp8(_ptr(xc), Xb, M, K, _ptr(wq), _ptr(sc), e8, E, N, _ptr(lhs), _ptr(rhs), P,
                                         code, _ptr(y), _ptr(ws), nbytes, _stream(x)), what)
