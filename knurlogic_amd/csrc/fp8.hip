@@ -39,14 +39,14 @@ struct Plan {
 
 Plan plan_dense(int64_t M, int64_t K) {
     if (M <= 64 || K > FP8_GEMM_MAX_K) return {false, M <= 16 ? 16 : M <= 32 ? 32 : 64};
-    return {true, 128};
+    return {true, M <= 128 ? 128 : 256};
 }
 
 // rows grouped by expert: by the average rows of an active one
 Plan plan_grouped(int64_t rows, int64_t P, int64_t E, int64_t K, bool glu) {
     const int64_t per = ceil_div(rows, P < E ? P : E);
     if (per <= 16 || K > FP8_GEMM_MAX_K) return {false, per <= 16 ? 16 : per <= 32 ? 32 : 64};
-    return {true, glu || per <= 64 ? 64 : 128};
+    return {true, !glu && per <= 64 ? 64 : 128};
 }
 
 size_t rows_bytes(int64_t rows, int64_t K, bool half) {

@@ -58,7 +58,7 @@ int launch_fp8_rows(const void* x, int dtype, int64_t rows, int64_t K, bool half
                     hipStream_t st);
 // K past which the row scales of a tile (128 bytes a block) crowd the LDS
 constexpr int64_t FP8_GEMM_MAX_K = 65536;
-// tiles of up to a.tm (64 or 128; gate|up 64) rows over such rows; gate|up takes
+// tiles of up to a.tm (64, 128 or 256; gate|up 128) rows over such rows; gate|up takes
 // its x in float16
 int launch_fp8_gemm(const F8Args& a, bool glu, int64_t tiles, hipStream_t st);
 

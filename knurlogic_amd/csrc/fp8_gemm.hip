@@ -1,24 +1,27 @@
-// Block-scaled E4M3 products of many rows, on tiles of 256 weight rows x up to
-// 128 activation rows (gate|up: 128 gate and 128 up rows x up to 64).
+// Block-scaled E4M3 products of many rows: tiles of 256 weight rows (gate|up: 128
+// gate and 128 up rows) x 64 to 256 activation rows.
 //
-// The rows of x are quantized by a pass before (fp8_rows).  A workgroup's 4
-// waves take 64 weight rows each and all of the tile's activation rows: weights
-// go from memory into the matrix operand as they are, one 128-input block
-// ahead, and only x, which every wave reads, passes through LDS (direct-to-LDS
-// loads, one block ahead; rows of 128 bytes with their 16-byte pieces permuted
-// by the row, so 8 rows' reads fall on distinct banks).  D holds activation rows
-// along its columns, so a lane has one row's scale per 16 x 16 tile.
+// The rows of x are quantized by a pass before (f8_rows).  4 or 8 waves take 64
+// weight rows x MB 16-row blocks of activations each.  Both operands arrive by
+// direct-to-LDS loads, S blocks of 128 inputs in a ring: 8 lanes take the 128
+// bytes of a row (straight into the operand, a lane per row, the address units
+// handled a lane at a time: 4900 of 6300 cycles per block), their 16-byte pieces
+// permuted by the row, so that 8 rows' reads fall on distinct banks.  The
+// barrier of a block stands before its last products, where all of its LDS reads
+// are done: those products run while the next block's first fragments are read.
+// D holds activation rows along its columns, so a lane has one row's scale per
+// 16 x 16 tile.
 #include "fp8.hpp"
 
 namespace kmi {
 
 namespace {
 
-#define KMI_F8_LDS(p) ((__attribute__((address_space(3))) void*)(p))
+#define KMI_F8_LDS(p) ((__attribute__((address_space(3))) unsigned char*)(p))
 
-constexpr int G_WAVES = 4;
-constexpr int G_STAGES = 2;
 constexpr uint32_t G_NONE = 0x80000000u;     // past every view: reads 0
+constexpr int G_WTILE = 256 * F8_BLOCK;      // a block's weights in LDS
+constexpr int G_CHUNK = 64;                  // blocks whose scales are held at a time
 
 // how weights and x meet: E4M3 operands with both scales applied to each
 // block's sums in float32 (weights' scales in float32), or by the instruction
@@ -27,30 +30,41 @@ enum Kind { F32S, E8S, HALF };
 
 template <int N_>
 __device__ __forceinline__ void g_wait() {
+    static_assert(N_ >= 0 && N_ < 64, "vmcnt");
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N_) : "memory");
 }
 
 // 16 bytes per lane from the view's offset into LDS at dst + 16 lane.  In asm, as
 // the compiler would wait for the load before any later read of LDS; the kernel
-// waits for it itself (g_wait), and its own counts, which miss these loads, only
-// wait for more.
+// waits for it itself (g_wait), and the compiler's own counts, which miss these
+// loads, only wait for more.
 __device__ __forceinline__ void g_dma16(__amdgpu_buffer_rsrc_t r, unsigned char* dst, uint32_t voff, uint32_t soff) {
-    const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)dst;
+    const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)KMI_F8_LDS(dst));
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                  ::"s"(at), "v"(voff), "s"(r), "s"(soff) : "memory", "m0");
 }
 
-template <int MB, Kind KIND, bool GLU>
-__global__ __launch_bounds__(64 * G_WAVES, 2) void f8_gemm(F8Args a, int nblocks, int tiles) {
-    constexpr int TM = 16 * MB, RB = 4;
-    constexpr int XB = KIND == HALF ? 256 : 128;              // bytes of a row's block in LDS
-    constexpr int PER = TM * XB / 1024 / G_WAVES;             // direct-to-LDS loads per wave and block
-    constexpr int STAGE = TM * XB;
-    static_assert(PER * 1024 * G_WAVES == STAGE, "whole loads per wave");
+// WM waves beside each other along the activation rows, MB 16-row blocks each
+template <Kind KIND, int MB, int WM, int S>
+struct Shape {
+    static constexpr int TM = 16 * MB * WM, WAVES = 4 * WM;
+    static constexpr int XB = KIND == HALF ? 256 : 128;       // bytes of a row's block
+    static constexpr int STAGE = G_WTILE + TM * XB;
+    static constexpr int XL = TM * XB / 1024 / WAVES, WL = G_WTILE / 1024 / WAVES;   // loads per wave and block
+    static constexpr int SCALES = G_CHUNK * TM;
+    static constexpr int LDS = S * STAGE + SCALES;
+    static_assert(XL * 1024 * WAVES == TM * XB, "whole loads per wave");
+};
+
+template <Kind KIND, int MB, int WM, int S, bool GLU>
+__global__ __launch_bounds__(256 * WM, 2 / WM) void f8_gemm(F8Args a, int nblocks, int tiles) {
+    typedef Shape<KIND, MB, WM, S> Z;
+    constexpr int RB = 4, TM = Z::TM, XB = Z::XB, XL = Z::XL, WL = Z::WL, WAVES = Z::WAVES;
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ int rid_s[TM];
+    unsigned char* const sc = smem + S * Z::STAGE;            // [G_CHUNK][WM][16][MB] scale bytes
     const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave & 3, wm = wave >> 2;
     const int l16 = lane & 15, c = lane >> 4;
     // workgroup -> (tile, column block).  Workgroups go to the 8 XCDs in turn, and
     // an XCD's neighbours should share weights and x in its L2.  Dense: each XCD
@@ -80,10 +94,7 @@ __global__ __launch_bounds__(64 * G_WAVES, 2) void f8_gemm(F8Args a, int nblocks
     if (count <= 0) return;
 
     const int K = (int)a.K, KB = (K + F8_BLOCK - 1) / F8_BLOCK;
-    const int64_t xld = a.xld;                                // bytes per x row
-    // x rows of the tile; its view starts at row x0
-    const int64_t x0 = a.tiles ? 0 : start;
-    unsigned char* sc = smem + G_STAGES * STAGE;              // [KB][16][8] scale bytes
+    const int64_t x0 = a.tiles ? 0 : start;                   // the x view's first row
     auto xrow = [&](int m) -> int64_t {                       // x row of tile row m, or -1
         if (m >= count) return -1;
         if (!a.tiles) return start + m;
@@ -93,47 +104,51 @@ __global__ __launch_bounds__(64 * G_WAVES, 2) void f8_gemm(F8Args a, int nblocks
         const int64_t r = b * a.Mper + rid % (int)a.Mper;
         return b >= 0 && r < a.xrows ? r : -1;
     };
-    const __amdgpu_buffer_rsrc_t rx = make_rsrc((const unsigned char*)a.x + x0 * xld, (a.xrows - x0) * xld);
-    uint32_t xoff[PER];
+    // direct-to-LDS loads: 8 (float16: 16) lanes per row, the lane's piece
+    // permuted by the row
+    const __amdgpu_buffer_rsrc_t rx = make_rsrc((const unsigned char*)a.x + x0 * a.xld, (a.xrows - x0) * a.xld);
+    uint32_t xoff[XL], woff[WL];
 #pragma unroll
-    for (int j = 0; j < PER; j++) {
-        constexpr int LPR = XB / 16;                          // lanes per row
-        const int m = (64 / LPR) * (wave + G_WAVES * j) + lane / LPR;
+    for (int j = 0; j < XL; j++) {
+        constexpr int LPR = XB / 16;
+        const int m = (64 / LPR) * (wave + WAVES * j) + lane / LPR;
         const int64_t r = xrow(m);
-        xoff[j] = r < 0 ? G_NONE : (uint32_t)((r - x0) * xld) + 16u * ((lane % LPR) ^ (m & 7));
+        xoff[j] = r < 0 ? G_NONE : (uint32_t)((r - x0) * a.xld) + 16u * ((lane % LPR) ^ (m & 7));
     }
-    auto issue_x = [&](int t) {
-        unsigned char* dst = smem + (t & 1) * STAGE;
+    // weight rows of the tile: row 64 v + 16 i + l of wave column v's fragment i
+    // (gate|up: fragments 0, 1 the gate rows 32 v .., 2, 3 the up rows)
+    const int64_t n0 = (int64_t)nb * (GLU ? 128 : 256);
+    const int64_t left = a.N - n0 < (GLU ? 128 : 256) ? a.N - n0 : (GLU ? 128 : 256);
+    const __amdgpu_buffer_rsrc_t rw = make_rsrc(a.w + (expert * a.wrows + n0) * a.K, left * a.K);
+    const __amdgpu_buffer_rsrc_t ru = make_rsrc(a.w + (expert * a.wrows + n0 + (GLU ? a.N : 0)) * a.K, left * a.K);
+    const int piece = (lane & 7) ^ (lane >> 3);               // row % 8 == lane / 8
 #pragma unroll
-        for (int j = 0; j < PER; j++)
-            g_dma16(rx, dst + (wave + G_WAVES * j) * 1024, t < KB ? xoff[j] : G_NONE, (uint32_t)t * XB);
+    for (int j = 0; j < WL; j++) {
+        const int m = 8 * (wave + WAVES * j) + (lane >> 3);
+        const int r = GLU ? (m >> 6) * 32 + (m & 31) : m;     // (bit 5 of m: up)
+        woff[j] = r < left ? (uint32_t)r * (uint32_t)K + 16u * piece : G_NONE;
+    }
+    auto issue = [&](int t) {                                 // block t (past the last: zeros)
+        unsigned char* dst = smem + (t % S) * Z::STAGE;
+        const bool in = t * F8_BLOCK + 16 * piece < K;        // inputs past the last: zeros
+#pragma unroll
+        for (int j = 0; j < WL; j++) {
+            const int m = 8 * (wave + WAVES * j);
+            g_dma16(GLU && (m & 32) ? ru : rw, dst + m * F8_BLOCK, in ? woff[j] : G_NONE, (uint32_t)t * F8_BLOCK);
+        }
+#pragma unroll
+        for (int j = 0; j < XL; j++)
+            g_dma16(rx, dst + G_WTILE + (wave + WAVES * j) * 1024, t < KB ? xoff[j] : G_NONE, (uint32_t)t * XB);
     };
-    // a wave's weights: rows 16 i + l16 of its 64 (gate|up: fragments 0, 1 of the
-    // gate rows, 2, 3 of the up rows); rows past the last read zeros
-    const int64_t n0 = GLU ? (int64_t)nb * 128 + 32 * wave : (int64_t)nb * 256 + 64 * wave;
+#pragma unroll
+    for (int t = 0; t < S; t++) issue(t);
+    // the weights' scales of the wave's rows, 64 blocks, one per lane (gate|up:
+    // gate, up), and the scale bytes of x's rows
     const int64_t SB = (a.wrows + F8_BLOCK - 1) / F8_BLOCK;
-    int64_t left = a.N - n0;
-    left = left < 0 ? 0 : left > (GLU ? 32 : 64) ? (GLU ? 32 : 64) : left;
-    const unsigned char* wbase = a.w + (expert * a.wrows + (left ? n0 : 0)) * a.K;
-    const __amdgpu_buffer_rsrc_t rw = make_rsrc(wbase, left * a.K);
-    const __amdgpu_buffer_rsrc_t ru = make_rsrc(wbase + (GLU ? a.N * a.K : 0), left * a.K);
-    uint32_t woff[RB];
-#pragma unroll
-    for (int i = 0; i < RB; i++) woff[i] = (uint32_t)(16 * (GLU ? i & 1 : i) + l16) * (uint32_t)K + 16u * c;
-    u32x4 wn[RB][2];
-    auto load_w = [&](int t) {
-        const uint32_t k = (uint32_t)(t < KB ? t : KB - 1) * F8_BLOCK;
-#pragma unroll
-        for (int i = 0; i < RB; i++)
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-                wn[i][h] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                    GLU && i >= 2 ? ru : rw, (int)(woff[i] + k + 64 * h), 0, 0));
-    };
-    // the weights' scales of 64 blocks, one per lane (gate|up: gate, up)
-    const int64_t sbase = (expert * SB + (left ? n0 : 0) / F8_BLOCK) * KB;
+    const int64_t nw = n0 + (GLU ? 0 : 64 * wn);
+    const int64_t sbase = (expert * SB + (nw < a.N ? nw : n0) / F8_BLOCK) * KB;
     uint32_t swl[GLU ? 2 : 1];
-    auto load_s = [&](int t) {
+    auto load_scales = [&](int t) {
         const int k = t + lane < KB ? t + lane : KB - 1;
 #pragma unroll
         for (int g = 0; g < (GLU ? 2 : 1); g++) {
@@ -142,85 +157,102 @@ __global__ __launch_bounds__(64 * G_WAVES, 2) void f8_gemm(F8Args a, int nblocks
             else if (a.e8) swl[g] = __float_as_uint(e8m0_to_f32(((const unsigned char*)a.s)[i]));
             else swl[g] = ((const uint32_t*)a.s)[i];
         }
-    };
-    issue_x(0);
-    load_w(0);
-    if (tid < TM) rid_s[tid] = tid >= count ? -1 : a.tiles ? a.sorted[start + tid] : (int)(start + tid);
-    // scale bytes of activation row 16 j + n at [block][n][j]
-    for (int m = tid & (TM - 1), q = tid / TM; 4 * q < KB; q += 64 * G_WAVES / TM) {
-        const int64_t r = xrow(m);
-        const uint32_t v = r < 0 ? 0x7f7f7f7fu : *(const uint32_t*)(a.xs + r * a.xs_ld + 4 * q);
 #pragma unroll
-        for (int b = 0; b < 4; b++)
-            if (4 * q + b < KB) sc[((4 * q + b) * 16 + (m & 15)) * 8 + (m >> 4)] = (unsigned char)(v >> (8 * b));
-    }
+        for (int g = 0; g < (GLU ? 2 : 1); g++) asm volatile("" : "+v"(swl[g]));     // waited for here, not in the loop
+        for (int m = tid & (TM - 1), q = tid / TM; q < G_CHUNK / 4 && t + 4 * q < KB; q += 64 * WAVES / TM) {
+            const int64_t r = xrow(m);
+            const uint32_t v = r < 0 ? 0x7f7f7f7fu : *(const uint32_t*)(a.xs + r * a.xs_ld + t + 4 * q);
+            const int w = m / (16 * MB), j = m / 16 % MB;
+#pragma unroll
+            for (int b = 0; b < 4; b++)
+                sc[(((4 * q + b) * WM + w) * 16 + (m & 15)) * MB + j] = (unsigned char)(v >> (8 * b));
+        }
+    };
+    load_scales(0);
+    if (tid < TM) rid_s[tid] = tid >= count ? -1 : a.tiles ? a.sorted[start + tid] : (int)(start + tid);
 
+    // fragment reads: weight row 64 wn + 16 i + l16, pieces c and c + 4; x row
+    // 16 (MB wm + j) + l16, the same (float16: 2 c, 2 c + 1 and 8 further)
+    uint32_t xo[XB / 64], wo[2];
+#pragma unroll
+    for (int q = 0; q < 2; q++) wo[q] = (uint32_t)(64 * wn + l16) * 128 + 16u * ((c + 4 * q) ^ (l16 & 7));
+#pragma unroll
+    for (int q = 0; q < XB / 64; q++) {
+        const int p = KIND == HALF ? 2 * c + (q & 1) + 8 * (q >> 1) : c + 4 * q;
+        xo[q] = G_WTILE + (uint32_t)(16 * MB * wm + l16) * XB + 16u * (p ^ (l16 & 7));
+    }
+    typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+    i32x8 w[RB], b[2];
+    f16x8 bh[2][4];
+    auto read_w = [&](const unsigned char* st, int i) {
+        w[i] = f8_operand(*(const u32x4*)(st + i * 2048 + wo[0]), *(const u32x4*)(st + i * 2048 + wo[1]));
+    };
+    auto read_b = [&](const unsigned char* st, int j) {
+        if constexpr (KIND == HALF) {
+#pragma unroll
+            for (int q = 0; q < 4; q++) bh[j & 1][q] = *(const f16x8*)(st + 16 * j * XB + xo[q]);
+        } else {
+            b[j & 1] = f8_operand(*(const u32x4*)(st + 16 * j * XB + xo[0]), *(const u32x4*)(st + 16 * j * XB + xo[1]));
+        }
+    };
     f32x4 acc[RB][MB];
 #pragma unroll
     for (int i = 0; i < RB; i++)
 #pragma unroll
         for (int j = 0; j < MB; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    // x fragment j: row 16 j + l16, pieces c and c + 4 (float16: 2 c, 2 c + 1 and
-    // 8 further)
-    uint32_t xo[XB / 64];
-#pragma unroll
-    for (int q = 0; q < XB / 64; q++) {
-        const int piece = KIND == HALF ? 2 * c + (q & 1) + 8 * (q >> 1) : c + 4 * q;
-        xo[q] = (uint32_t)l16 * XB + 16u * (piece ^ (l16 & 7));
-    }
 
-    for (int t = 0; t < KB; t++) {
-        if ((t & 63) == 0) load_s(t);
-        // what the block before asked for has landed: this block's x and weights
-        g_wait<0>();
+    g_wait<(S - 1) * (XL + WL)>();
+    lds_barrier();
 #pragma unroll
-        for (int i = 0; i < RB; i++) asm volatile("" : "+v"(wn[i][0]), "+v"(wn[i][1]));
+    for (int i = 0; i < RB; i++) read_w(smem, i);
+    read_b(smem, 0);
+    static_assert(MB % 2 == 0, "x fragments alternate");
+    for (int t0 = 0; t0 < KB; t0 += G_CHUNK) {
+    if (t0) {                                    // every wave is past its reads of the last chunk's scales
+        load_scales(t0);
         lds_barrier();
-        u32x4 w[RB][2];
+    }
+    const int t1 = t0 + G_CHUNK < KB ? t0 + G_CHUNK : KB;
+    for (int t = t0; t < t1; t++) {              // (no branch inside: the compiler would sink products past it)
+        const unsigned char* st = smem + (t % S) * Z::STAGE;
+        const unsigned char* nx = smem + ((t + 1) % S) * Z::STAGE;
+        uint32_t sx[MB / 4];
 #pragma unroll
-        for (int i = 0; i < RB; i++) {
-            w[i][0] = wn[i][0];
-            w[i][1] = wn[i][1];
-        }
-        load_w(t + 1);
-        issue_x(t + 1);
-        if (t == KB - 1 && K % F8_BLOCK) {       // inputs past the last: the next row's
-#pragma unroll
-            for (int i = 0; i < RB; i++)
-#pragma unroll
-                for (int h = 0; h < 2; h++)
-                    if (64 * h + 16 * c >= K % F8_BLOCK) w[i][h] = u32x4{0, 0, 0, 0};
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        const unsigned char* xs = smem + (t & 1) * STAGE;
-        const u32x2 sx = *(const u32x2*)(sc + (t * 16 + l16) * 8);
+        for (int q = 0; q < MB / 4; q++)
+            sx[q] = *(const uint32_t*)(sc + ((t % G_CHUNK * WM + wm) * 16 + l16) * MB + 4 * q);
         uint32_t sw[GLU ? 2 : 1];
 #pragma unroll
-        for (int g = 0; g < (GLU ? 2 : 1); g++) sw[g] = (uint32_t)__builtin_amdgcn_readlane((int)swl[g], t & 63);
-        auto row_scale = [&](int j) { return __uint_as_float(((j < 4 ? sx.x : sx.y) >> (8 * (j & 3)) & 0xffu) << 23); };
+        for (int g = 0; g < (GLU ? 2 : 1); g++) sw[g] = (uint32_t)__builtin_amdgcn_readlane((int)swl[g], t % G_CHUNK);
+        auto row_scale = [&](int j) { return __uint_as_float((sx[j / 4] >> (8 * (j & 3)) & 0xffu) << 23); };
+        // after the block's last LDS read: the next block has landed, and this
+        // one's place is free
+        auto turn = [&]() {
+            g_wait<(S - 2) * (XL + WL)>();
+            lds_barrier();
+            issue(t + S);
+        };
         if constexpr (KIND == HALF) {
-            typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
             f16x8 wh[RB][4];
 #pragma unroll
             for (int i = 0; i < RB; i++)
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
-                    const uint32_t d0 = w[i][q >> 1][(q & 1) * 2], d1 = w[i][q >> 1][(q & 1) * 2 + 1];
+                    const uint32_t d0 = (uint32_t)w[i][2 * q], d1 = (uint32_t)w[i][2 * q + 1];
                     const f16x2 p0 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(d0, 1.f, false);
                     const f16x2 p1 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(d0, 1.f, true);
                     const f16x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(d1, 1.f, false);
                     const f16x2 p3 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(d1, 1.f, true);
                     wh[i][q] = f16x8{p0.x, p0.y, p1.x, p1.y, p2.x, p2.y, p3.x, p3.y};
                 }
-            f16x8 b[2][4];
-            auto read_b = [&](int j) {
-#pragma unroll
-                for (int q = 0; q < 4; q++) b[j & 1][q] = *(const f16x8*)(xs + 16 * j * XB + xo[q]);
-            };
-            read_b(0);
 #pragma unroll
             for (int j = 0; j < MB; j++) {
-                if (j + 1 < MB) read_b(j + 1);
+                if (j + 1 < MB) {
+                    read_b(st, j + 1);
+                } else {
+                    turn();
+#pragma unroll
+                    for (int i = 0; i < RB; i++) read_w(nx, i);
+                }
                 const float f = row_scale(j);
                 f32x4 p[RB];
 #pragma unroll
@@ -228,7 +260,8 @@ __global__ __launch_bounds__(64 * G_WAVES, 2) void f8_gemm(F8Args a, int nblocks
 #pragma unroll
                 for (int q = 0; q < 4; q++)
 #pragma unroll
-                    for (int i = 0; i < RB; i++) p[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh[i][q], b[j & 1][q], p[i], 0, 0, 0);
+                    for (int i = 0; i < RB; i++)
+                        p[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh[i][q], bh[j & 1][q], p[i], 0, 0, 0);
 #pragma unroll
                 for (int i = 0; i < RB; i++) {
                     const float g = f * __uint_as_float(sw[GLU && i >= 2 ? 1 : 0]);
@@ -236,14 +269,8 @@ __global__ __launch_bounds__(64 * G_WAVES, 2) void f8_gemm(F8Args a, int nblocks
                     for (int q = 0; q < 4; q++) acc[i][j][q] = __builtin_fmaf(p[i][q], g, acc[i][j][q]);
                 }
             }
+            read_b(nx, 0);
         } else {
-            i32x8 wv[RB], b[2];
-#pragma unroll
-            for (int i = 0; i < RB; i++) wv[i] = f8_operand(w[i][0], w[i][1]);
-            auto read_b = [&](int j) {
-                b[j & 1] = f8_operand(*(const u32x4*)(xs + 16 * j * XB + xo[0]), *(const u32x4*)(xs + 16 * j * XB + xo[1]));
-            };
-            read_b(0);
             // product n = 4 j + i; its sums are scaled two products later
             constexpr int NP = RB * MB;
             f32x4 p[3];
@@ -256,14 +283,19 @@ __global__ __launch_bounds__(64 * G_WAVES, 2) void f8_gemm(F8Args a, int nblocks
 #pragma unroll
             for (int n = 0; n < NP; n++) {
                 const int i = n % RB, j = n / RB;
-                if (i == 0 && j + 1 < MB) read_b(j + 1);
+                if (i == 0) {
+                    if (j + 1 < MB) read_b(st, j + 1);
+                    else turn();
+                }
+                if (n == NP - RB) read_b(nx, 0);
                 if constexpr (KIND == E8S) {
-                    acc[i][j] = f8_mfma_at(wv[i], b[j & 1], acc[i][j], sw[0], j < 4 ? sx.x : sx.y, j & 3);
+                    acc[i][j] = f8_mfma_at(w[i], b[j & 1], acc[i][j], sw[0], sx[j / 4], j & 3);
                 } else {
                     if (i == 0) f[j & 1] = row_scale(j) * __uint_as_float(sw[0]);
-                    p[n % 3] = f8_mfma(wv[i], b[j & 1], f32x4{0.f, 0.f, 0.f, 0.f}, 127u, 127u);
+                    p[n % 3] = f8_mfma(w[i], b[j & 1], f32x4{0.f, 0.f, 0.f, 0.f}, 127u, 127u);
                     if (n >= 2) apply(n - 2);
                 }
+                if (j == MB - 1) read_w(nx, i);
                 __builtin_amdgcn_sched_barrier(0);
             }
             if constexpr (KIND == F32S) {
@@ -271,6 +303,7 @@ __global__ __launch_bounds__(64 * G_WAVES, 2) void f8_gemm(F8Args a, int nblocks
                 apply(NP - 1);
             }
         }
+    }
     }
     g_wait<0>();                                 // no load still writes LDS below
 
@@ -290,17 +323,17 @@ __global__ __launch_bounds__(64 * G_WAVES, 2) void f8_gemm(F8Args a, int nblocks
                     o[q] = cvt_pk_bf16(silu_bf16r(__uint_as_float(gg << 16)) * __uint_as_float(uu << 16),
                                        silu_bf16r(__uint_as_float(gg & 0xffff0000u)) * __uint_as_float(uu & 0xffff0000u));
                 }
-                *(u32x2*)(smem + (16 * j + l16) * 272 + (32 * wave + 16 * i + 4 * c) * 2) = u32x2{o[0], o[1]};
+                *(u32x2*)(smem + (16 * (MB * wm + j) + l16) * 272 + (32 * wn + 16 * i + 4 * c) * 2) = u32x2{o[0], o[1]};
             }
         lds_barrier();
-        for (int m = tid >> 4; m < count; m += 64 * G_WAVES / 16) {
+        for (int m = tid >> 4; m < count; m += 4 * WAVES) {
             F8Raw<F8BF16, 8> v;
             v.v[0] = *(const u32x4*)(smem + m * 272 + 16 * l16);
             uint32_t top = v.amax();
 #pragma unroll
             for (int o = 8; o; o >>= 1) {
-                const uint32_t b = (uint32_t)__shfl_xor((int)top, o, 16);
-                top = b > top ? b : top;
+                const uint32_t u = (uint32_t)__shfl_xor((int)top, o, 16);
+                top = u > top ? u : top;
             }
             uint32_t byte = f8_scale_byte(top);
             const bool nan = byte == 255;        // as f8_rows
@@ -315,12 +348,13 @@ __global__ __launch_bounds__(64 * G_WAVES, 2) void f8_gemm(F8Args a, int nblocks
         const bool wide = a.N % 4 == 0 && ((uintptr_t)a.y & 7) == 0;
 #pragma unroll
         for (int j = 0; j < MB; j++) {
-            const int rid = rid_s[16 * j + l16];
+            const int m = 16 * (MB * wm + j) + l16;
+            const int rid = rid_s[m];
             if (rid < 0) continue;
-            const bool seen = !a.lhs || xrow(16 * j + l16) >= 0;
+            const bool seen = !a.lhs || xrow(m) >= 0;
 #pragma unroll
             for (int i = 0; i < RB; i++) {
-                const int64_t n = n0 + 16 * i + 4 * c;
+                const int64_t n = n0 + 64 * wn + 16 * i + 4 * c;
                 u32x2 o;
                 if (a.half) {
                     o.x = f32_to_f16(acc[i][j][0]) | (uint32_t)f32_to_f16(acc[i][j][1]) << 16;
@@ -330,13 +364,13 @@ __global__ __launch_bounds__(64 * G_WAVES, 2) void f8_gemm(F8Args a, int nblocks
                     o.y = cvt_pk_bf16(acc[i][j][2], acc[i][j][3]);
                 }
                 if (!seen) o = u32x2{0, 0};
-                uint16_t* p = y + (int64_t)rid * a.N + n;
+                uint16_t* q = y + (int64_t)rid * a.N + n;
                 if (wide) {
-                    if (n < a.N) *(u32x2*)p = o;
+                    if (n < a.N) *(u32x2*)q = o;
                 } else {
 #pragma unroll
-                    for (int q = 0; q < 4; q++)
-                        if (n + q < a.N) p[q] = (uint16_t)(o[q >> 1] >> (16 * (q & 1)));
+                    for (int e = 0; e < 4; e++)
+                        if (n + e < a.N) q[e] = (uint16_t)(o[e >> 1] >> (16 * (e & 1)));
                 }
             }
         }
@@ -382,23 +416,20 @@ __global__ __launch_bounds__(256) void f8_rows(const typename T::storage* __rest
     if (l == 0) s[r * sld + b] = (unsigned char)byte;
 }
 
-template <int MB, Kind KIND, bool GLU>
+template <Kind KIND, int MB, int WM, int S, bool GLU>
 int go(const F8Args& a, int64_t tiles, hipStream_t st) {
-    if (a.K > FP8_GEMM_MAX_K || a.xld != fp8_row_bytes(a.K, KIND == HALF)) {
-        set_error("fp8: K=%lld on tiles", (long long)a.K);
+    if (a.K > FP8_GEMM_MAX_K || a.xld != fp8_row_bytes(a.K, KIND == HALF) || a.tm > 16 * MB * WM) {
+        set_error("fp8: K=%lld in tiles of %d", (long long)a.K, a.tm);
         return EINVAL_ARG;
     }
-    const int KB = (int)ceil_div(a.K, F8_BLOCK);
     const int nblocks = (int)ceil_div(a.N, GLU ? 128 : 256);
-    const size_t stages = (size_t)G_STAGES * 16 * MB * (KIND == HALF ? 256 : 128) + (size_t)KB * 128;
-    const size_t lds = GLU && stages < (size_t)16 * MB * 272 ? (size_t)16 * MB * 272 : stages;
     const int64_t wgs = a.tiles ? ceil_div(tiles, 16) * 16 * nblocks : ceil_div(tiles * nblocks, 8) * 8;
     if (wgs >= (1LL << 31)) {
         set_error("fp8: grid of %lld workgroups", (long long)wgs);
         return EINVAL_ARG;
     }
-    allow_dynamic_lds_once((const void*)f8_gemm<MB, KIND, GLU>);
-    f8_gemm<MB, KIND, GLU><<<(unsigned)wgs, 64 * G_WAVES, lds, st>>>(a, nblocks, (int)tiles);
+    allow_dynamic_lds_once((const void*)f8_gemm<KIND, MB, WM, S, GLU>);
+    f8_gemm<KIND, MB, WM, S, GLU><<<(unsigned)wgs, 256 * WM, Shape<KIND, MB, WM, S>::LDS, st>>>(a, nblocks, (int)tiles);
     KMI_CHECK_LAUNCH("fp8 tiles");
     return OK;
 }
@@ -430,9 +461,10 @@ int launch_fp8_rows(const void* x, int dtype, int64_t rows, int64_t K, bool half
 }
 
 int launch_fp8_gemm(const F8Args& a, bool glu, int64_t tiles, hipStream_t st) {
-    if (glu) return go<4, HALF, true>(a, tiles, st);
-    if (a.tm <= 64) return a.e8 ? go<4, E8S, false>(a, tiles, st) : go<4, F32S, false>(a, tiles, st);
-    return a.e8 ? go<8, E8S, false>(a, tiles, st) : go<8, F32S, false>(a, tiles, st);
+    if (glu) return go<HALF, 4, 2, 2, true>(a, tiles, st);
+    if (a.tm <= 64) return a.e8 ? go<E8S, 4, 1, 2, false>(a, tiles, st) : go<F32S, 4, 1, 2, false>(a, tiles, st);
+    if (a.tm <= 128) return a.e8 ? go<E8S, 4, 2, 3, false>(a, tiles, st) : go<F32S, 4, 2, 3, false>(a, tiles, st);
+    return a.e8 ? go<E8S, 8, 2, 2, false>(a, tiles, st) : go<F32S, 8, 2, 2, false>(a, tiles, st);
 }
 
 }  // namespace kmi
