@@ -49,16 +49,16 @@ Plan plan_grouped(int64_t rows, int64_t P, int64_t E, int64_t K, bool glu) {
     return {true, !glu && per <= 64 ? 64 : 128};
 }
 
-size_t rows_bytes(int64_t rows, int64_t K, bool half) {
-    return align256((size_t)rows * fp8_row_bytes(K, half)) + align256((size_t)rows * fp8_row_scales(K));
+size_t rows_bytes(int64_t rows, int64_t K) {
+    return align256((size_t)rows * fp8_row_bytes(K)) + align256((size_t)rows * fp8_row_scales(K));
 }
 
 // x quantized at ws (rows_bytes), as a's x
-int quantize_rows(F8Args& a, const void* x, int dtype, int64_t rows, bool half, char* ws, hipStream_t st) {
+int quantize_rows(F8Args& a, const void* x, int dtype, int64_t rows, char* ws, hipStream_t st) {
     unsigned char* q = (unsigned char*)ws;
-    unsigned char* s = q + align256((size_t)rows * fp8_row_bytes(a.K, half));
-    a.x = q; a.xrows = rows; a.xld = fp8_row_bytes(a.K, half); a.xs = s; a.xs_ld = fp8_row_scales(a.K);
-    return launch_fp8_rows(x, dtype, rows, a.K, half, q, s, st);
+    unsigned char* s = q + align256((size_t)rows * fp8_row_bytes(a.K));
+    a.x = q; a.xrows = rows; a.xld = fp8_row_bytes(a.K); a.xs = s; a.xs_ld = fp8_row_scales(a.K);
+    return launch_fp8_rows(x, dtype, rows, a.K, q, s, st);
 }
 
 }  // namespace
@@ -71,7 +71,7 @@ extern "C" {
 
 size_t kmi_qmm_fp8_workspace_bytes(int64_t M, int64_t K, int64_t N, int dtype) {
     if (M <= 0 || K <= 0 || N <= 0 || !plan_dense(M, K).gemm) return 0;
-    return rows_bytes(M, K, false);
+    return rows_bytes(M, K);
 }
 
 int kmi_qmm_fp8(const void* x, int64_t M, int64_t K, int64_t N, const uint32_t* w, const void* scales, int e8m0,
@@ -91,7 +91,7 @@ int kmi_qmm_fp8(const void* x, int64_t M, int64_t K, int64_t N, const uint32_t* 
     a.w = (const unsigned char*)w; a.s = scales; a.e8 = e8m0; a.E = 1; a.wrows = N; a.K = K; a.N = N;
     a.x = x; a.xrows = M; a.y = y; a.rows = M; a.tm = p.tm; a.half = dtype == F16;
     if (!p.gemm) return launch_fp8_skinny(a, dtype, false, ceil_div(M, a.tm), st);
-    rc = quantize_rows(a, x, dtype, M, false, (char*)workspace, st);
+    rc = quantize_rows(a, x, dtype, M, (char*)workspace, st);
     return rc ? rc : launch_fp8_gemm(a, false, ceil_div(M, a.tm), st);
 }
 
@@ -99,7 +99,7 @@ size_t kmi_gather_qmm_fp8_workspace_bytes(int64_t P, int64_t X, int64_t M, int64
                                           int dtype) {
     if (P <= 0 || X <= 0 || M <= 0 || E <= 0 || K <= 0 || N <= 0) return 0;
     const Plan p = plan_grouped(P * M, P, E, K, false);
-    return sort_index_bytes(P * M, E, p.tm) + (p.gemm ? rows_bytes(X * M, K, false) : 0);
+    return sort_index_bytes(P * M, E, p.tm) + (p.gemm ? rows_bytes(X * M, K) : 0);
 }
 
 int kmi_gather_qmm_fp8(const void* x, int64_t X, int64_t M, int64_t K, const uint32_t* w, const void* scales,
@@ -115,7 +115,7 @@ int kmi_gather_qmm_fp8(const void* x, int64_t X, int64_t M, int64_t K, const uin
     if (P == 0) return OK;
     KMI_CHECK_ARG(x && w && scales && lhs && rhs && y, "%s: null pointer", what);
     const Plan p = plan_grouped(P * M, P, E, K, false);
-    KMI_CHECK_ARG(!p.gemm || X * M * fp8_row_bytes(K, false) < (1LL << 31), "%s: x past 2 GiB of codes", what);
+    KMI_CHECK_ARG(!p.gemm || X * M * fp8_row_bytes(K) < (1LL << 31), "%s: x past 2 GiB of codes", what);
     rc = check_workspace(what, kmi_gather_qmm_fp8_workspace_bytes(P, X, M, E, K, N, dtype), workspace,
                          workspace_bytes);
     if (rc) return rc;
@@ -128,7 +128,7 @@ int kmi_gather_qmm_fp8(const void* x, int64_t X, int64_t M, int64_t K, const uin
     a.x = x; a.xrows = X * M; a.y = y; a.rows = P * M; a.tm = p.tm; a.half = dtype == F16;
     a.tiles = sr.tiles; a.sorted = sr.sorted; a.lhs = lhs; a.lhs_div = 1; a.Mper = M;
     if (!p.gemm) return launch_fp8_skinny(a, dtype, false, sr.max_tiles, st);
-    rc = quantize_rows(a, x, dtype, X * M, false, (char*)workspace + sort_index_bytes(P * M, E, p.tm), st);
+    rc = quantize_rows(a, x, dtype, X * M, (char*)workspace + sort_index_bytes(P * M, E, p.tm), st);
     return rc ? rc : launch_fp8_gemm(a, false, sr.max_tiles, st);
 }
 
@@ -137,7 +137,7 @@ size_t kmi_switch_glu_fp8_workspace_bytes(int64_t T, int64_t H, int64_t I, int k
     const int64_t P = T * k;
     const Plan p = plan_grouped(P, P, E, H > I ? H : I, true);
     return align256((size_t)P * H * 2) + sort_index_bytes(P, E, p.tm) +
-           (p.gemm ? rows_bytes(T, H, true) + rows_bytes(P, I, false) : align256((size_t)P * I * 2));
+           (p.gemm ? rows_bytes(T, H) + rows_bytes(P, I) : align256((size_t)P * I * 2));
 }
 
 int kmi_switch_glu_fp8(const void* x, int64_t T, int64_t H, int64_t I, int k, const int32_t* inds,
@@ -158,7 +158,7 @@ int kmi_switch_glu_fp8(const void* x, int64_t T, int64_t H, int64_t I, int k, co
     KMI_CHECK_ARG(x && inds && w_gu && s_gu && w_down && s_down && out, "%s: null pointer", what);
     const int64_t P = T * k;
     const Plan p = plan_grouped(P, P, E, H > I ? H : I, true);
-    KMI_CHECK_ARG(!p.gemm || (T * fp8_row_bytes(H, true) < (1LL << 31) && P * I < (1LL << 31)),
+    KMI_CHECK_ARG(!p.gemm || (T * fp8_row_bytes(H) < (1LL << 31) && P * I < (1LL << 31)),
                   "%s: activations past 2 GiB", what);
     rc = check_workspace(what, kmi_switch_glu_fp8_workspace_bytes(T, H, I, k, E), workspace, workspace_bytes);
     if (rc) return rc;
@@ -178,9 +178,9 @@ int kmi_switch_glu_fp8(const void* x, int64_t T, int64_t H, int64_t I, int k, co
     d.w = (const unsigned char*)w_down; d.s = s_down; d.wrows = H; d.K = I; d.N = H; d.xrows = P; d.y = y;
     d.lhs_div = 1;
     if (p.gemm) {
-        rc = quantize_rows(g, x, dtype, T, true, ws, st);
+        rc = quantize_rows(g, x, dtype, T, ws, st);
         if (rc) return rc;
-        ws += rows_bytes(T, H, true);
+        ws += rows_bytes(T, H);
         d.x = g.y = ws; d.xld = I; d.xs_ld = g.ys_ld = fp8_row_scales(I);
         d.xs = g.ys = (unsigned char*)ws + align256((size_t)P * I);
         rc = launch_fp8_gemm(g, true, sr.max_tiles, st);

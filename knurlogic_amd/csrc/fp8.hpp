@@ -50,16 +50,14 @@ struct F8Args {
 int launch_fp8_skinny(const F8Args& a, int dtype, bool glu, int64_t tiles, hipStream_t st);
 
 // Rows quantized ahead: codes in rows of fp8_row_bytes (a multiple of 128, the
-// tail zero; half: the codes' values in float16) and scale bytes in rows of
-// fp8_row_scales.
-int64_t fp8_row_bytes(int64_t K, bool half);
+// tail zero) and scale bytes in rows of fp8_row_scales.
+int64_t fp8_row_bytes(int64_t K);
 int64_t fp8_row_scales(int64_t K);
-int launch_fp8_rows(const void* x, int dtype, int64_t rows, int64_t K, bool half, unsigned char* q, unsigned char* s,
+int launch_fp8_rows(const void* x, int dtype, int64_t rows, int64_t K, unsigned char* q, unsigned char* s,
                     hipStream_t st);
 // K past which the row scales of a tile (128 bytes a block) crowd the LDS
 constexpr int64_t FP8_GEMM_MAX_K = 65536;
-// tiles of up to a.tm (64, 128 or 256; gate|up 128) rows over such rows; gate|up takes
-// its x in float16
+// tiles of up to a.tm (64, 128 or 256; gate|up 128) rows over such rows
 int launch_fp8_gemm(const F8Args& a, bool glu, int64_t tiles, hipStream_t st);
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));

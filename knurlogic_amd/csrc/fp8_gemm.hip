@@ -20,7 +20,6 @@ namespace {
 #define KMI_F8_LDS(p) ((__attribute__((address_space(3))) unsigned char*)(p))
 
 constexpr uint32_t G_NONE = 0x80000000u;     // past every view: reads 0
-constexpr int G_WTILE = 256 * F8_BLOCK;      // a block's weights in LDS
 constexpr int G_CHUNK = 64;                  // blocks whose scales are held at a time
 
 // how weights and x meet: E4M3 operands with both scales applied to each
@@ -44,27 +43,27 @@ __device__ __forceinline__ void g_dma16(__amdgpu_buffer_rsrc_t r, unsigned char*
                  ::"s"(at), "v"(voff), "s"(r), "s"(soff) : "memory", "m0");
 }
 
-// WM waves beside each other along the activation rows, MB 16-row blocks each
-template <Kind KIND, int MB, int WM, int S>
+// NW x WM waves: 64 weight rows x MB 16-row blocks of activations each
+template <int NW, int WM, int MB, int S>
 struct Shape {
-    static constexpr int TM = 16 * MB * WM, WAVES = 4 * WM;
-    static constexpr int XB = KIND == HALF ? 256 : 128;       // bytes of a row's block
-    static constexpr int STAGE = G_WTILE + TM * XB;
-    static constexpr int XL = TM * XB / 1024 / WAVES, WL = G_WTILE / 1024 / WAVES;   // loads per wave and block
-    static constexpr int SCALES = G_CHUNK * TM;
-    static constexpr int LDS = S * STAGE + SCALES;
-    static_assert(XL * 1024 * WAVES == TM * XB, "whole loads per wave");
+    static constexpr int TN = 64 * NW, TM = 16 * MB * WM, WAVES = NW * WM;
+    static constexpr int WTILE = TN * F8_BLOCK, STAGE = WTILE + TM * F8_BLOCK;   // a block's bytes in LDS
+    static constexpr int XL = TM / 8 / WAVES, WL = TN / 8 / WAVES;               // loads per wave and block
+    static constexpr int LDS = S * STAGE + G_CHUNK * TM;
+    static_assert(XL * 8 * WAVES == TM && WL * 8 * WAVES == TN, "whole loads per wave");
 };
 
-template <Kind KIND, int MB, int WM, int S, bool GLU>
-__global__ __launch_bounds__(256 * WM, 2 / WM) void f8_gemm(F8Args a, int nblocks, int tiles) {
-    typedef Shape<KIND, MB, WM, S> Z;
-    constexpr int RB = 4, TM = Z::TM, XB = Z::XB, XL = Z::XL, WL = Z::WL, WAVES = Z::WAVES;
+template <Kind KIND, int NW, int WM, int MB, int S, bool GLU>
+__global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks, int tiles) {
+    typedef Shape<NW, WM, MB, S> Z;
+    static_assert(!GLU || NW == 4, "gate|up: 128 columns per workgroup");
+    constexpr int RB = 4, TN = Z::TN, TM = Z::TM, XL = Z::XL, WL = Z::WL, WAVES = Z::WAVES, WTILE = Z::WTILE;
+    constexpr int COLS = GLU ? TN / 2 : TN;
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ int rid_s[TM];
     unsigned char* const sc = smem + S * Z::STAGE;            // [G_CHUNK][WM][16][MB] scale bytes
     const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave & 3, wm = wave >> 2;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave % NW, wm = wave / NW;
     const int l16 = lane & 15, c = lane >> 4;
     // workgroup -> (tile, column block).  Workgroups go to the 8 XCDs in turn, and
     // an XCD's neighbours should share weights and x in its L2.  Dense: each XCD
@@ -104,24 +103,21 @@ __global__ __launch_bounds__(256 * WM, 2 / WM) void f8_gemm(F8Args a, int nblock
         const int64_t r = b * a.Mper + rid % (int)a.Mper;
         return b >= 0 && r < a.xrows ? r : -1;
     };
-    // direct-to-LDS loads: 8 (float16: 16) lanes per row, the lane's piece
-    // permuted by the row
+    // direct-to-LDS loads: 8 lanes per row, the lane's piece permuted by the row
+    const int piece = (lane & 7) ^ (lane >> 3);               // (row % 8 == lane / 8)
     const __amdgpu_buffer_rsrc_t rx = make_rsrc((const unsigned char*)a.x + x0 * a.xld, (a.xrows - x0) * a.xld);
     uint32_t xoff[XL], woff[WL];
 #pragma unroll
     for (int j = 0; j < XL; j++) {
-        constexpr int LPR = XB / 16;
-        const int m = (64 / LPR) * (wave + WAVES * j) + lane / LPR;
-        const int64_t r = xrow(m);
-        xoff[j] = r < 0 ? G_NONE : (uint32_t)((r - x0) * a.xld) + 16u * ((lane % LPR) ^ (m & 7));
+        const int64_t r = xrow(8 * (wave + WAVES * j) + (lane >> 3));
+        xoff[j] = r < 0 ? G_NONE : (uint32_t)((r - x0) * a.xld) + 16u * piece;
     }
     // weight rows of the tile: row 64 v + 16 i + l of wave column v's fragment i
     // (gate|up: fragments 0, 1 the gate rows 32 v .., 2, 3 the up rows)
-    const int64_t n0 = (int64_t)nb * (GLU ? 128 : 256);
-    const int64_t left = a.N - n0 < (GLU ? 128 : 256) ? a.N - n0 : (GLU ? 128 : 256);
+    const int64_t n0 = (int64_t)nb * COLS;
+    const int64_t left = a.N - n0 < COLS ? a.N - n0 : COLS;
     const __amdgpu_buffer_rsrc_t rw = make_rsrc(a.w + (expert * a.wrows + n0) * a.K, left * a.K);
     const __amdgpu_buffer_rsrc_t ru = make_rsrc(a.w + (expert * a.wrows + n0 + (GLU ? a.N : 0)) * a.K, left * a.K);
-    const int piece = (lane & 7) ^ (lane >> 3);               // row % 8 == lane / 8
 #pragma unroll
     for (int j = 0; j < WL; j++) {
         const int m = 8 * (wave + WAVES * j) + (lane >> 3);
@@ -138,7 +134,7 @@ __global__ __launch_bounds__(256 * WM, 2 / WM) void f8_gemm(F8Args a, int nblock
         }
 #pragma unroll
         for (int j = 0; j < XL; j++)
-            g_dma16(rx, dst + G_WTILE + (wave + WAVES * j) * 1024, t < KB ? xoff[j] : G_NONE, (uint32_t)t * XB);
+            g_dma16(rx, dst + WTILE + (wave + WAVES * j) * 1024, t < KB ? xoff[j] : G_NONE, (uint32_t)t * F8_BLOCK);
     };
 #pragma unroll
     for (int t = 0; t < S; t++) issue(t);
@@ -172,28 +168,19 @@ __global__ __launch_bounds__(256 * WM, 2 / WM) void f8_gemm(F8Args a, int nblock
     if (tid < TM) rid_s[tid] = tid >= count ? -1 : a.tiles ? a.sorted[start + tid] : (int)(start + tid);
 
     // fragment reads: weight row 64 wn + 16 i + l16, pieces c and c + 4; x row
-    // 16 (MB wm + j) + l16, the same (float16: 2 c, 2 c + 1 and 8 further)
-    uint32_t xo[XB / 64], wo[2];
+    // 16 (MB wm + j) + l16, the same
+    uint32_t xo[2], wo[2];
 #pragma unroll
-    for (int q = 0; q < 2; q++) wo[q] = (uint32_t)(64 * wn + l16) * 128 + 16u * ((c + 4 * q) ^ (l16 & 7));
-#pragma unroll
-    for (int q = 0; q < XB / 64; q++) {
-        const int p = KIND == HALF ? 2 * c + (q & 1) + 8 * (q >> 1) : c + 4 * q;
-        xo[q] = G_WTILE + (uint32_t)(16 * MB * wm + l16) * XB + 16u * (p ^ (l16 & 7));
+    for (int q = 0; q < 2; q++) {
+        wo[q] = (uint32_t)(64 * wn + l16) * F8_BLOCK + 16u * ((c + 4 * q) ^ (l16 & 7));
+        xo[q] = WTILE + (uint32_t)(16 * MB * wm + l16) * F8_BLOCK + 16u * ((c + 4 * q) ^ (l16 & 7));
     }
-    typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
     i32x8 w[RB], b[2];
-    f16x8 bh[2][4];
     auto read_w = [&](const unsigned char* st, int i) {
         w[i] = f8_operand(*(const u32x4*)(st + i * 2048 + wo[0]), *(const u32x4*)(st + i * 2048 + wo[1]));
     };
     auto read_b = [&](const unsigned char* st, int j) {
-        if constexpr (KIND == HALF) {
-#pragma unroll
-            for (int q = 0; q < 4; q++) bh[j & 1][q] = *(const f16x8*)(st + 16 * j * XB + xo[q]);
-        } else {
-            b[j & 1] = f8_operand(*(const u32x4*)(st + 16 * j * XB + xo[0]), *(const u32x4*)(st + 16 * j * XB + xo[1]));
-        }
+        b[j & 1] = f8_operand(*(const u32x4*)(st + j * 2048 + xo[0]), *(const u32x4*)(st + j * 2048 + xo[1]));
     };
     f32x4 acc[RB][MB];
 #pragma unroll
@@ -216,10 +203,14 @@ __global__ __launch_bounds__(256 * WM, 2 / WM) void f8_gemm(F8Args a, int nblock
     for (int t = t0; t < t1; t++) {              // (no branch inside: the compiler would sink products past it)
         const unsigned char* st = smem + (t % S) * Z::STAGE;
         const unsigned char* nx = smem + ((t + 1) % S) * Z::STAGE;
-        uint32_t sx[MB / 4];
+        uint32_t sx[(MB + 3) / 4];
+        const unsigned char* sp = sc + ((t % G_CHUNK * WM + wm) * 16 + l16) * MB;
+        if constexpr (MB == 2) {
+            sx[0] = *(const uint16_t*)sp;
+        } else {
 #pragma unroll
-        for (int q = 0; q < MB / 4; q++)
-            sx[q] = *(const uint32_t*)(sc + ((t % G_CHUNK * WM + wm) * 16 + l16) * MB + 4 * q);
+            for (int q = 0; q < MB / 4; q++) sx[q] = *(const uint32_t*)(sp + 4 * q);
+        }
         uint32_t sw[GLU ? 2 : 1];
 #pragma unroll
         for (int g = 0; g < (GLU ? 2 : 1); g++) sw[g] = (uint32_t)__builtin_amdgcn_readlane((int)swl[g], t % G_CHUNK);
@@ -232,18 +223,20 @@ __global__ __launch_bounds__(256 * WM, 2 / WM) void f8_gemm(F8Args a, int nblock
             issue(t + S);
         };
         if constexpr (KIND == HALF) {
+            typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+            auto halves = [](const i32x8& v, int q) -> f16x8 {       // codes 8 q .. 8 q + 7
+                const uint32_t d0 = (uint32_t)v[2 * q], d1 = (uint32_t)v[2 * q + 1];
+                const f16x2 p0 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(d0, 1.f, false);
+                const f16x2 p1 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(d0, 1.f, true);
+                const f16x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(d1, 1.f, false);
+                const f16x2 p3 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(d1, 1.f, true);
+                return f16x8{p0.x, p0.y, p1.x, p1.y, p2.x, p2.y, p3.x, p3.y};
+            };
             f16x8 wh[RB][4];
 #pragma unroll
             for (int i = 0; i < RB; i++)
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    const uint32_t d0 = (uint32_t)w[i][2 * q], d1 = (uint32_t)w[i][2 * q + 1];
-                    const f16x2 p0 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(d0, 1.f, false);
-                    const f16x2 p1 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(d0, 1.f, true);
-                    const f16x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(d1, 1.f, false);
-                    const f16x2 p3 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(d1, 1.f, true);
-                    wh[i][q] = f16x8{p0.x, p0.y, p1.x, p1.y, p2.x, p2.y, p3.x, p3.y};
-                }
+                for (int q = 0; q < 4; q++) wh[i][q] = halves(w[i], q);
 #pragma unroll
             for (int j = 0; j < MB; j++) {
                 if (j + 1 < MB) {
@@ -254,6 +247,9 @@ __global__ __launch_bounds__(256 * WM, 2 / WM) void f8_gemm(F8Args a, int nblock
                     for (int i = 0; i < RB; i++) read_w(nx, i);
                 }
                 const float f = row_scale(j);
+                f16x8 bh[4];
+#pragma unroll
+                for (int q = 0; q < 4; q++) bh[q] = halves(b[j & 1], q);
                 f32x4 p[RB];
 #pragma unroll
                 for (int i = 0; i < RB; i++) p[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -261,7 +257,7 @@ __global__ __launch_bounds__(256 * WM, 2 / WM) void f8_gemm(F8Args a, int nblock
                 for (int q = 0; q < 4; q++)
 #pragma unroll
                     for (int i = 0; i < RB; i++)
-                        p[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh[i][q], bh[j & 1][q], p[i], 0, 0, 0);
+                        p[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh[i][q], bh[q], p[i], 0, 0, 0);
 #pragma unroll
                 for (int i = 0; i < RB; i++) {
                     const float g = f * __uint_as_float(sw[GLU && i >= 2 ? 1 : 0]);
@@ -378,8 +374,8 @@ __global__ __launch_bounds__(256 * WM, 2 / WM) void f8_gemm(F8Args a, int nblock
 }
 
 // x's rows into codes [rows, ld] (tails zero) and scale bytes [rows, sld]: 16
-// lanes per row and block.  HALF: the codes' values in float16 instead.
-template <class T, bool HALF_>
+// lanes per row and block.
+template <class T>
 __global__ __launch_bounds__(256) void f8_rows(const typename T::storage* __restrict__ x, int64_t rows, int K, int KB,
                                                unsigned char* __restrict__ q, int64_t ld,
                                                unsigned char* __restrict__ s, int64_t sld) {
@@ -402,69 +398,58 @@ __global__ __launch_bounds__(256) void f8_rows(const typename T::storage* __rest
     const bool nan = byte == 255;
     if (nan) byte = 127;
     const float scale = __uint_as_float(byte << 23);
-    const uint32_t c0 = nan ? 0x7f7f7f7fu : v.codes(0, scale), c1 = nan ? 0x7f7f7f7fu : v.codes(1, scale);
-    if constexpr (HALF_) {
-        u32x4 o;
-        o.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c0, 1.f, false));
-        o.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c0, 1.f, true));
-        o.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c1, 1.f, false));
-        o.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c1, 1.f, true));
-        *(u32x4*)(q + r * ld + 2 * k) = o;
-    } else {
-        *(u32x2*)(q + r * ld + k) = u32x2{c0, c1};
-    }
+    *(u32x2*)(q + r * ld + k) = nan ? u32x2{0x7f7f7f7fu, 0x7f7f7f7fu} : u32x2{v.codes(0, scale), v.codes(1, scale)};
     if (l == 0) s[r * sld + b] = (unsigned char)byte;
 }
 
-template <Kind KIND, int MB, int WM, int S, bool GLU>
+template <Kind KIND, int NW, int WM, int MB, int S, bool GLU>
 int go(const F8Args& a, int64_t tiles, hipStream_t st) {
-    if (a.K > FP8_GEMM_MAX_K || a.xld != fp8_row_bytes(a.K, KIND == HALF) || a.tm > 16 * MB * WM) {
+    typedef Shape<NW, WM, MB, S> Z;
+    if (a.K > FP8_GEMM_MAX_K || a.xld != fp8_row_bytes(a.K) || a.tm > Z::TM) {
         set_error("fp8: K=%lld in tiles of %d", (long long)a.K, a.tm);
         return EINVAL_ARG;
     }
-    const int nblocks = (int)ceil_div(a.N, GLU ? 128 : 256);
+    const int nblocks = (int)ceil_div(a.N, GLU ? Z::TN / 2 : Z::TN);
     const int64_t wgs = a.tiles ? ceil_div(tiles, 16) * 16 * nblocks : ceil_div(tiles * nblocks, 8) * 8;
     if (wgs >= (1LL << 31)) {
         set_error("fp8: grid of %lld workgroups", (long long)wgs);
         return EINVAL_ARG;
     }
-    allow_dynamic_lds_once((const void*)f8_gemm<KIND, MB, WM, S, GLU>);
-    f8_gemm<KIND, MB, WM, S, GLU><<<(unsigned)wgs, 256 * WM, Shape<KIND, MB, WM, S>::LDS, st>>>(a, nblocks, (int)tiles);
+    allow_dynamic_lds_once((const void*)f8_gemm<KIND, NW, WM, MB, S, GLU>);
+    f8_gemm<KIND, NW, WM, MB, S, GLU><<<(unsigned)wgs, 64 * Z::WAVES, Z::LDS, st>>>(a, nblocks, (int)tiles);
     KMI_CHECK_LAUNCH("fp8 tiles");
     return OK;
 }
 
+template <int NW, int WM, int MB, int S>
+int go(const F8Args& a, int64_t tiles, hipStream_t st) {
+    return a.e8 ? go<E8S, NW, WM, MB, S, false>(a, tiles, st) : go<F32S, NW, WM, MB, S, false>(a, tiles, st);
+}
+
 }  // namespace
 
-int64_t fp8_row_bytes(int64_t K, bool half) { return ceil_div(K, F8_BLOCK) * F8_BLOCK * (half ? 2 : 1); }
+int64_t fp8_row_bytes(int64_t K) { return ceil_div(K, F8_BLOCK) * F8_BLOCK; }
 int64_t fp8_row_scales(int64_t K) { return ceil_div(ceil_div(K, F8_BLOCK), 4) * 4; }
 
-int launch_fp8_rows(const void* x, int dtype, int64_t rows, int64_t K, bool half, unsigned char* q, unsigned char* s,
+int launch_fp8_rows(const void* x, int dtype, int64_t rows, int64_t K, unsigned char* q, unsigned char* s,
                     hipStream_t st) {
     const int64_t KB = ceil_div(K, F8_BLOCK), grid = ceil_div(rows * KB, 16);
     if (grid >= (1LL << 31)) {
         set_error("fp8: %lld rows", (long long)rows);
         return EINVAL_ARG;
     }
-    const int64_t ld = fp8_row_bytes(K, half), sld = fp8_row_scales(K);
-#define KMI_ROWS(T, H) f8_rows<T, H><<<(unsigned)grid, 256, 0, st>>>((const uint16_t*)x, rows, (int)K, (int)KB, q, ld, s, sld)
-    if (half) {
-        if (dtype == BF16) KMI_ROWS(F8BF16, true);
-        else KMI_ROWS(F8F16, true);
-    } else {
-        if (dtype == BF16) KMI_ROWS(F8BF16, false);
-        else KMI_ROWS(F8F16, false);
-    }
-#undef KMI_ROWS
+    const int64_t ld = fp8_row_bytes(K), sld = fp8_row_scales(K);
+    if (dtype == BF16) f8_rows<F8BF16><<<(unsigned)grid, 256, 0, st>>>((const uint16_t*)x, rows, (int)K, (int)KB, q, ld, s, sld);
+    else f8_rows<F8F16><<<(unsigned)grid, 256, 0, st>>>((const uint16_t*)x, rows, (int)K, (int)KB, q, ld, s, sld);
     KMI_CHECK_LAUNCH("fp8 rows");
     return OK;
 }
 
 int launch_fp8_gemm(const F8Args& a, bool glu, int64_t tiles, hipStream_t st) {
-    if (glu) return go<HALF, 4, 2, 2, true>(a, tiles, st);
-    if (a.tm <= 64) return a.e8 ? go<E8S, 4, 1, 2, false>(a, tiles, st) : go<F32S, 4, 1, 2, false>(a, tiles, st);
-    if (a.tm <= 128) return a.e8 ? go<E8S, 4, 2, 3, false>(a, tiles, st) : go<F32S, 4, 2, 3, false>(a, tiles, st);
-    return a.e8 ? go<E8S, 8, 2, 2, false>(a, tiles, st) : go<F32S, 8, 2, 2, false>(a, tiles, st);
+    if (glu) return go<HALF, 4, 2, 4, 3, true>(a, tiles, st);
+    if (a.tm <= 64) return go<2, 2, 2, 3>(a, tiles, st);
+    if (a.tm <= 128) return go<2, 2, 4, 2>(a, tiles, st);
+    return go<4, 2, 8, 2>(a, tiles, st);
 }
 
 }  // namespace kmi
