@@ -38,14 +38,17 @@ struct Plan {
 };
 
 Plan plan_dense(int64_t M, int64_t K) {
-    if (M <= 64 || K > FP8_GEMM_MAX_K) return {false, M <= 16 ? 16 : M <= 32 ? 32 : 64};
-    return {true, M <= 128 ? 128 : 256};
+    if (M <= 32) {
+        const int tm = M <= 16 ? 16 : 32;
+        if (K <= fp8_skinny_max_k(tm, false)) return {false, tm};
+    }
+    return {true, M <= 64 ? 64 : M <= 128 ? 128 : 256};
 }
 
 // rows grouped by expert: by the average rows of an active one
 Plan plan_grouped(int64_t rows, int64_t P, int64_t E, int64_t K, bool glu) {
     const int64_t per = ceil_div(rows, P < E ? P : E);
-    if (per <= 16 || K > FP8_GEMM_MAX_K) return {false, per <= 16 ? 16 : per <= 32 ? 32 : 64};
+    if (per <= 16 && K <= fp8_skinny_max_k(16, glu)) return {false, 16};
     return {true, !glu && per <= 64 ? 64 : 128};
 }
 

@@ -46,7 +46,8 @@ struct F8Args {
     int half;                   // y is float16
 };
 
-// tiles of up to a.tm (16, 32 or 64) rows; dtype BF16 or F16
+// tiles of up to a.tm (16 or 32; gate|up 16) rows; dtype BF16 or F16
+int64_t fp8_skinny_max_k(int tm, bool glu);
 int launch_fp8_skinny(const F8Args& a, int dtype, bool glu, int64_t tiles, hipStream_t st);
 
 // Rows quantized ahead: codes in rows of fp8_row_bytes (a multiple of 128, the

@@ -114,6 +114,15 @@ def test_matmul_sizes(dev, M, N, Kd):
     _check(got, x, q, s)
 
 
+@pytest.mark.parametrize("M", [1, 20, 70, 150])
+@pytest.mark.parametrize("Kd", [256, 400, 1008, 2048, 4096, 8192, 8208, 16384, 16400])
+def test_matmul_depths(dev, M, Kd):
+    """Every way of splitting K, full and with a partial last block."""
+    (q, s), (wq, sc) = _w(M + Kd, (80, Kd), "f32" if M % 4 else "e8m0", dev)
+    x = _x(M, (M, Kd), BF, dev)
+    _check(K.quantized_matmul(x, wq, sc, mode="fp8"), x, q, s)
+
+
 @pytest.mark.parametrize("dtype", [BF, FH])
 @pytest.mark.parametrize("kind", ["f32", "e8m0"])
 @pytest.mark.parametrize("M", [1, 20, 50, 200, 520])
@@ -310,7 +319,7 @@ def _experts(seed, E, H, I, kind, dev):
 
 
 @pytest.mark.parametrize("T,k,E", [(1, 1, 1), (1, 8, 16), (3, 2, 4), (16, 4, 8), (50, 2, 3), (200, 2, 3), (70, 10, 12)])
-@pytest.mark.parametrize("H,I", [(256, 128), (400, 384)])
+@pytest.mark.parametrize("H,I", [(256, 128), (400, 384), (1040, 640), (4160, 256)])
 def test_switch_glu(dev, T, k, E, H, I):
     kind = "e8m0" if T % 2 == 0 else "f32"
     hg, hd, wg, wd = _experts(T + H, E, H, I, kind, dev)
