@@ -35,6 +35,7 @@ int check_workspace(const char* what, size_t need, const void* ws, size_t bytes)
 struct Plan {
     bool gemm;
     int tm;
+    bool pairs;        // f8_stream pair by pair, without the sort
 };
 
 Plan plan_dense(int64_t M, int64_t K) {
@@ -48,7 +49,7 @@ Plan plan_dense(int64_t M, int64_t K) {
 // rows grouped by expert: by the average rows of an active one
 Plan plan_grouped(int64_t rows, int64_t P, int64_t E, int64_t K, bool glu) {
     const int64_t per = ceil_div(rows, P < E ? P : E);
-    if (per <= 16 && K <= fp8_skinny_max_k(16, glu)) return {false, 16};
+    if (per <= 16 && K <= fp8_skinny_max_k(16, glu)) return {false, 16, rows == P && (P <= 16 || 4 * P <= E)};
     return {true, !glu && per <= 64 ? 64 : 128};
 }
 
@@ -102,6 +103,7 @@ size_t kmi_gather_qmm_fp8_workspace_bytes(int64_t P, int64_t X, int64_t M, int64
                                           int dtype) {
     if (P <= 0 || X <= 0 || M <= 0 || E <= 0 || K <= 0 || N <= 0) return 0;
     const Plan p = plan_grouped(P * M, P, E, K, false);
+    if (p.pairs) return 0;
     return sort_index_bytes(P * M, E, p.tm) + (p.gemm ? rows_bytes(X * M, K) : 0);
 }
 
@@ -122,14 +124,21 @@ int kmi_gather_qmm_fp8(const void* x, int64_t X, int64_t M, int64_t K, const uin
     rc = check_workspace(what, kmi_gather_qmm_fp8_workspace_bytes(P, X, M, E, K, N, dtype), workspace,
                          workspace_bytes);
     if (rc) return rc;
-    SortedRows sr;
     hipStream_t st = (hipStream_t)stream;
-    rc = launch_sort_rows(rhs, P, M, (int)E, p.tm, workspace, (uint16_t*)y, N, st, &sr);
-    if (rc) return rc;
+    SortedRows sr = {};
+    if (!p.pairs) {
+        rc = launch_sort_rows(rhs, P, M, (int)E, p.tm, workspace, (uint16_t*)y, N, st, &sr);
+        if (rc) return rc;
+    }
     F8Args a = {};
     a.w = (const unsigned char*)w; a.s = scales; a.e8 = e8m0; a.E = E; a.wrows = N; a.K = K; a.N = N;
     a.x = x; a.xrows = X * M; a.y = y; a.rows = P * M; a.tm = p.tm; a.half = dtype == F16;
     a.tiles = sr.tiles; a.sorted = sr.sorted; a.lhs = lhs; a.lhs_div = 1; a.Mper = M;
+    if (p.pairs) {
+        a.route = rhs;
+        a.tm = 1;
+        return launch_fp8_skinny(a, dtype, false, P, st);
+    }
     if (!p.gemm) return launch_fp8_skinny(a, dtype, false, sr.max_tiles, st);
     rc = quantize_rows(a, x, dtype, X * M, (char*)workspace + sort_index_bytes(P * M, E, p.tm), st);
     return rc ? rc : launch_fp8_gemm(a, false, sr.max_tiles, st);
@@ -139,7 +148,7 @@ size_t kmi_switch_glu_fp8_workspace_bytes(int64_t T, int64_t H, int64_t I, int k
     if (T <= 0 || H <= 0 || I <= 0 || k <= 0 || E <= 0) return 0;
     const int64_t P = T * k;
     const Plan p = plan_grouped(P, P, E, H > I ? H : I, true);
-    return align256((size_t)P * H * 2) + sort_index_bytes(P, E, p.tm) +
+    return align256((size_t)P * H * 2) + (p.pairs ? 0 : sort_index_bytes(P, E, p.tm)) +
            (p.gemm ? rows_bytes(T, H) + rows_bytes(P, I) : align256((size_t)P * I * 2));
 }
 
@@ -169,10 +178,12 @@ int kmi_switch_glu_fp8(const void* x, int64_t T, int64_t H, int64_t I, int k, co
     char* ws = (char*)workspace;
     uint16_t* y = scores ? (uint16_t*)ws : (uint16_t*)out;
     ws += align256((size_t)P * H * 2);
-    SortedRows sr;
-    rc = launch_sort_rows(inds, P, 1, (int)E, p.tm, ws, y, H, st, &sr);
-    if (rc) return rc;
-    ws += sort_index_bytes(P, E, p.tm);
+    SortedRows sr = {};
+    if (!p.pairs) {
+        rc = launch_sort_rows(inds, P, 1, (int)E, p.tm, ws, y, H, st, &sr);
+        if (rc) return rc;
+        ws += sort_index_bytes(P, E, p.tm);
+    }
     F8Args g = {};
     g.w = (const unsigned char*)w_gu; g.s = s_gu; g.e8 = e8m0; g.E = E; g.wrows = 2 * I; g.K = H; g.N = I;
     g.x = x; g.xrows = T; g.rows = P; g.tm = p.tm;
@@ -190,10 +201,15 @@ int kmi_switch_glu_fp8(const void* x, int64_t T, int64_t H, int64_t I, int k, co
         if (rc) return rc;
         rc = launch_fp8_gemm(d, false, sr.max_tiles, st);
     } else {
+        if (p.pairs) {
+            g.route = d.route = inds;
+            g.tm = d.tm = 1;
+        }
         d.x = g.y = ws;
-        rc = launch_fp8_skinny(g, dtype, true, sr.max_tiles, st);
+        rc = launch_fp8_skinny(g, dtype, true, p.pairs ? P : sr.max_tiles, st);
         if (rc) return rc;
-        rc = launch_fp8_skinny(d, dtype, false, sr.max_tiles, st);
+        if (p.pairs && scores && fp8_combine_supported(I, k)) return launch_fp8_combine(d, scores, k, T, out, st);
+        rc = launch_fp8_skinny(d, dtype, false, p.pairs ? P : sr.max_tiles, st);
     }
     if (rc) return rc;
     if (scores) return kmi_moe_combine(y, scores, dtype, T, k, H, out, stream);

@@ -11,6 +11,8 @@
 // take and give 16-bit activations, float32 ones are refused.
 #pragma once
 
+#include <type_traits>
+
 #include "common.hpp"
 
 namespace kmi {
@@ -35,6 +37,9 @@ struct F8Args {
     const int32_t* lhs;
     int64_t lhs_div, Mper;
     int tm;
+    // f8_stream, instead of tiles: the expert of each of the `rows` pairs; tile z =
+    // pair z, of x row (lhs ? lhs[z] : z / lhs_div)
+    const int32_t* route;
     // launch_fp8_gemm: x is rows of codes as launch_fp8_rows writes them (xld
     // bytes each) with scale bytes xs [xrows, xs_ld]; gate|up writes codes y
     // [rows, N] and scale bytes ys [rows, ys_ld] of the activations
@@ -49,6 +54,12 @@ struct F8Args {
 // tiles of up to a.tm (16 or 32; gate|up 16) rows; dtype BF16 or F16
 int64_t fp8_skinny_max_k(int tm, bool glu);
 int launch_fp8_skinny(const F8Args& a, int dtype, bool glu, int64_t tiles, hipStream_t st);
+
+// out [T, N] = the combine of every token's k pairs over a's weights (bf16): pair
+// t k + s reads x row t k + s and expert route[t k + s]; the products rounded
+// to bf16, weighted by scores [T, k] and summed as kmi_moe_combine does
+bool fp8_combine_supported(int64_t K, int k);
+int launch_fp8_combine(const F8Args& a, const void* scores, int k, int64_t T, void* out, hipStream_t st);
 
 // Rows quantized ahead: codes in rows of fp8_row_bytes (a multiple of 128, the
 // tail zero) and scale bytes in rows of fp8_row_scales.
@@ -91,12 +102,20 @@ __device__ __forceinline__ f32x4 f8_mfma_at(i32x8 a, i32x8 b, f32x4 c, uint32_t 
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, (int)sa, 3, (int)sb);
 }
 
-// max over the four lanes l, l ^ 16, l ^ 32, l ^ 48
-__device__ __forceinline__ uint32_t f8_max_quads(uint32_t v) {
-    const auto p = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    v = p[0] > p[1] ? p[0] : p[1];
-    const auto q = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    return q[0] > q[1] ? q[0] : q[1];
+// max over each 16 neighbouring lanes, by rotations of a row of lanes (a shuffle
+// through LDS takes some twenty times as long)
+__device__ __forceinline__ uint32_t f8_max16(uint32_t v) {
+    auto turn = [](uint32_t x, auto by) {
+        return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, 0x120 + decltype(by)::value, 0xf, 0xf, false);
+    };
+    uint32_t u = turn(v, std::integral_constant<int, 8>());
+    v = u > v ? u : v;
+    u = turn(v, std::integral_constant<int, 4>());
+    v = u > v ? u : v;
+    u = turn(v, std::integral_constant<int, 2>());
+    v = u > v ? u : v;
+    u = turn(v, std::integral_constant<int, 1>());
+    return u > v ? u : v;
 }
 
 // N activations as loaded (16-byte pieces), their largest magnitude's float32

@@ -325,13 +325,7 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
         for (int m = tid >> 4; m < count; m += 4 * WAVES) {
             F8Raw<F8BF16, 8> v;
             v.v[0] = *(const u32x4*)(smem + m * 272 + 16 * l16);
-            uint32_t top = v.amax();
-#pragma unroll
-            for (int o = 8; o; o >>= 1) {
-                const uint32_t u = (uint32_t)__shfl_xor((int)top, o, 16);
-                top = u > top ? u : top;
-            }
-            uint32_t byte = f8_scale_byte(top);
+            uint32_t byte = f8_scale_byte(f8_max16(v.amax()));
             const bool nan = byte == 255;        // as f8_rows
             if (nan) byte = 127;
             const float scale = __uint_as_float(byte << 23);
@@ -387,14 +381,8 @@ __global__ __launch_bounds__(256) void f8_rows(const typename T::storage* __rest
     F8Raw<T, 8> v;
     if (k < K) v.load(x + r * K + k);
     else v.zero();
-    uint32_t top = v.amax();
-#pragma unroll
-    for (int o = 8; o; o >>= 1) {
-        const uint32_t t = (uint32_t)__shfl_xor((int)top, o, 16);
-        top = t > top ? t : top;
-    }
     // a block with an infinity or a NaN: NaN codes, so the scale stays a number
-    uint32_t byte = f8_scale_byte(top);
+    uint32_t byte = f8_scale_byte(f8_max16(v.amax()));
     const bool nan = byte == 255;
     if (nan) byte = 127;
     const float scale = __uint_as_float(byte << 23);

@@ -44,17 +44,19 @@ __device__ __forceinline__ f32x4 st_times(const i32x8& w, const i32x8& x) {
 }
 
 // R row blocks per wave and step; KPW blocks of K per wave at most
-template <class T, int MB, int KP, int KPW, int R, bool GLU>
-__global__ __launch_bounds__(64 * ST_WAVES) void f8_stream(F8Args a, int steps) {
-    constexpr int RB = GLU ? 2 : 1, NP = ST_WAVES / KP, F = R * RB * KPW;
-    // weight blocks (2 KB) in flight per wave: 8, or 4 where x takes 128 registers
-    constexpr int DEPTH = KPW * MB >= 16 ? 4 : 8, D = F < DEPTH ? F : DEPTH;
+// and W waves (GLU: 3 workgroups of 4 on a CU, or one of 8; else 2 or 1 of 8)
+template <class T, int MB, int KP, int KPW, int R, bool GLU, int W>
+__global__ __launch_bounds__(64 * W, W == 4 ? 3 : GLU || KPW * MB >= 8 ? 2 : 4) void f8_stream(F8Args a, int steps) {
+    constexpr int RB = GLU ? 2 : 1, NP = W / KP, F = R * RB * KPW;
+    // weight blocks (2 KB) in flight per wave: 8, or 4 where x, or gate|up's float16
+    // operands, take the registers
+    constexpr int DEPTH = GLU || KPW * MB >= 16 ? 4 : 8, D = F < DEPTH ? F : DEPTH;
     constexpr int BATCH = KPW * MB < 4 ? KPW : 4 / MB;       // x blocks quantized at a time
     static_assert(F % D == 0 && KPW % BATCH == 0, "ring");
     // a wave's x codes, and after them its sums (two steps'), in turn
     constexpr int SUMS = R * RB * MB * 1024, AREA = 2 * SUMS > BATCH * MB * 2048 ? 2 * SUMS : BATCH * MB * 2048;
-    __shared__ __align__(16) unsigned char area[ST_WAVES][AREA];
-    __shared__ unsigned char xe[ST_WAVES][BATCH * MB * 16];
+    __shared__ __align__(16) unsigned char area[W][AREA];
+    __shared__ unsigned char xe[W][BATCH * MB * 16];
     __shared__ int rid_s[16 * MB], xrow_s[16 * MB];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kp = wave % KP, np = wave / KP;
@@ -66,6 +68,16 @@ __global__ __launch_bounds__(64 * ST_WAVES) void f8_stream(F8Args a, int steps) 
         expert = __builtin_amdgcn_readfirstlane(t[0]);
         start = __builtin_amdgcn_readfirstlane(t[1]);
         count = __builtin_amdgcn_readfirstlane(t[2]);
+    }
+    if (a.route) {
+        expert = __builtin_amdgcn_readfirstlane(a.route[start]);
+        count = 1;
+        if (expert < 0 || expert >= a.E) {                   // a zero row (gate|up: not read)
+            if (!GLU)
+                for (int64_t n = (int64_t)blockIdx.x * blockDim.x + tid; n < a.N; n += (int64_t)gridDim.x * blockDim.x)
+                    ((typename T::storage*)a.y)[start * a.N + n] = 0;
+            return;
+        }
     }
     if (count <= 0) return;                                  // (the whole workgroup)
 
@@ -112,7 +124,7 @@ __global__ __launch_bounds__(64 * ST_WAVES) void f8_stream(F8Args a, int steps) 
         if (tid < count) {
             rid = a.tiles ? a.sorted[start + tid] : (int)(start + tid);
             xr = rid;
-            if (a.tiles) {
+            if (a.tiles || a.route) {
                 const int p = rid / (int)a.Mper, m = rid % (int)a.Mper;
                 const int64_t b = a.lhs ? a.lhs[p] : p / (int)a.lhs_div;
                 const int64_t r = b * a.Mper + m;
@@ -141,28 +153,32 @@ __global__ __launch_bounds__(64 * ST_WAVES) void f8_stream(F8Args a, int steps) 
                 }
             continue;
         }
-#pragma unroll 4
-        for (int m = 0; m < count; m++) {
-            const int xr = xrow_s[m];
-            F8Raw<T, 8> v;
-            if (c < BATCH && k < K) v.load((const typename T::storage*)a.x + (int64_t)(xr < 0 ? 0 : xr) * a.K + k);
-            else v.zero();
-            uint32_t top = v.amax();
+        auto rows = [&](int m0, auto many) {                 // several rows' loads before the first is used
+            constexpr int G = decltype(many)::value;
+            F8Raw<T, 8> v[G];
 #pragma unroll
-            for (int o = 8; o; o >>= 1) {
-                const uint32_t u = (uint32_t)__shfl_xor((int)top, o, 16);
-                top = u > top ? u : top;
+            for (int g = 0; g < G; g++) {
+                const int xr = xrow_s[m0 + g < count ? m0 + g : count - 1];
+                if (c < BATCH && k < K) v[g].load((const typename T::storage*)a.x + (int64_t)(xr < 0 ? 0 : xr) * a.K + k);
+                else v[g].zero();
             }
-            uint32_t byte = f8_scale_byte(top);
-            const bool nan = byte == 255;                    // NaN codes, so the scale stays a number
-            if (nan) byte = 127;
-            const float scale = __uint_as_float(byte << 23);
-            const u32x2 o = nan ? u32x2{0x7f7f7f7fu, 0x7f7f7f7fu} : u32x2{v.codes(0, scale), v.codes(1, scale)};
-            if (c < BATCH) {
-                *(u32x2*)(area[wave] + (c * MB * 16 + m) * 128 + 16 * ((l16 >> 1) ^ (m & 7)) + 8 * (l16 & 1)) = o;
-                if (l16 == 0) xe[wave][c * MB * 16 + m] = (unsigned char)byte;
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+                uint32_t byte = f8_scale_byte(f8_max16(v[g].amax()));
+                const bool nan = byte == 255;                // NaN codes, so the scale stays a number
+                if (nan) byte = 127;
+                const float scale = __uint_as_float(byte << 23);
+                const u32x2 o = nan ? u32x2{0x7f7f7f7fu, 0x7f7f7f7fu} : u32x2{v[g].codes(0, scale), v[g].codes(1, scale)};
+                const int m = m0 + g;
+                if (c < BATCH && m < count) {
+                    *(u32x2*)(area[wave] + (c * MB * 16 + m) * 128 + 16 * ((l16 >> 1) ^ (m & 7)) + 8 * (l16 & 1)) = o;
+                    if (l16 == 0) xe[wave][c * MB * 16 + m] = (unsigned char)byte;
+                }
             }
-        }
+        };
+        if (count == 1) rows(0, std::integral_constant<int, 1>());
+        else
+            for (int m = 0; m < count; m += 8) rows(m, std::integral_constant<int, 8>());
         // (a wave reads what it wrote: LDS is in order within it)
 #pragma unroll
         for (int i = 0; i < BATCH; i++)
@@ -211,6 +227,7 @@ __global__ __launch_bounds__(64 * ST_WAVES) void f8_stream(F8Args a, int steps) 
                 for (int e = 0; e < 4; e++) acc[r][g][j][e] = __builtin_fmaf(p[e], f, acc[r][g][j][e]);
             }
             load((q + D) % F, q + D < F ? step : next);
+            if constexpr (GLU) __builtin_amdgcn_sched_barrier(0);    // one block's float16 operands at a time
         }
 #pragma unroll
         for (int r = 0; r < R; r++)
@@ -220,7 +237,7 @@ __global__ __launch_bounds__(64 * ST_WAVES) void f8_stream(F8Args a, int steps) 
                 for (int j = 0; j < MB; j++) *(f32x4*)(area[wave] + buf * SUMS + ((r * RB + g) * MB + j) * 1024 + 16 * lane) = acc[r][g][j];
         lds_barrier();
         // D: row 4 (l / 16) + e of the block, activation row l % 16
-        for (int idx = tid; idx < NP * R * MB * 64; idx += 64 * ST_WAVES) {
+        for (int idx = tid; idx < NP * R * MB * 64; idx += 64 * W) {
             const int l = idx & 63, j = idx / 64 % MB, r = idx / 64 / MB % R, p = idx / 64 / MB / R;
             const int tok = 16 * j + (l & 15), rid = rid_s[tok];
             if (rid < 0) continue;
@@ -250,35 +267,125 @@ __global__ __launch_bounds__(64 * ST_WAVES) void f8_stream(F8Args a, int steps) 
     }
 }
 
-// waves of the device's CUs that stream at once: two workgroups each
+// The down product and the weighted combine of a token's pairs: one workgroup per
+// 16 output columns and token, one wave per pair (in turn past 8), so that no
+// product leaves the workgroup before it is summed.  K up to CB_MAX_K.
+constexpr int CB_MAX_K = 4096, CB_MAX_SLOTS = 64, CB_DEPTH = 8;
+
+__global__ __launch_bounds__(64 * ST_WAVES) void f8_combine(F8Args a, const uint16_t* __restrict__ scores, int k,
+                                                            uint16_t* __restrict__ out) {
+    __shared__ __align__(16) unsigned char xs[ST_WAVES][CB_MAX_K];
+    __shared__ unsigned char xe[ST_WAVES][CB_MAX_K / F8_BLOCK];
+    __shared__ float sums[CB_MAX_SLOTS][16], weight[CB_MAX_SLOTS];
+    const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, c = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int K = (int)a.K, KB = (K + F8_BLOCK - 1) / F8_BLOCK;
+    const int64_t SB = (a.wrows + F8_BLOCK - 1) / F8_BLOCK, n0 = (int64_t)blockIdx.x * 16;
+    const int64_t left = a.N - n0 < 16 ? a.N - n0 : 16;
+    const int64_t token = blockIdx.y;
+    if (tid < k) weight[tid] = bf16_to_f32(scores[token * k + tid]);
+    for (int slot = wave; slot < k; slot += ST_WAVES) {
+        const int64_t pair = token * k + slot;
+        const int64_t expert = __builtin_amdgcn_readfirstlane(a.route[pair]);
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        if (expert >= 0 && expert < a.E) {
+            const __amdgpu_buffer_rsrc_t rs = make_rsrc(a.w + (expert * a.wrows + n0) * a.K, left * a.K);
+            const uint32_t off = (uint32_t)l16 * (uint32_t)K + 16u * c;
+            const int64_t si = (expert * SB + n0 / F8_BLOCK) * KB + (lane < KB ? lane : 0);
+            const float sw = a.e8 ? e8m0_to_f32(((const unsigned char*)a.s)[si]) : ((const float*)a.s)[si];
+            i32x8 w[CB_DEPTH];
+            auto load = [&](int kb, int d) {
+                const int in = K - kb * F8_BLOCK;
+                w[d] = f8_operand(
+                    __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                        rs, (int)(16 * c < in ? off : ST_NONE), kb * F8_BLOCK, AUX_NT)),
+                    __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                        rs, (int)(64 + 16 * c < in ? off : ST_NONE), kb * F8_BLOCK + 64, AUX_NT)));
+            };
+#pragma unroll
+            for (int d = 0; d < CB_DEPTH; d++) load(d, d);
+            // the pair's activations: 16 lanes per block
+            for (int b0 = 0; b0 < KB; b0 += 4) {
+                const int kk = (b0 + c) * F8_BLOCK + 8 * l16;
+                F8Raw<F8BF16, 8> v;
+                if (kk < K) v.load((const uint16_t*)a.x + pair * a.K + kk);
+                else v.zero();
+                uint32_t byte = f8_scale_byte(f8_max16(v.amax()));
+                const bool nan = byte == 255;
+                if (nan) byte = 127;
+                const float scale = __uint_as_float(byte << 23);
+                if (b0 + c < KB) {
+                    *(u32x2*)(xs[wave] + kk) = nan ? u32x2{0x7f7f7f7fu, 0x7f7f7f7fu} : u32x2{v.codes(0, scale), v.codes(1, scale)};
+                    if (l16 == 0) xe[wave][b0 + c] = (unsigned char)byte;
+                }
+            }
+            for (int b0 = 0; b0 < KB; b0 += CB_DEPTH) {
+#pragma unroll
+                for (int d = 0; d < CB_DEPTH; d++) {
+                    const int kb = b0 + d, at = kb < KB ? kb : 0;
+                    // every column the same row: column 0 is used
+                    const i32x8 x = f8_operand(*(const u32x4*)(xs[wave] + at * F8_BLOCK + 16 * c),
+                                               *(const u32x4*)(xs[wave] + at * F8_BLOCK + 64 + 16 * c));
+                    const f32x4 p = f8_mfma(w[d], x, f32x4{0.f, 0.f, 0.f, 0.f}, 127u, 127u);
+                    const float s = __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(sw), at)) *
+                                    __uint_as_float((uint32_t)xe[wave][at] << 23);
+                    const float f = kb < KB ? s : 0.f;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[e] = __builtin_fmaf(kb < KB ? p[e] : 0.f, f, acc[e]);
+                    load(kb + CB_DEPTH, d);
+                }
+            }
+        }
+        if (l16 == 0) *(f32x4*)&sums[slot][4 * c] = acc;
+    }
+    __syncthreads();
+    if (tid < left) {
+        double o = 0.0;
+        for (int s = 0; s < k; s++)
+            o += (double)TBF16::round(TBF16::round(sums[s][tid]) * weight[s]);
+        float f = (float)o;
+        asm volatile("" : "+v"(f));              // rounded to float32 and then to bf16, as moe_combine
+        out[token * a.N + n0 + tid] = f32_to_bf16(f);
+    }
+}
+
+// workgroups of 8 waves that stream at once: two on each CU
 constexpr int64_t ST_GRID = 512;
 
-template <class T, int MB, int KP, int KPW, int R, bool GLU>
+template <class T, int MB, int KP, int KPW, int R, bool GLU, int W = ST_WAVES>
 int go(const F8Args& a, int64_t tiles, hipStream_t st) {
-    const int64_t steps = ceil_div(a.N, 16 * R * (ST_WAVES / KP));
+    const int64_t steps = ceil_div(a.N, 16 * R * (W / KP));
     if (steps >= (1LL << 31)) {
         set_error("fp8: N=%lld", (long long)a.N);
         return EINVAL_ARG;
     }
     // as many workgroups per tile as keep every one's steps alike
-    const int64_t per = ceil_div(steps * tiles, ST_GRID);
+    const int64_t per = ceil_div(steps * tiles, W == 4 ? 3 * ST_GRID / 2 : ST_GRID);
     const int64_t gx = ceil_div(steps, per < steps ? per : steps);
-    f8_stream<T, MB, KP, KPW, R, GLU><<<dim3((unsigned)gx, (unsigned)tiles), 64 * ST_WAVES, 0, st>>>(a, (int)steps);
+    f8_stream<T, MB, KP, KPW, R, GLU, W><<<dim3((unsigned)gx, (unsigned)tiles), 64 * W, 0, st>>>(a, (int)steps);
     KMI_CHECK_LAUNCH("fp8 stream");
     return OK;
 }
 
-// The parts of K: 8 where each then has at most KPW blocks, or fewer for a short K
-// (a part with no block would idle).
+// The parts of K: as few as leave a wave's x in its registers (KPW blocks), so that
+// a part with no block is rare.
 template <class T, int MB, bool GLU>
 int parts(const F8Args& a, int64_t tiles, hipStream_t st) {
     const int64_t KB = ceil_div(a.K, F8_BLOCK);
-    if (KB <= 2) return go<T, MB, 2, 1, GLU ? 2 : 4, GLU>(a, tiles, st);
-    if (KB <= 4) return go<T, MB, 2, 2, GLU ? 1 : 2, GLU>(a, tiles, st);
-    if (KB <= 8) return go<T, MB, 2, 4, 1, GLU>(a, tiles, st);
-    if (KB <= 16) return go<T, MB, 4, 4, 1, GLU>(a, tiles, st);
-    if (KB <= 32) return go<T, MB, 8, 4, 1, GLU>(a, tiles, st);
-    if (KB <= 64) return go<T, MB, 8, 8, 1, GLU>(a, tiles, st);
+    if constexpr (GLU) {
+        if (KB <= 4) return go<T, MB, 2, 2, 1, GLU, 4>(a, tiles, st);
+        if (KB <= 8) return go<T, MB, 2, 4, 1, GLU, 4>(a, tiles, st);
+        if (KB <= 16) return go<T, MB, 4, 4, 1, GLU, 4>(a, tiles, st);
+        if (KB <= 32) return go<T, MB, 8, 4, 1, GLU>(a, tiles, st);
+        if (KB <= 64) return go<T, MB, 8, 8, 1, GLU>(a, tiles, st);
+    } else {
+        if (KB <= 2) return go<T, MB, 2, 1, 4, GLU>(a, tiles, st);
+        if (KB <= 4) return go<T, MB, 2, 2, 2, GLU>(a, tiles, st);
+        if (KB <= 8) return go<T, MB, 2, 4, 1, GLU>(a, tiles, st);
+        if (KB <= 16) return go<T, MB, 4, 4, 1, GLU>(a, tiles, st);
+        if (KB <= 32) return go<T, MB, 8, 4, 1, GLU>(a, tiles, st);
+        if (KB <= 64) return go<T, MB, 8, 8, 1, GLU>(a, tiles, st);
+    }
     if constexpr (MB == 1 && !GLU) return go<T, MB, 8, 16, 1, GLU>(a, tiles, st);
     set_error("fp8: K=%lld for tiles of %d rows", (long long)a.K, a.tm);
     return EINVAL_ARG;
@@ -297,6 +404,19 @@ int launch_fp8_skinny(const F8Args& a, int dtype, bool glu, int64_t tiles, hipSt
     if (glu) return parts<F8BF16, 1, true>(a, tiles, st);
     if (a.tm <= 16) return dtype == BF16 ? parts<F8BF16, 1, false>(a, tiles, st) : parts<F8F16, 1, false>(a, tiles, st);
     return dtype == BF16 ? parts<F8BF16, 2, false>(a, tiles, st) : parts<F8F16, 2, false>(a, tiles, st);
+}
+
+bool fp8_combine_supported(int64_t K, int k) { return K <= CB_MAX_K && k <= CB_MAX_SLOTS; }
+
+int launch_fp8_combine(const F8Args& a, const void* scores, int k, int64_t T, void* out, hipStream_t st) {
+    const int64_t nb = ceil_div(a.N, 16);
+    if (!a.route || !fp8_combine_supported(a.K, k) || T < 1 || T >= 65536 || nb >= (1LL << 31)) {
+        set_error("fp8: combine of %lld tokens, K=%lld", (long long)T, (long long)a.K);
+        return EINVAL_ARG;
+    }
+    f8_combine<<<dim3((unsigned)nb, (unsigned)T), 64 * ST_WAVES, 0, st>>>(a, (const uint16_t*)scores, k, (uint16_t*)out);
+    KMI_CHECK_LAUNCH("fp8 combine");
+    return OK;
 }
 
 }  // namespace kmi

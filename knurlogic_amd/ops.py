@@ -12,6 +12,7 @@ tensors' device and stream; nothing falls back to the CPU.
 from __future__ import annotations
 
 import contextlib
+import functools
 import math
 
 import torch
@@ -863,16 +864,27 @@ def moe_experts(x: torch.Tensor, logits: torch.Tensor, k: int, w_gu, s_gu, b_gu,
 # --- E4M3 weights with a scale per block of 128 x 128 -------------------------------
 
 def _one_device(what, *ts):
-    _on_gpu(*ts)
-    dev = ts[0].device
-    for t in ts[1:]:
-        if t is not None and t.device != dev:
-            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
+    dev = ts[0].get_device()
+    for t in ts:
+        if t is not None and (t.get_device() != dev or not t.is_cuda):
+            _on_gpu(*ts)
+            raise ValueError(f"{what}: tensors on {ts[0].device} and {t.device}")
+
+
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_HERE = contextlib.nullcontext()
 
 
 def _on(t: torch.Tensor):
     """A context with t's device current (kernels launch on the current one)."""
-    return contextlib.nullcontext() if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _HERE if t.get_device() == _current_device() else torch.cuda.device(t.device)
+
+
+@functools.lru_cache(maxsize=1024)
+def _fp8_workspace(name: str, *sizes) -> int:
+    """The workspace query ``name`` (a function of sizes alone; asking the
+    library each time takes 0.7 us of a small call)."""
+    return getattr(_lib(), name)(*sizes)
 
 
 def _fp8_blocks(n: int) -> int:
@@ -901,12 +913,15 @@ def _check_fp8(what, w, scales, biases, group_size, bits):
     if scales.dtype not in (torch.float32, torch.uint8):
         raise ValueError(f"{what}: fp8 scales are float32 or uint8 E8M0 exponents (got {scales.dtype})")
     wq = _fp8_codes(what, w)
-    if wq.ndim < 2 or wq.shape[-1] % 4:
-        raise ValueError(f"{what}: w packs {tuple(wq.shape)} words; inputs come in multiples of 16")
-    want = (*wq.shape[:-2], _fp8_blocks(wq.shape[-2]), _fp8_blocks(wq.shape[-1] * 4))
-    if tuple(scales.shape) != want:
-        raise ValueError(f"{what}: scales {tuple(scales.shape)} for a [{wq.shape[-2]}, {wq.shape[-1] * 4}] fp8 "
-                         f"weight; expected {want}")
+    shape = wq.shape
+    if len(shape) < 2 or shape[-1] % 4:
+        raise ValueError(f"{what}: w packs {tuple(shape)} words; inputs come in multiples of 16")
+    N, K = shape[-2], shape[-1] * 4
+    sshape = scales.shape
+    if len(sshape) != len(shape) or sshape[-1] != (K + 127) // 128 or sshape[-2] != (N + 127) // 128 \
+            or sshape[:-2] != shape[:-2]:
+        raise ValueError(f"{what}: scales {tuple(sshape)} for a [{N}, {K}] fp8 weight; expected "
+                         f"{(*shape[:-2], _fp8_blocks(N), _fp8_blocks(K))}")
     return wq, scales.contiguous(), int(scales.dtype == torch.uint8)
 
 
@@ -965,7 +980,7 @@ def _qmm_fp8(x, w, scales, biases, transpose, group_size, bits):
     L = _lib()
     code = DTYPE_CODE[x.dtype]
     with _on(x):
-        nbytes = L.kmi_qmm_fp8_workspace_bytes(M, K, N, code)
+        nbytes = _fp8_workspace("kmi_qmm_fp8_workspace_bytes", M, K, N, code)
         ws = _workspace(nbytes, x.device)
         _abi.check(L.kmi_qmm_fp8(_ptr(xc), M, K, N, _ptr(wq), _ptr(sc), e8, code, _ptr(y), _ptr(ws), nbytes,
                                  _stream(x)), what)
@@ -989,7 +1004,7 @@ def _gather_fp8(x, w, scales, biases, lhs_indices, rhs_indices, transpose, group
     L = _lib()
     code = DTYPE_CODE[x.dtype]
     with _on(x):
-        nbytes = L.kmi_gather_qmm_fp8_workspace_bytes(P, Xb, M, E, K, N, code)
+        nbytes = _fp8_workspace("kmi_gather_qmm_fp8_workspace_bytes", P, Xb, M, E, K, N, code)
         ws = _workspace(nbytes, x.device)
         _abi.check(L.kmi_gather_qmm_fp8(_ptr(xc), Xb, M, K, _ptr(wq), _ptr(sc), e8, E, N, _ptr(lhs), _ptr(rhs), P,
                                         code, _ptr(y), _ptr(ws), nbytes, _stream(x)), what)
@@ -1034,7 +1049,7 @@ def switch_glu_fp8(x: torch.Tensor, indices: torch.Tensor, w_gu, s_gu, w_down, s
     kc = None if scores is None else scores.contiguous()
     L = _lib()
     with _on(x):
-        nbytes = L.kmi_switch_glu_fp8_workspace_bytes(T, H, I, k, E)
+        nbytes = _fp8_workspace("kmi_switch_glu_fp8_workspace_bytes", T, H, I, k, E)
         ws = _workspace(nbytes, x.device)
         _abi.check(L.kmi_switch_glu_fp8(_ptr(xc), T, H, I, k, _ptr(ic), _ptr(kc), _ptr(wg), _ptr(sg), _ptr(wd),
                                         _ptr(sd), e8, E, DTYPE_CODE[x.dtype], _ptr(out), _ptr(ws), nbytes,

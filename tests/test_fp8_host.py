@@ -97,10 +97,10 @@ def test_c_entries_refuse_on_the_host():
 
     def gather(**kw):
         return L.kmi_gather_qmm_fp8(*{**g, **kw}.values())
-    assert gather() == -3 and b"workspace" in L.kmi_last_error()
+    assert gather(P=400) == -3 and b"workspace" in L.kmi_last_error()
     assert gather(E=5000) == -1 and gather(E=0) == -1 and gather(K=8) == -1 and gather(P=1 << 40) == -1
     assert gather(l=None) == -1 and gather(P=0) == 0
-    assert L.kmi_gather_qmm_fp8_workspace_bytes(4, 4, 1, 4, 256, 64, 0) > 0
+    assert L.kmi_gather_qmm_fp8_workspace_bytes(400, 4, 1, 4, 256, 64, 0) > 0
     u = dict(x=16, T=4, H=256, I=128, k=2, i=16, sc=16, wg=16, sg=16, wd=16, sd=16, e8=0, E=4, dt=0, o=16, ws=None,
              n=0, st=None)
 
