@@ -26,7 +26,7 @@ FLAGS = [
 # D = 512 97.4 -> 80.2; the GEMMs and the VQ kernels measured even or slower
 # with it, and keep their accumulators in AGPRs).
 EXTRA = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for f in ("qgemv.hip", "qgemv_xs.hip", "qgemv_dl.hip", "kv8.hip",
-                                                                  "fp8_skinny.hip", "fp8_gemm.hip")}
+                                                                  "fp8_skinny.hip", "fp8_gemm.hip", "fp8_glu.hip")}
 
 
 # The compiler's per-kernel resource remarks (registers, scratch, occupancy),
@@ -39,7 +39,7 @@ RESOURCE_REMARKS = "-Rpass-analysis=kernel-resource-usage"
 # spill's scratch store or load above all -- sits among them.  Every kernel
 # compiled from a source (or a local header it includes) that names one of
 # these must use no scratch.
-DMA_MARKERS = ("buffer_load_lds", "wait_vmcnt<")
+DMA_MARKERS = ("buffer_load_lds", "wait_vmcnt<", "g_dma16")
 
 
 def sources():

@@ -96,7 +96,7 @@ int kmi_qmm_fp8(const void* x, int64_t M, int64_t K, int64_t N, const uint32_t* 
     a.x = x; a.xrows = M; a.y = y; a.rows = M; a.tm = p.tm; a.half = dtype == F16;
     if (!p.gemm) return launch_fp8_skinny(a, dtype, false, ceil_div(M, a.tm), st);
     rc = quantize_rows(a, x, dtype, M, (char*)workspace, st);
-    return rc ? rc : launch_fp8_gemm(a, false, ceil_div(M, a.tm), st);
+    return rc ? rc : launch_fp8_gemm(a, ceil_div(M, a.tm), st);
 }
 
 size_t kmi_gather_qmm_fp8_workspace_bytes(int64_t P, int64_t X, int64_t M, int64_t E, int64_t K, int64_t N,
@@ -141,7 +141,7 @@ int kmi_gather_qmm_fp8(const void* x, int64_t X, int64_t M, int64_t K, const uin
     }
     if (!p.gemm) return launch_fp8_skinny(a, dtype, false, sr.max_tiles, st);
     rc = quantize_rows(a, x, dtype, X * M, (char*)workspace + sort_index_bytes(P * M, E, p.tm), st);
-    return rc ? rc : launch_fp8_gemm(a, false, sr.max_tiles, st);
+    return rc ? rc : launch_fp8_gemm(a, sr.max_tiles, st);
 }
 
 size_t kmi_switch_glu_fp8_workspace_bytes(int64_t T, int64_t H, int64_t I, int k, int64_t E) {
@@ -197,9 +197,9 @@ int kmi_switch_glu_fp8(const void* x, int64_t T, int64_t H, int64_t I, int k, co
         ws += rows_bytes(T, H);
         d.x = g.y = ws; d.xld = I; d.xs_ld = g.ys_ld = fp8_row_scales(I);
         d.xs = g.ys = (unsigned char*)ws + align256((size_t)P * I);
-        rc = launch_fp8_gemm(g, true, sr.max_tiles, st);
+        rc = launch_fp8_glu(g, sr.max_tiles, st);
         if (rc) return rc;
-        rc = launch_fp8_gemm(d, false, sr.max_tiles, st);
+        rc = launch_fp8_gemm(d, sr.max_tiles, st);
     } else {
         if (p.pairs) {
             g.route = d.route = inds;

@@ -67,10 +67,12 @@ int64_t fp8_row_bytes(int64_t K);
 int64_t fp8_row_scales(int64_t K);
 int launch_fp8_rows(const void* x, int dtype, int64_t rows, int64_t K, unsigned char* q, unsigned char* s,
                     hipStream_t st);
-// K past which the row scales of a tile (128 bytes a block) crowd the LDS
-constexpr int64_t FP8_GEMM_MAX_K = 65536;
-// tiles of up to a.tm (64, 128 or 256; gate|up 128) rows over such rows
-int launch_fp8_gemm(const F8Args& a, bool glu, int64_t tiles, hipStream_t st);
+constexpr int64_t FP8_GEMM_MAX_K = 65536;     // a tile's rows within 32-bit offsets
+// tiles of up to a.tm (64, 128 or 256) rows over such rows
+int launch_fp8_gemm(const F8Args& a, int64_t tiles, hipStream_t st);
+// the gate|up products of expert tiles of up to 128 rows, and their activations
+// as codes and scale bytes
+int launch_fp8_glu(const F8Args& a, int64_t tiles, hipStream_t st);
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef short s16x2 __attribute__((ext_vector_type(2)));

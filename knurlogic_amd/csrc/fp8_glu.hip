@@ -1,0 +1,254 @@
+// The gate|up products of block-scaled E4M3 experts at prefill sizes: tiles of up to
+// 128 rows of one expert x 128 gate and 128 up rows, SwiGLU, and the activations
+// quantized for the down product.
+//
+// What these products are rounded to, E4M3 again, turns a small error of a sum into
+// an eighth of a value where a code falls to its neighbour; the 8-bit matrix
+// instructions drop too much of small products for that (fp8.hpp).  So the codes
+// are turned into bfloat16, which holds them exactly, x's with its row's scale (a
+// power of two), on their way from LDS to v_mfma_f32_32x32x16_bf16; a block's sums
+// meet the weights' scale in float32.
+//
+// 8 waves: 32 gate and 32 up rows x two blocks of 32 activation rows each (those
+// past the tile's rows are skipped: a tile's cost follows its rows).  A lane holds
+// its row's 64 bytes of a 128-input block in registers, so an LDS block is free
+// once they are read, a block ahead: two blocks' loads are in flight beside the one
+// that has landed.
+#include "fp8_tiles.hpp"
+
+namespace kmi {
+
+namespace {
+
+constexpr int U_TM = 128, U_STAGES = 3, U_WAVES = 8;
+constexpr int U_WTILE = 256 * F8_BLOCK, U_STAGE = U_WTILE + U_TM * F8_BLOCK;
+constexpr int U_WL = 256 / 8 / U_WAVES, U_XL = U_TM / 8 / U_WAVES;     // loads per wave and block
+constexpr int U_LDS = U_STAGES * U_STAGE + G_CHUNK * U_TM;
+constexpr int U_ROW = 272;                                             // bytes of an activation row in LDS, padded
+
+__device__ __forceinline__ bf16x8 u_operand(uint32_t lo, uint32_t hi, float scale) {      // 8 codes times scale
+    u32x4 r;
+    r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false));
+    r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true));
+    r.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false));
+    r.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true));
+    return as_bf16x8(r);
+}
+
+__global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks, int tiles) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ int rid_s[U_TM];
+    unsigned char* const sc = smem + U_STAGES * U_STAGE;      // [G_CHUNK][U_TM] scale bytes
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave & 3, wm = wave >> 2;
+    const int l32 = lane & 31, h = lane >> 5;
+    int tile, nb;
+    g_place((int)blockIdx.x, nblocks, tile, nb);
+    if (tile >= tiles) return;
+    const int32_t* tp = a.tiles + 3 * (int64_t)tile;
+    const int64_t expert = tp[0], start = tp[1];
+    const int count = __builtin_amdgcn_readfirstlane(tp[2]);
+    if (count <= 0) return;
+
+    const int K = (int)a.K, KB = (K + F8_BLOCK - 1) / F8_BLOCK;
+    const __amdgpu_buffer_rsrc_t rx = make_rsrc(a.x, a.xrows * a.xld);
+    // direct-to-LDS loads: 8 lanes per row, the lane's piece permuted by the row;
+    // LDS weight row 64 v + r: gate row 32 v + r of the block, r < 32, or up row
+    const int piece = (lane & 7) ^ (lane >> 3);
+    uint32_t xoff[U_XL], woff[U_WL];
+#pragma unroll
+    for (int j = 0; j < U_XL; j++) {
+        const int64_t r = g_xrow(a, start, count, 8 * (wave + U_WAVES * j) + (lane >> 3));
+        xoff[j] = r < 0 ? G_NONE : (uint32_t)(r * a.xld) + 16u * piece;
+    }
+    const int64_t n0 = (int64_t)nb * 128;                     // N is a multiple of 128
+    const __amdgpu_buffer_rsrc_t rg = make_rsrc(a.w + (expert * a.wrows + n0) * a.K, 128 * a.K);
+    const __amdgpu_buffer_rsrc_t ru = make_rsrc(a.w + (expert * a.wrows + n0 + a.N) * a.K, 128 * a.K);
+#pragma unroll
+    for (int j = 0; j < U_WL; j++) {
+        const int m = 8 * (wave + U_WAVES * j) + (lane >> 3);
+        woff[j] = (uint32_t)((m >> 6) * 32 + (m & 31)) * (uint32_t)K + 16u * piece;
+    }
+    auto issue = [&](int t) {                                 // block t (past the last: zeros)
+        unsigned char* dst = smem + (t % U_STAGES) * U_STAGE;
+        const bool in = t * F8_BLOCK + 16 * piece < K;        // inputs past the last: zeros
+#pragma unroll
+        for (int j = 0; j < U_WL; j++) {
+            const int m = 8 * (wave + U_WAVES * j);           // (bit 5: up)
+            g_dma16(m & 32 ? ru : rg, dst + m * F8_BLOCK, in ? woff[j] : G_NONE, (uint32_t)t * F8_BLOCK);
+        }
+#pragma unroll
+        for (int j = 0; j < U_XL; j++)
+            g_dma16(rx, dst + U_WTILE + (wave + U_WAVES * j) * 1024, t < KB ? xoff[j] : G_NONE, (uint32_t)t * F8_BLOCK);
+    };
+#pragma unroll
+    for (int t = 0; t < U_STAGES; t++) issue(t);
+    // the weights' scales, 64 blocks, one per lane (gate, up), and x's scale bytes
+    const int64_t SB = (a.wrows + F8_BLOCK - 1) / F8_BLOCK;
+    const int64_t sbase = (expert * SB + nb) * KB;
+    float swl[2];
+    auto load_scales = [&](int t) {
+        const int k = t + lane < KB ? t + lane : KB - 1;
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+            const int64_t i = sbase + (g ? a.N / F8_BLOCK * KB : 0) + k;
+            swl[g] = a.e8 ? e8m0_to_f32(((const unsigned char*)a.s)[i]) : ((const float*)a.s)[i];
+            asm volatile("" : "+v"(swl[g]));                  // waited for here, not in the loop
+        }
+        for (int m = tid & (U_TM - 1), q = tid / U_TM; q < G_CHUNK / 4 && t + 4 * q < KB; q += 64 * U_WAVES / U_TM) {
+            const int64_t r = g_xrow(a, start, count, m);
+            const uint32_t v = r < 0 ? 0x7f7f7f7fu : *(const uint32_t*)(a.xs + r * a.xs_ld + t + 4 * q);
+#pragma unroll
+            for (int b = 0; b < 4; b++) sc[(4 * q + b) * U_TM + m] = (unsigned char)(v >> (8 * b));
+        }
+    };
+    load_scales(0);
+    if (tid < U_TM) rid_s[tid] = tid < count ? a.sorted[start + tid] : -1;
+
+    // this lane's row of fragment i (weights) or j (x rows 32 (wm + 2 j) ..): bytes
+    // 64 h .. of a block, in 16-byte pieces 4 h + q
+    uint32_t wo[4], xo[4];
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        const uint32_t p = 16u * ((4 * h + q) ^ (l32 & 7));
+        wo[q] = (uint32_t)(64 * wn + l32) * F8_BLOCK + p;
+        xo[q] = U_WTILE + (uint32_t)(32 * wm + l32) * F8_BLOCK + p;
+    }
+    f32x16 acc[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) acc[i][j][r] = 0.f;
+
+    // NJ: this wave's blocks of 32 activation rows
+    auto run = [&](auto nj) {
+        constexpr int NJ = decltype(nj)::value;
+        u32x4 w[2][4], x[NJ ? NJ : 1][4];
+        uint32_t xb[NJ ? NJ : 1];
+        auto read = [&](int t, int q) {                       // piece q of every fragment
+            const unsigned char* st = smem + (t % U_STAGES) * U_STAGE;
+#pragma unroll
+            for (int i = 0; i < 2; i++) w[i][q] = *(const u32x4*)(st + i * 4096 + wo[q]);
+#pragma unroll
+            for (int j = 0; j < NJ; j++) x[j][q] = *(const u32x4*)(st + j * 8192 + xo[q]);
+        };
+        auto read_scales = [&](int t) {
+#pragma unroll
+            for (int j = 0; j < NJ; j++) xb[j] = sc[t % G_CHUNK * U_TM + 32 * (wm + 2 * j) + l32];
+        };
+        g_wait<(U_STAGES - 1) * (U_WL + U_XL)>();
+        lds_barrier();
+        if constexpr (NJ > 0)
+            for (int q = 0; q < 4; q++) read(0, q);
+        for (int t0 = 0; t0 < KB; t0 += G_CHUNK) {
+            if (t0) {                                         // every wave is past its reads of the last chunk's scales
+                load_scales(t0);
+                lds_barrier();
+            }
+            const int t1 = t0 + G_CHUNK < KB ? t0 + G_CHUNK : KB;
+            for (int t = t0; t < t1; t++) {
+                if constexpr (NJ > 0) read_scales(t);
+                // this block is in registers everywhere and the next one has landed
+                g_wait<(U_STAGES - 2) * (U_WL + U_XL)>();
+                lds_barrier();
+                issue(t + U_STAGES);
+                if constexpr (NJ > 0) {
+                    float sx[NJ];
+#pragma unroll
+                    for (int j = 0; j < NJ; j++) sx[j] = __uint_as_float(xb[j] << 23);
+                    f32x16 p[2][NJ];
+#pragma unroll
+                    for (int i = 0; i < 2; i++)
+#pragma unroll
+                        for (int j = 0; j < NJ; j++)
+#pragma unroll
+                            for (int r = 0; r < 16; r++) p[i][j][r] = 0.f;
+#pragma unroll
+                    for (int s = 0; s < 8; s++) {
+                        bf16x8 wv[2], xv[NJ];
+#pragma unroll
+                        for (int i = 0; i < 2; i++) wv[i] = u_operand(w[i][s / 2][s % 2 * 2], w[i][s / 2][s % 2 * 2 + 1], 1.f);
+#pragma unroll
+                        for (int j = 0; j < NJ; j++) xv[j] = u_operand(x[j][s / 2][s % 2 * 2], x[j][s / 2][s % 2 * 2 + 1], sx[j]);
+#pragma unroll
+                        for (int i = 0; i < 2; i++)
+#pragma unroll
+                            for (int j = 0; j < NJ; j++)
+                                p[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wv[i], xv[j], p[i][j], 0, 0, 0);
+                        if (s % 2) read(t + 1, s / 2);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const float sw = __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(swl[i]), t % G_CHUNK));
+#pragma unroll
+                        for (int j = 0; j < NJ; j++)
+#pragma unroll
+                            for (int r = 0; r < 16; r++) acc[i][j][r] = __builtin_fmaf(p[i][j][r], sw, acc[i][j][r]);
+                    }
+                }
+            }
+        }
+    };
+    const int blocks = (count + 31) / 32, nj = (blocks - wm + 1) / 2;
+    if (nj == 2) run(std::integral_constant<int, 2>());
+    else if (nj == 1) run(std::integral_constant<int, 1>());
+    else run(std::integral_constant<int, 0>());
+    g_wait<0>();                                 // no load still writes LDS below
+    lds_barrier();
+
+    // activations of 128 columns per row through LDS, where 16 lanes quantize a
+    // row's group.  D: row 8 (r / 4) + 4 h + r % 4 of the fragment, x row l % 32
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        if (j >= nj) break;
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            uint32_t o[2];
+#pragma unroll
+            for (int q = 0; q < 2; q++) {
+                const uint32_t g = cvt_pk_bf16(acc[0][j][r + 2 * q], acc[0][j][r + 2 * q + 1]);
+                const uint32_t u = cvt_pk_bf16(acc[1][j][r + 2 * q], acc[1][j][r + 2 * q + 1]);
+                o[q] = cvt_pk_bf16(silu_bf16r(__uint_as_float(g << 16)) * __uint_as_float(u << 16),
+                                   silu_bf16r(__uint_as_float(g & 0xffff0000u)) * __uint_as_float(u & 0xffff0000u));
+            }
+            *(u32x2*)(smem + (32 * (wm + 2 * j) + l32) * U_ROW + (32 * wn + 2 * r + 4 * h) * 2) = u32x2{o[0], o[1]};
+        }
+    }
+    lds_barrier();
+    const int l16 = tid & 15;
+    for (int m = tid >> 4; m < count; m += 4 * U_WAVES) {
+        F8Raw<F8BF16, 8> v;
+        v.v[0] = *(const u32x4*)(smem + m * U_ROW + 16 * l16);
+        uint32_t byte = f8_scale_byte(f8_max16(v.amax()));
+        const bool nan = byte == 255;            // as f8_rows
+        if (nan) byte = 127;
+        const float scale = __uint_as_float(byte << 23);
+        unsigned char* y = (unsigned char*)a.y + (int64_t)rid_s[m] * a.N + nb * 128 + 8 * l16;
+        *(u32x2*)y = nan ? u32x2{0x7f7f7f7fu, 0x7f7f7f7fu} : u32x2{v.codes(0, scale), v.codes(1, scale)};
+        if (l16 == 0) a.ys[(int64_t)rid_s[m] * a.ys_ld + nb] = (unsigned char)byte;
+    }
+}
+
+}  // namespace
+
+int launch_fp8_glu(const F8Args& a, int64_t tiles, hipStream_t st) {
+    if (!a.tiles || a.K > FP8_GEMM_MAX_K || a.xld != fp8_row_bytes(a.K) || a.tm != U_TM || a.N % 128 ||
+        a.xrows * a.xld >= (1LL << 31)) {
+        set_error("fp8: gate|up tiles of %d rows, K=%lld, N=%lld", a.tm, (long long)a.K, (long long)a.N);
+        return EINVAL_ARG;
+    }
+    const int64_t nblocks = a.N / 128, wgs = g_place_grid(tiles, nblocks);
+    if (wgs >= (1LL << 31)) {
+        set_error("fp8: grid of %lld workgroups", (long long)wgs);
+        return EINVAL_ARG;
+    }
+    allow_dynamic_lds_once((const void*)f8_glu);
+    f8_glu<<<(unsigned)wgs, 64 * U_WAVES, U_LDS, st>>>(a, (int)nblocks, (int)tiles);
+    KMI_CHECK_LAUNCH("fp8 gate|up");
+    return OK;
+}
+
+}  // namespace kmi

@@ -970,20 +970,22 @@ def _qmm_fp8(x, w, scales, biases, transpose, group_size, bits):
         raise ValueError(f"{what}: fp8 takes a 2-D weight with transpose=True (got {tuple(w.shape)}, "
                          f"transpose={transpose})")
     wq, sc, e8 = _check_fp8(what, w, scales, biases, group_size, bits)
-    N, K = wq.shape[0], wq.shape[1] * 4
+    N, words = wq.shape
+    K = words * 4
     _one_device(what, x, wq, sc)
     xc = _fp8_x(what, x, K)
     y = x.new_empty((*x.shape[:-1], N))
-    if y.numel() == 0:
+    total = y.numel()
+    if total == 0:
         return y
-    M = xc.numel() // K if K else 0
-    L = _lib()
     code = DTYPE_CODE[x.dtype]
     with _on(x):
-        nbytes = _fp8_workspace("kmi_qmm_fp8_workspace_bytes", M, K, N, code)
-        ws = _workspace(nbytes, x.device)
-        _abi.check(L.kmi_qmm_fp8(_ptr(xc), M, K, N, _ptr(wq), _ptr(sc), e8, code, _ptr(y), _ptr(ws), nbytes,
-                                 _stream(x)), what)
+        nbytes = _fp8_workspace("kmi_qmm_fp8_workspace_bytes", total // N, K, N, code)
+        ws = _workspace(nbytes, x.device) if nbytes else None
+        rc = _lib().kmi_qmm_fp8(xc.data_ptr(), total // N, K, N, wq.data_ptr(), sc.data_ptr(), e8, code,
+                                y.data_ptr(), _ptr(ws), nbytes, _stream(x))
+        if rc:
+            _abi.check(rc, what)
     return y
 
 
@@ -1021,39 +1023,41 @@ def switch_glu_fp8(x: torch.Tensor, indices: torch.Tensor, w_gu, s_gu, w_down, s
     The same results as ``gather_qmm``, ``swiglu``, ``gather_qmm`` and
     ``moe_combine`` in turn."""
     what = "switch_glu_fp8"
-    if x.dtype != torch.bfloat16:
+    if x.dtype is not torch.bfloat16:
         raise ValueError(f"{what}: only bfloat16 activations are implemented")
     wg, sg, e8 = _check_fp8(what, w_gu, s_gu, None, FP8_BLOCK, 8)
     wd, sd, e8d = _check_fp8(what, w_down, s_down, None, FP8_BLOCK, 8)
     if e8 != e8d:
         raise ValueError(f"{what}: both weights' scales must be float32, or both uint8")
     _one_device(what, x, indices, wg, sg, wd, sd, scores)
-    lead, H = tuple(x.shape[:-1]), x.shape[-1]
-    if indices.ndim < 1 or tuple(indices.shape[:-1]) != lead or indices.dtype.is_floating_point:
+    xshape, ishape = x.shape, indices.shape
+    lead, H = xshape[:-1], xshape[-1]
+    if not ishape or ishape[:-1] != lead or indices.dtype.is_floating_point:
         raise ValueError(f"{what}: integer indices [..., k] must match x [..., H]")
-    k = indices.shape[-1]
+    k = ishape[-1]
     if wg.ndim != 3 or wd.ndim != 3:
         raise ValueError(f"{what}: w_gu and w_down must be [E, rows, words]")
     E, I = wg.shape[0], wd.shape[2] * 4
-    if tuple(wg.shape) != (E, 2 * I, H // 4) or tuple(wd.shape) != (E, H, I // 4) or H % 16 or I % FP8_BLOCK:
+    if wg.shape != (E, 2 * I, H // 4) or wd.shape != (E, H, I // 4) or H % 16 or I % FP8_BLOCK:
         raise ValueError(f"{what}: w_gu {tuple(wg.shape)} and w_down {tuple(wd.shape)} for x of {H} features "
                          f"(H in multiples of 16, I of {FP8_BLOCK})")
-    if scores is not None and (scores.shape != indices.shape or scores.dtype != x.dtype):
+    if scores is not None and (scores.shape != ishape or scores.dtype != x.dtype):
         raise ValueError(f"{what}: scores must match indices in shape and x in dtype")
+    out = x.new_empty(xshape if scores is not None else (*ishape, H))
     T = math.prod(lead)
-    out = torch.empty((*lead, H) if scores is not None else (*lead, k, H), dtype=x.dtype, device=x.device)
-    if T == 0 or k == 0:
+    if T == 0 or k == 0 or H == 0:
         return out.zero_()
     xc = _aligned16(x)
-    ic = indices.reshape(T, k).to(torch.int32).contiguous()
+    ic = (indices if indices.dtype is torch.int32 else indices.to(torch.int32)).contiguous()
     kc = None if scores is None else scores.contiguous()
-    L = _lib()
     with _on(x):
         nbytes = _fp8_workspace("kmi_switch_glu_fp8_workspace_bytes", T, H, I, k, E)
-        ws = _workspace(nbytes, x.device)
-        _abi.check(L.kmi_switch_glu_fp8(_ptr(xc), T, H, I, k, _ptr(ic), _ptr(kc), _ptr(wg), _ptr(sg), _ptr(wd),
-                                        _ptr(sd), e8, E, DTYPE_CODE[x.dtype], _ptr(out), _ptr(ws), nbytes,
-                                        _stream(x)), what)
+        ws = x.new_empty(nbytes // 2)                  # (a multiple of 256 bytes)
+        rc = _lib().kmi_switch_glu_fp8(xc.data_ptr(), T, H, I, k, ic.data_ptr(), _ptr(kc), wg.data_ptr(),
+                                       sg.data_ptr(), wd.data_ptr(), sd.data_ptr(), e8, E, 0, out.data_ptr(),
+                                       ws.data_ptr(), nbytes, _stream(x))
+        if rc:
+            _abi.check(rc, what)
     return out
 
 
