@@ -133,7 +133,7 @@ int kmi_gather_qmm_fp8(const void* x, int64_t X, int64_t M, int64_t K, const uin
     F8Args a = {};
     a.w = (const unsigned char*)w; a.s = scales; a.e8 = e8m0; a.E = E; a.wrows = N; a.K = K; a.N = N;
     a.x = x; a.xrows = X * M; a.y = y; a.rows = P * M; a.tm = p.tm; a.half = dtype == F16;
-    a.tiles = sr.tiles; a.sorted = sr.sorted; a.lhs = lhs; a.lhs_div = 1; a.Mper = M;
+    a.tiles = sr.tiles; a.sorted = sr.sorted; a.lhs = lhs; a.lhs_div = 1; a.lhs_inv = 1.0; a.Mper = M;
     if (p.pairs) {
         a.route = rhs;
         a.tm = 1;
@@ -187,10 +187,10 @@ int kmi_switch_glu_fp8(const void* x, int64_t T, int64_t H, int64_t I, int k, co
     F8Args g = {};
     g.w = (const unsigned char*)w_gu; g.s = s_gu; g.e8 = e8m0; g.E = E; g.wrows = 2 * I; g.K = H; g.N = I;
     g.x = x; g.xrows = T; g.rows = P; g.tm = p.tm;
-    g.tiles = sr.tiles; g.sorted = sr.sorted; g.lhs_div = k; g.Mper = 1;
+    g.tiles = sr.tiles; g.sorted = sr.sorted; g.lhs_div = k; g.lhs_inv = 1.0 / k; g.Mper = 1;
     F8Args d = g;
     d.w = (const unsigned char*)w_down; d.s = s_down; d.wrows = H; d.K = I; d.N = H; d.xrows = P; d.y = y;
-    d.lhs_div = 1;
+    d.lhs_div = 1; d.lhs_inv = 1.0;
     if (p.gemm) {
         rc = quantize_rows(g, x, dtype, T, ws, st);
         if (rc) return rc;

@@ -36,6 +36,7 @@ struct F8Args {
     const int32_t* sorted;
     const int32_t* lhs;
     int64_t lhs_div, Mper;
+    double lhs_inv;             // 1.0 / lhs_div (the tiled kernels)
     int tm;
     // f8_stream, instead of tiles: the expert of each of the `rows` pairs; tile z =
     // pair z, of x row (lhs ? lhs[z] : z / lhs_div)
@@ -64,7 +65,7 @@ int launch_fp8_combine(const F8Args& a, const void* scores, int k, int64_t T, vo
 // Rows quantized ahead: codes in rows of fp8_row_bytes (a multiple of 128, the
 // tail zero) and scale bytes in rows of fp8_row_scales.
 int64_t fp8_row_bytes(int64_t K);
-int64_t fp8_row_scales(int64_t K);
+int64_t fp8_row_scales(int64_t K);             // (a multiple of 16)
 int launch_fp8_rows(const void* x, int dtype, int64_t rows, int64_t K, unsigned char* q, unsigned char* s,
                     hipStream_t st);
 constexpr int64_t FP8_GEMM_MAX_K = 65536;     // a tile's rows within 32-bit offsets
@@ -94,14 +95,6 @@ __device__ __forceinline__ f32x4 f8_mfma(i32x8 a, i32x8 b, f32x4 c, uint32_t sa,
 
 __device__ __forceinline__ i32x8 f8_operand(u32x4 lo, u32x4 hi) {
     return i32x8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
-}
-
-// the same with B's scale in byte `at` (a constant) of sb
-__device__ __forceinline__ f32x4 f8_mfma_at(i32x8 a, i32x8 b, f32x4 c, uint32_t sa, uint32_t sb, int at) {
-    if (at == 0) return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, (int)sa, 0, (int)sb);
-    if (at == 1) return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, (int)sa, 1, (int)sb);
-    if (at == 2) return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, (int)sa, 2, (int)sb);
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, (int)sa, 3, (int)sb);
 }
 
 // max over each 16 neighbouring lanes, by rotations of a row of lanes (a shuffle

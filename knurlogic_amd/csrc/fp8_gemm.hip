@@ -37,7 +37,7 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
     constexpr int RB = 4, TN = Z::TN, TM = Z::TM, XL = Z::XL, WL = Z::WL, WAVES = Z::WAVES, WTILE = Z::WTILE;
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ int rid_s[TM];
-    unsigned char* const sc = smem + S * Z::STAGE;            // [G_CHUNK][WM][16][MB] scale bytes
+    unsigned char* const sc = smem + S * Z::STAGE;            // [G_CHUNK / 16][TM][16] scale bytes
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave % NW, wm = wave / NW;
     const int l16 = lane & 15, c = lane >> 4;
@@ -55,28 +55,37 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
         tile = 8 * strip + in % height;
         nb = in / height;
     }
-    int64_t expert = 0, start = (int64_t)tile * a.tm;
-    int count = (int)(a.rows - start < a.tm ? a.rows - start : a.tm);
-    if (a.tiles) {
-        const int32_t* t = a.tiles + 3 * (int64_t)tile;
-        expert = t[0]; start = t[1]; count = t[2];
-    }
+    const GTile T = g_tile(a, tile);
+    const int count = T.count;
     if (count <= 0) return;
 
     const int K = (int)a.K, KB = (K + F8_BLOCK - 1) / F8_BLOCK;
-    const int64_t x0 = a.tiles ? 0 : start;                   // the x view's first row
-    auto xrow = [&](int m) { return g_xrow(a, start, count, m); };
-    // direct-to-LDS loads: 8 lanes per row, the lane's piece permuted by the row
+    const int64_t x0 = a.tiles ? 0 : T.start;                 // the x view's first row
+    // the weights' scales of the wave's rows, 64 blocks, one per lane
+    const int64_t n0 = (int64_t)nb * TN, left = a.N - n0 < TN ? a.N - n0 : TN;
+    const int64_t SB = (a.wrows + F8_BLOCK - 1) / F8_BLOCK, nw = n0 + 64 * wn;
+    const int64_t sbase = (T.expert * SB + (nw < a.N ? nw : n0) / F8_BLOCK) * KB;
+    uint32_t swl;
+    auto load_scales = [&](int t) {
+        const int64_t i = sbase + (t + lane < KB ? t + lane : KB - 1);
+        if (KIND == E8S) swl = ((const unsigned char*)a.s)[i];
+        else swl = ((const uint32_t*)a.s)[i];
+        asm volatile("" : "+v"(swl));            // waited for here, not in the loop
+    };
+    load_scales(0);
+    if (tid < TM) rid_s[tid] = tid >= count ? -1 : a.tiles ? a.sorted[T.start + tid] : (int)(T.start + tid);
+    // direct-to-LDS loads: 8 lanes per row, the lane's piece permuted by the row.
+    // (From here on the compiler's counts miss what is in flight: no load that it
+    // would wait for.)
     const int piece = (lane & 7) ^ (lane >> 3);               // (row % 8 == lane / 8)
     const __amdgpu_buffer_rsrc_t rx = make_rsrc((const unsigned char*)a.x + x0 * a.xld, (a.xrows - x0) * a.xld);
+    const __amdgpu_buffer_rsrc_t rw = make_rsrc(a.w + (T.expert * a.wrows + n0) * a.K, left * a.K);
     uint32_t xoff[XL], woff[WL];
 #pragma unroll
     for (int j = 0; j < XL; j++) {
-        const int64_t r = xrow(8 * (wave + WAVES * j) + (lane >> 3));
+        const int64_t r = g_xrow(a, T, 8 * (wave + WAVES * j) + (lane >> 3));
         xoff[j] = r < 0 ? G_NONE : (uint32_t)((r - x0) * a.xld) + 16u * piece;
     }
-    const int64_t n0 = (int64_t)nb * TN, left = a.N - n0 < TN ? a.N - n0 : TN;
-    const __amdgpu_buffer_rsrc_t rw = make_rsrc(a.w + (expert * a.wrows + n0) * a.K, left * a.K);
 #pragma unroll
     for (int j = 0; j < WL; j++) {
         const int m = 8 * (wave + WAVES * j) + (lane >> 3);
@@ -92,29 +101,9 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
         for (int j = 0; j < XL; j++)
             g_dma16(rx, dst + WTILE + (wave + WAVES * j) * 1024, t < KB ? xoff[j] : G_NONE, (uint32_t)t * F8_BLOCK);
     };
+    g_scales<TM, WAVES>(a, T, sc, 0, KB, wave, lane);
 #pragma unroll
     for (int t = 0; t < S; t++) issue(t);
-    // the weights' scales of the wave's rows, 64 blocks, one per lane, and the scale
-    // bytes of x's rows
-    const int64_t SB = (a.wrows + F8_BLOCK - 1) / F8_BLOCK, nw = n0 + 64 * wn;
-    const int64_t sbase = (expert * SB + (nw < a.N ? nw : n0) / F8_BLOCK) * KB;
-    uint32_t swl;
-    auto load_scales = [&](int t) {
-        const int64_t i = sbase + (t + lane < KB ? t + lane : KB - 1);
-        if (KIND == E8S) swl = ((const unsigned char*)a.s)[i];
-        else swl = ((const uint32_t*)a.s)[i];
-        asm volatile("" : "+v"(swl));            // waited for here, not in the loop
-        for (int m = tid & (TM - 1), q = tid / TM; q < G_CHUNK / 4 && t + 4 * q < KB; q += 64 * WAVES / TM) {
-            const int64_t r = xrow(m);
-            const uint32_t v = r < 0 ? 0x7f7f7f7fu : *(const uint32_t*)(a.xs + r * a.xs_ld + t + 4 * q);
-            const int w = m / (16 * MB), j = m / 16 % MB;
-#pragma unroll
-            for (int b = 0; b < 4; b++)
-                sc[(((4 * q + b) * WM + w) * 16 + (m & 15)) * MB + j] = (unsigned char)(v >> (8 * b));
-        }
-    };
-    load_scales(0);
-    if (tid < TM) rid_s[tid] = tid >= count ? -1 : a.tiles ? a.sorted[start + tid] : (int)(start + tid);
 
     // fragment reads: weight row 64 wn + 16 i + l16, pieces c and c + 4; x row
     // 16 (MB wm + j) + l16, the same
@@ -146,22 +135,18 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
     for (int t0 = 0; t0 < KB; t0 += G_CHUNK) {
     if (t0) {                                    // every wave is past its reads of the last chunk's scales
         load_scales(t0);
+        g_scales<TM, WAVES>(a, T, sc, t0, KB, wave, lane);
+        g_wait<0>();
         lds_barrier();
     }
     const int t1 = t0 + G_CHUNK < KB ? t0 + G_CHUNK : KB;
     for (int t = t0; t < t1; t++) {              // (no branch inside: the compiler would sink products past it)
         const unsigned char* st = smem + (t % S) * Z::STAGE;
         const unsigned char* nx = smem + ((t + 1) % S) * Z::STAGE;
-        uint32_t sx[(MB + 3) / 4];
-        const unsigned char* sp = sc + ((t % G_CHUNK * WM + wm) * 16 + l16) * MB;
-        if constexpr (MB == 2) {
-            sx[0] = *(const uint16_t*)sp;
-        } else {
+        uint32_t sx[MB];
 #pragma unroll
-            for (int q = 0; q < MB / 4; q++) sx[q] = *(const uint32_t*)(sp + 4 * q);
-        }
+        for (int j = 0; j < MB; j++) sx[j] = g_scale(sc, TM, 16 * (MB * wm + j) + l16, t);
         const uint32_t sw = (uint32_t)__builtin_amdgcn_readlane((int)swl, t % G_CHUNK);
-        auto row_scale = [&](int j) { return __uint_as_float((sx[j / 4] >> (8 * (j & 3)) & 0xffu) << 23); };
         // after the block's last LDS read: the next block has landed, and this
         // one's place is free
         auto turn = [&]() {
@@ -188,9 +173,9 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
                 }
                 if (n == NP - RB) read_b(nx, 0);
                 if constexpr (KIND == E8S) {
-                    acc[i][j] = f8_mfma_at(w[i], b[j & 1], acc[i][j], sw, sx[j / 4], j & 3);
+                    acc[i][j] = f8_mfma(w[i], b[j & 1], acc[i][j], sw, sx[j]);
                 } else {
-                    if (i == 0) f[j & 1] = row_scale(j) * __uint_as_float(sw);
+                    if (i == 0) f[j & 1] = __uint_as_float(sx[j] << 23) * __uint_as_float(sw);
                     p[n % 3] = f8_mfma(w[i], b[j & 1], f32x4{0.f, 0.f, 0.f, 0.f}, 127u, 127u);
                     if (n >= 2) apply(n - 2);
                 }
@@ -214,7 +199,7 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
             const int m = 16 * (MB * wm + j) + l16;
             const int rid = rid_s[m];
             if (rid < 0) continue;
-            const bool seen = !a.lhs || xrow(m) >= 0;
+            const bool seen = !a.lhs || g_xrow(a, T, m) >= 0;
 #pragma unroll
             for (int i = 0; i < RB; i++) {
                 const int64_t n = n0 + 64 * wn + 16 * i + 4 * c;
@@ -290,7 +275,7 @@ int go(const F8Args& a, int64_t tiles, hipStream_t st) {
 }  // namespace
 
 int64_t fp8_row_bytes(int64_t K) { return ceil_div(K, F8_BLOCK) * F8_BLOCK; }
-int64_t fp8_row_scales(int64_t K) { return ceil_div(ceil_div(K, F8_BLOCK), 4) * 4; }
+int64_t fp8_row_scales(int64_t K) { return ceil_div(ceil_div(K, F8_BLOCK), 16) * 16; }
 
 int launch_fp8_rows(const void* x, int dtype, int64_t rows, int64_t K, unsigned char* q, unsigned char* s,
                     hipStream_t st) {

@@ -38,32 +38,49 @@ __device__ __forceinline__ bf16x8 u_operand(uint32_t lo, uint32_t hi, float scal
 __global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks, int tiles) {
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ int rid_s[U_TM];
-    unsigned char* const sc = smem + U_STAGES * U_STAGE;      // [G_CHUNK][U_TM] scale bytes
+    unsigned char* const sc = smem + U_STAGES * U_STAGE;      // [G_CHUNK / 16][U_TM][16] scale bytes
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave & 3, wm = wave >> 2;
     const int l32 = lane & 31, h = lane >> 5;
     int tile, nb;
     g_place((int)blockIdx.x, nblocks, tile, nb);
     if (tile >= tiles) return;
-    const int32_t* tp = a.tiles + 3 * (int64_t)tile;
-    const int64_t expert = tp[0], start = tp[1];
-    const int count = __builtin_amdgcn_readfirstlane(tp[2]);
+    const GTile T = g_tile(a, tile);
+    const int count = T.count;
     if (count <= 0) return;
 
     const int K = (int)a.K, KB = (K + F8_BLOCK - 1) / F8_BLOCK;
-    const __amdgpu_buffer_rsrc_t rx = make_rsrc(a.x, a.xrows * a.xld);
+    // the weights' scales, 64 blocks, one per lane (gate, up)
+    const int64_t SB = (a.wrows + F8_BLOCK - 1) / F8_BLOCK;
+    const int64_t sbase = (T.expert * SB + nb) * KB;
+    float swl[2];
+    auto load_scales = [&](int t) {
+        const int k = t + lane < KB ? t + lane : KB - 1;
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+            const int64_t i = sbase + (g ? a.N / F8_BLOCK * KB : 0) + k;
+            swl[g] = a.e8 ? e8m0_to_f32(((const unsigned char*)a.s)[i]) : ((const float*)a.s)[i];
+        }
+#pragma unroll
+        for (int g = 0; g < 2; g++) asm volatile("" : "+v"(swl[g]));      // waited for here, not in the loop
+    };
+    load_scales(0);
+    if (tid < U_TM) rid_s[tid] = tid < count ? a.sorted[T.start + tid] : -1;
     // direct-to-LDS loads: 8 lanes per row, the lane's piece permuted by the row;
-    // LDS weight row 64 v + r: gate row 32 v + r of the block, r < 32, or up row
+    // LDS weight row 64 v + r: gate row 32 v + r of the block, r < 32, or up row.
+    // (From here on the compiler's counts miss what is in flight: no load that it
+    // would wait for.)
     const int piece = (lane & 7) ^ (lane >> 3);
+    const int64_t n0 = (int64_t)nb * 128;                     // N is a multiple of 128
+    const __amdgpu_buffer_rsrc_t rx = make_rsrc(a.x, a.xrows * a.xld);
+    const __amdgpu_buffer_rsrc_t rg = make_rsrc(a.w + (T.expert * a.wrows + n0) * a.K, 128 * a.K);
+    const __amdgpu_buffer_rsrc_t ru = make_rsrc(a.w + (T.expert * a.wrows + n0 + a.N) * a.K, 128 * a.K);
     uint32_t xoff[U_XL], woff[U_WL];
 #pragma unroll
     for (int j = 0; j < U_XL; j++) {
-        const int64_t r = g_xrow(a, start, count, 8 * (wave + U_WAVES * j) + (lane >> 3));
+        const int64_t r = g_xrow(a, T, 8 * (wave + U_WAVES * j) + (lane >> 3));
         xoff[j] = r < 0 ? G_NONE : (uint32_t)(r * a.xld) + 16u * piece;
     }
-    const int64_t n0 = (int64_t)nb * 128;                     // N is a multiple of 128
-    const __amdgpu_buffer_rsrc_t rg = make_rsrc(a.w + (expert * a.wrows + n0) * a.K, 128 * a.K);
-    const __amdgpu_buffer_rsrc_t ru = make_rsrc(a.w + (expert * a.wrows + n0 + a.N) * a.K, 128 * a.K);
 #pragma unroll
     for (int j = 0; j < U_WL; j++) {
         const int m = 8 * (wave + U_WAVES * j) + (lane >> 3);
@@ -81,29 +98,9 @@ __global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks,
         for (int j = 0; j < U_XL; j++)
             g_dma16(rx, dst + U_WTILE + (wave + U_WAVES * j) * 1024, t < KB ? xoff[j] : G_NONE, (uint32_t)t * F8_BLOCK);
     };
+    g_scales<U_TM, U_WAVES>(a, T, sc, 0, KB, wave, lane);
 #pragma unroll
     for (int t = 0; t < U_STAGES; t++) issue(t);
-    // the weights' scales, 64 blocks, one per lane (gate, up), and x's scale bytes
-    const int64_t SB = (a.wrows + F8_BLOCK - 1) / F8_BLOCK;
-    const int64_t sbase = (expert * SB + nb) * KB;
-    float swl[2];
-    auto load_scales = [&](int t) {
-        const int k = t + lane < KB ? t + lane : KB - 1;
-#pragma unroll
-        for (int g = 0; g < 2; g++) {
-            const int64_t i = sbase + (g ? a.N / F8_BLOCK * KB : 0) + k;
-            swl[g] = a.e8 ? e8m0_to_f32(((const unsigned char*)a.s)[i]) : ((const float*)a.s)[i];
-            asm volatile("" : "+v"(swl[g]));                  // waited for here, not in the loop
-        }
-        for (int m = tid & (U_TM - 1), q = tid / U_TM; q < G_CHUNK / 4 && t + 4 * q < KB; q += 64 * U_WAVES / U_TM) {
-            const int64_t r = g_xrow(a, start, count, m);
-            const uint32_t v = r < 0 ? 0x7f7f7f7fu : *(const uint32_t*)(a.xs + r * a.xs_ld + t + 4 * q);
-#pragma unroll
-            for (int b = 0; b < 4; b++) sc[(4 * q + b) * U_TM + m] = (unsigned char)(v >> (8 * b));
-        }
-    };
-    load_scales(0);
-    if (tid < U_TM) rid_s[tid] = tid < count ? a.sorted[start + tid] : -1;
 
     // this lane's row of fragment i (weights) or j (x rows 32 (wm + 2 j) ..): bytes
     // 64 h .. of a block, in 16-byte pieces 4 h + q
@@ -136,7 +133,7 @@ __global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks,
         };
         auto read_scales = [&](int t) {
 #pragma unroll
-            for (int j = 0; j < NJ; j++) xb[j] = sc[t % G_CHUNK * U_TM + 32 * (wm + 2 * j) + l32];
+            for (int j = 0; j < NJ; j++) xb[j] = g_scale(sc, U_TM, 32 * (wm + 2 * j) + l32, t);
         };
         g_wait<(U_STAGES - 1) * (U_WL + U_XL)>();
         lds_barrier();
@@ -145,6 +142,8 @@ __global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks,
         for (int t0 = 0; t0 < KB; t0 += G_CHUNK) {
             if (t0) {                                         // every wave is past its reads of the last chunk's scales
                 load_scales(t0);
+                g_scales<U_TM, U_WAVES>(a, T, sc, t0, KB, wave, lane);
+                g_wait<0>();
                 lds_barrier();
             }
             const int t1 = t0 + G_CHUNK < KB ? t0 + G_CHUNK : KB;

@@ -27,15 +27,61 @@ __device__ __forceinline__ void g_dma16(__amdgpu_buffer_rsrc_t r, unsigned char*
                  ::"s"(at), "v"(voff), "s"(r), "s"(soff) : "memory", "m0");
 }
 
-// x row of row m of a tile of `count` rows from `start`, or -1
-__device__ __forceinline__ int64_t g_xrow(const F8Args& a, int64_t start, int count, int m) {
-    if (m >= count) return -1;
-    if (!a.tiles) return start + m;
-    const int rid = a.sorted[start + m];
-    const int p = rid / (int)a.Mper;
-    const int64_t b = a.lhs ? a.lhs[p] : p / (int)a.lhs_div;
-    const int64_t r = b * a.Mper + rid % (int)a.Mper;
+// A tile: (expert, first row, rows) of the list, or rows [a.tm z, ..) of expert 0.
+struct GTile {
+    int64_t expert, start;
+    int count;
+};
+__device__ __forceinline__ GTile g_tile(const F8Args& a, int tile) {
+    if (!a.tiles) {
+        const int64_t start = (int64_t)tile * a.tm;
+        return {0, start, (int)(a.rows - start < a.tm ? a.rows - start : a.tm)};
+    }
+    // (through the scalar cache: one load for the wave)
+    typedef const __attribute__((address_space(4))) int32_t* sptr;
+    const sptr t = (sptr)(uintptr_t)(a.tiles + 3 * (int64_t)tile);
+    return {t[0], t[1], t[2]};
+}
+
+// x row of row m of a tile, or -1
+__device__ __forceinline__ int64_t g_xrow(const F8Args& a, const GTile& t, int m) {
+    if (m >= t.count) return -1;
+    if (!a.tiles) return t.start + m;
+    const int rid = a.sorted[t.start + m];
+    int p = rid, in = 0;
+    if (a.Mper != 1) {
+        p = rid / (int)a.Mper;
+        in = rid - p * (int)a.Mper;
+    }
+    // p / lhs_div: half a step from every border, so exact in float64
+    const int64_t b = a.lhs ? a.lhs[p] : a.lhs_div == 1 ? p : (int)(((double)p + 0.5) * a.lhs_inv);
+    const int64_t r = b * a.Mper + in;
     return b >= 0 && r < a.xrows ? r : -1;
+}
+
+// The scale bytes of a tile's TM rows, G_CHUNK blocks from t0, by direct-to-LDS
+// loads into sc[G_CHUNK / 16][TM][16]: g_scale_loads per wave.
+template <int TM, int WAVES>
+constexpr int g_scale_loads = (G_CHUNK / 16 * TM / 64 + WAVES - 1) / WAVES;
+template <int TM, int WAVES>
+__device__ __forceinline__ void g_scales(const F8Args& a, const GTile& tile, unsigned char* sc, int t0, int KB, int wave,
+                                         int lane) {
+    constexpr int N = g_scale_loads<TM, WAVES>, G = TM / 64;
+    static_assert(N * WAVES == G_CHUNK / 16 * G, "whole loads per wave");
+    const int64_t x0 = a.tiles ? 0 : tile.start;
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(a.xs + x0 * a.xs_ld, (a.xrows - x0) * a.xs_ld);
+    uint32_t off[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) {                // 16 blocks' piece u / G, 64 rows u % G
+        const int u = wave + WAVES * i, t = t0 + 16 * (u / G);
+        const int64_t row = g_xrow(a, tile, 64 * (u % G) + lane);
+        off[i] = row >= 0 && t < KB ? (uint32_t)((row - x0) * a.xs_ld) + t : G_NONE;
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) g_dma16(r, sc + (wave + WAVES * i) * 1024, off[i], 0);
+}
+__device__ __forceinline__ uint32_t g_scale(const unsigned char* sc, int TM, int row, int t) {
+    return sc[(t % G_CHUNK / 16 * TM + row) * 16 + t % 16];
 }
 
 // Grouped tiles: workgroup -> (tile, column block).  Workgroups go to the 8 XCDs
