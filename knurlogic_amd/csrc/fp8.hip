@@ -50,7 +50,7 @@ Plan plan_dense(int64_t M, int64_t K) {
 Plan plan_grouped(int64_t rows, int64_t P, int64_t E, int64_t K, bool glu) {
     const int64_t per = ceil_div(rows, P < E ? P : E);
     if (per <= 16 && K <= fp8_skinny_max_k(16, glu)) return {false, 16, rows == P && (P <= 16 || 4 * P <= E)};
-    return {true, !glu && per <= 64 ? 64 : 128};
+    return {true, glu || per <= 64 ? 64 : 128};
 }
 
 size_t rows_bytes(int64_t rows, int64_t K) {
@@ -195,7 +195,7 @@ int kmi_switch_glu_fp8(const void* x, int64_t T, int64_t H, int64_t I, int k, co
         rc = quantize_rows(g, x, dtype, T, ws, st);
         if (rc) return rc;
         ws += rows_bytes(T, H);
-        d.x = g.y = ws; d.xld = I; d.xs_ld = g.ys_ld = fp8_row_scales(I);
+        d.x = g.y = ws; d.xld = I; d.in_order = 1; d.xs_ld = g.ys_ld = fp8_row_scales(I);
         d.xs = g.ys = (unsigned char*)ws + align256((size_t)P * I);
         rc = launch_fp8_glu(g, sr.max_tiles, st);
         if (rc) return rc;

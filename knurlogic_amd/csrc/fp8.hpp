@@ -37,12 +37,13 @@ struct F8Args {
     const int32_t* lhs;
     int64_t lhs_div, Mper;
     double lhs_inv;             // 1.0 / lhs_div (the tiled kernels)
+    int in_order;               // tiled kernels: x's rows lie in the order of `sorted`
     int tm;
     // f8_stream, instead of tiles: the expert of each of the `rows` pairs; tile z =
     // pair z, of x row (lhs ? lhs[z] : z / lhs_div)
     const int32_t* route;
     // launch_fp8_gemm: x is rows of codes as launch_fp8_rows writes them (xld
-    // bytes each) with scale bytes xs [xrows, xs_ld]; gate|up writes codes y
+    // bytes each) with scale bytes xs [xrows, xs_ld]; launch_fp8_glu writes codes y
     // [rows, N] and scale bytes ys [rows, ys_ld] of the activations
     int64_t xld;
     const unsigned char* xs;
@@ -71,8 +72,8 @@ int launch_fp8_rows(const void* x, int dtype, int64_t rows, int64_t K, unsigned 
 constexpr int64_t FP8_GEMM_MAX_K = 65536;     // a tile's rows within 32-bit offsets
 // tiles of up to a.tm (64, 128 or 256) rows over such rows
 int launch_fp8_gemm(const F8Args& a, int64_t tiles, hipStream_t st);
-// the gate|up products of expert tiles of up to 128 rows, and their activations
-// as codes and scale bytes
+// the gate|up products of expert tiles of up to 64 rows, and their activations as
+// codes and scale bytes, in the order of a.sorted
 int launch_fp8_glu(const F8Args& a, int64_t tiles, hipStream_t st);
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));

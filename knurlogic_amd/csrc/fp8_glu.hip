@@ -1,5 +1,5 @@
 // The gate|up products of block-scaled E4M3 experts at prefill sizes: tiles of up to
-// 128 rows of one expert x 128 gate and 128 up rows, SwiGLU, and the activations
+// 64 rows of one expert x 128 gate and 128 up rows, SwiGLU, and the activations
 // quantized for the down product.
 //
 // What these products are rounded to, E4M3 again, turns a small error of a sum into
@@ -9,10 +9,12 @@
 // power of two), on their way from LDS to v_mfma_f32_32x32x16_bf16; a block's sums
 // meet the weights' scale in float32.
 //
-// 8 waves: 32 gate and 32 up rows x two blocks of 32 activation rows each (those
-// past the tile's rows are skipped: a tile's cost follows its rows).  A lane holds
-// its row's 64 bytes of a 128-input block in registers, so an LDS block is free
-// once they are read, a block ahead: two blocks' loads are in flight beside the one
+// 4 waves: 32 gate and 32 up rows x the tile's one or two blocks of 32 rows each.
+// A workgroup starts with a chain of latencies (its tile, its rows, their first
+// inputs: 4 us) and ends with SwiGLU (5 us) beside some 20 us of products, so two
+// of them share a CU: K goes in halves of a block, 64 inputs, 20 KB of LDS each.  A
+// lane holds its row's 32 bytes of a half in registers, so the half's place is free
+// once they are read, a half ahead: two halves' loads are in flight beside the one
 // that has landed.
 #include "fp8_tiles.hpp"
 
@@ -20,9 +22,9 @@ namespace kmi {
 
 namespace {
 
-constexpr int U_TM = 128, U_STAGES = 3, U_WAVES = 8;
-constexpr int U_WTILE = 256 * F8_BLOCK, U_STAGE = U_WTILE + U_TM * F8_BLOCK;
-constexpr int U_WL = 256 / 8 / U_WAVES, U_XL = U_TM / 8 / U_WAVES;     // loads per wave and block
+constexpr int U_TM = 64, U_WAVES = 4, U_STAGES = 3, U_K = 64;          // U_K: inputs of a half
+constexpr int U_WTILE = 256 * U_K, U_STAGE = U_WTILE + U_TM * U_K;
+constexpr int U_WL = U_WTILE / 1024 / U_WAVES, U_XL = U_TM * U_K / 1024 / U_WAVES;      // loads per wave and half
 constexpr int U_LDS = U_STAGES * U_STAGE + G_CHUNK * U_TM;
 constexpr int U_ROW = 272;                                             // bytes of an activation row in LDS, padded
 
@@ -37,10 +39,9 @@ __device__ __forceinline__ bf16x8 u_operand(uint32_t lo, uint32_t hi, float scal
 
 __global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks, int tiles) {
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ int rid_s[U_TM];
     unsigned char* const sc = smem + U_STAGES * U_STAGE;      // [G_CHUNK / 16][U_TM][16] scale bytes
     const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave & 3, wm = wave >> 2;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l32 = lane & 31, h = lane >> 5;
     int tile, nb;
     g_place((int)blockIdx.x, nblocks, tile, nb);
@@ -65,12 +66,11 @@ __global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks,
         for (int g = 0; g < 2; g++) asm volatile("" : "+v"(swl[g]));      // waited for here, not in the loop
     };
     load_scales(0);
-    if (tid < U_TM) rid_s[tid] = tid < count ? a.sorted[T.start + tid] : -1;
-    // direct-to-LDS loads: 8 lanes per row, the lane's piece permuted by the row;
-    // LDS weight row 64 v + r: gate row 32 v + r of the block, r < 32, or up row.
-    // (From here on the compiler's counts miss what is in flight: no load that it
-    // would wait for.)
-    const int piece = (lane & 7) ^ (lane >> 3);
+    // direct-to-LDS loads: 4 lanes per row of 64 bytes, the lane's piece permuted by
+    // the row, so that 8 rows' reads fall on distinct banks; LDS weight row 64 v + r:
+    // gate row 32 v + r of the block, r < 32, or up row.  (From here on the compiler's
+    // counts miss what is in flight: no load that it would wait for.)
+    const int piece = (lane & 3) ^ (lane >> 3 & 3);           // (row / 2 % 4 == lane / 8 % 4)
     const int64_t n0 = (int64_t)nb * 128;                     // N is a multiple of 128
     const __amdgpu_buffer_rsrc_t rx = make_rsrc(a.x, a.xrows * a.xld);
     const __amdgpu_buffer_rsrc_t rg = make_rsrc(a.w + (T.expert * a.wrows + n0) * a.K, 128 * a.K);
@@ -78,38 +78,38 @@ __global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks,
     uint32_t xoff[U_XL], woff[U_WL];
 #pragma unroll
     for (int j = 0; j < U_XL; j++) {
-        const int64_t r = g_xrow(a, T, 8 * (wave + U_WAVES * j) + (lane >> 3));
+        const int64_t r = g_xrow(a, T, 16 * (wave + U_WAVES * j) + (lane >> 2));
         xoff[j] = r < 0 ? G_NONE : (uint32_t)(r * a.xld) + 16u * piece;
     }
 #pragma unroll
     for (int j = 0; j < U_WL; j++) {
-        const int m = 8 * (wave + U_WAVES * j) + (lane >> 3);
+        const int m = 16 * (wave + U_WAVES * j) + (lane >> 2);
         woff[j] = (uint32_t)((m >> 6) * 32 + (m & 31)) * (uint32_t)K + 16u * piece;
     }
-    auto issue = [&](int t) {                                 // block t (past the last: zeros)
+    auto issue = [&](int t) {                                 // half t (past the last: zeros)
         unsigned char* dst = smem + (t % U_STAGES) * U_STAGE;
-        const bool in = t * F8_BLOCK + 16 * piece < K;        // inputs past the last: zeros
+        const bool in = t * U_K + 16 * piece < K;             // inputs past the last: zeros
 #pragma unroll
         for (int j = 0; j < U_WL; j++) {
-            const int m = 8 * (wave + U_WAVES * j);           // (bit 5: up)
-            g_dma16(m & 32 ? ru : rg, dst + m * F8_BLOCK, in ? woff[j] : G_NONE, (uint32_t)t * F8_BLOCK);
+            const int m = 16 * (wave + U_WAVES * j);          // (bit 5: up)
+            g_dma16(m & 32 ? ru : rg, dst + m * U_K, in ? woff[j] : G_NONE, (uint32_t)t * U_K);
         }
 #pragma unroll
         for (int j = 0; j < U_XL; j++)
-            g_dma16(rx, dst + U_WTILE + (wave + U_WAVES * j) * 1024, t < KB ? xoff[j] : G_NONE, (uint32_t)t * F8_BLOCK);
+            g_dma16(rx, dst + U_WTILE + (wave + U_WAVES * j) * 1024, t < 2 * KB ? xoff[j] : G_NONE, (uint32_t)t * U_K);
     };
     g_scales<U_TM, U_WAVES>(a, T, sc, 0, KB, wave, lane);
 #pragma unroll
     for (int t = 0; t < U_STAGES; t++) issue(t);
 
-    // this lane's row of fragment i (weights) or j (x rows 32 (wm + 2 j) ..): bytes
-    // 64 h .. of a block, in 16-byte pieces 4 h + q
-    uint32_t wo[4], xo[4];
+    // this lane's row of fragment i (weights) or j (x): bytes 32 h .. of a half, in
+    // 16-byte pieces 2 h + q
+    uint32_t wo[2], xo[2];
 #pragma unroll
-    for (int q = 0; q < 4; q++) {
-        const uint32_t p = 16u * ((4 * h + q) ^ (l32 & 7));
-        wo[q] = (uint32_t)(64 * wn + l32) * F8_BLOCK + p;
-        xo[q] = U_WTILE + (uint32_t)(32 * wm + l32) * F8_BLOCK + p;
+    for (int q = 0; q < 2; q++) {
+        const uint32_t p = 16u * ((2 * h + q) ^ (l32 >> 1 & 3));
+        wo[q] = (uint32_t)(64 * wave + l32) * U_K + p;
+        xo[q] = U_WTILE + (uint32_t)l32 * U_K + p;
     }
     f32x16 acc[2][2];
 #pragma unroll
@@ -119,26 +119,21 @@ __global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks,
 #pragma unroll
             for (int r = 0; r < 16; r++) acc[i][j][r] = 0.f;
 
-    // NJ: this wave's blocks of 32 activation rows
+    // NJ: the tile's blocks of 32 rows
     auto run = [&](auto nj) {
         constexpr int NJ = decltype(nj)::value;
-        u32x4 w[2][4], x[NJ ? NJ : 1][4];
-        uint32_t xb[NJ ? NJ : 1];
-        auto read = [&](int t, int q) {                       // piece q of every fragment
+        u32x4 w[2][2], x[NJ][2];
+        auto read = [&](int t, int q) {                       // piece q of every fragment of half t
             const unsigned char* st = smem + (t % U_STAGES) * U_STAGE;
 #pragma unroll
-            for (int i = 0; i < 2; i++) w[i][q] = *(const u32x4*)(st + i * 4096 + wo[q]);
+            for (int i = 0; i < 2; i++) w[i][q] = *(const u32x4*)(st + i * 32 * U_K + wo[q]);
 #pragma unroll
-            for (int j = 0; j < NJ; j++) x[j][q] = *(const u32x4*)(st + j * 8192 + xo[q]);
-        };
-        auto read_scales = [&](int t) {
-#pragma unroll
-            for (int j = 0; j < NJ; j++) xb[j] = g_scale(sc, U_TM, 32 * (wm + 2 * j) + l32, t);
+            for (int j = 0; j < NJ; j++) x[j][q] = *(const u32x4*)(st + j * 32 * U_K + xo[q]);
         };
         g_wait<(U_STAGES - 1) * (U_WL + U_XL)>();
         lds_barrier();
-        if constexpr (NJ > 0)
-            for (int q = 0; q < 4; q++) read(0, q);
+#pragma unroll
+        for (int q = 0; q < 2; q++) read(0, q);
         for (int t0 = 0; t0 < KB; t0 += G_CHUNK) {
             if (t0) {                                         // every wave is past its reads of the last chunk's scales
                 load_scales(t0);
@@ -148,24 +143,24 @@ __global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks,
             }
             const int t1 = t0 + G_CHUNK < KB ? t0 + G_CHUNK : KB;
             for (int t = t0; t < t1; t++) {
-                if constexpr (NJ > 0) read_scales(t);
-                // this block is in registers everywhere and the next one has landed
-                g_wait<(U_STAGES - 2) * (U_WL + U_XL)>();
-                lds_barrier();
-                issue(t + U_STAGES);
-                if constexpr (NJ > 0) {
-                    float sx[NJ];
+                float sx[NJ];
 #pragma unroll
-                    for (int j = 0; j < NJ; j++) sx[j] = __uint_as_float(xb[j] << 23);
-                    f32x16 p[2][NJ];
+                for (int j = 0; j < NJ; j++) sx[j] = __uint_as_float(g_scale(sc, U_TM, 32 * j + l32, t) << 23);
+                f32x16 p[2][NJ];
 #pragma unroll
-                    for (int i = 0; i < 2; i++)
+                for (int i = 0; i < 2; i++)
 #pragma unroll
-                        for (int j = 0; j < NJ; j++)
+                    for (int j = 0; j < NJ; j++)
 #pragma unroll
-                            for (int r = 0; r < 16; r++) p[i][j][r] = 0.f;
+                        for (int r = 0; r < 16; r++) p[i][j][r] = 0.f;
 #pragma unroll
-                    for (int s = 0; s < 8; s++) {
+                for (int half = 0; half < 2; half++) {
+                    // this half is in registers everywhere and the next one has landed
+                    g_wait<(U_STAGES - 2) * (U_WL + U_XL)>();
+                    lds_barrier();
+                    issue(2 * t + half + U_STAGES);
+#pragma unroll
+                    for (int s = 0; s < 4; s++) {
                         bf16x8 wv[2], xv[NJ];
 #pragma unroll
                         for (int i = 0; i < 2; i++) wv[i] = u_operand(w[i][s / 2][s % 2 * 2], w[i][s / 2][s % 2 * 2 + 1], 1.f);
@@ -176,25 +171,24 @@ __global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks,
 #pragma unroll
                             for (int j = 0; j < NJ; j++)
                                 p[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wv[i], xv[j], p[i][j], 0, 0, 0);
-                        if (s % 2) read(t + 1, s / 2);
+                        if (s % 2) read(2 * t + half + 1, s / 2);
                         __builtin_amdgcn_sched_barrier(0);
                     }
+                }
 #pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        const float sw = __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(swl[i]), t % G_CHUNK));
+                for (int i = 0; i < 2; i++) {
+                    const float sw = __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(swl[i]), t % G_CHUNK));
 #pragma unroll
-                        for (int j = 0; j < NJ; j++)
+                    for (int j = 0; j < NJ; j++)
 #pragma unroll
-                            for (int r = 0; r < 16; r++) acc[i][j][r] = __builtin_fmaf(p[i][j][r], sw, acc[i][j][r]);
-                    }
+                        for (int r = 0; r < 16; r++) acc[i][j][r] = __builtin_fmaf(p[i][j][r], sw, acc[i][j][r]);
                 }
             }
         }
     };
-    const int blocks = (count + 31) / 32, nj = (blocks - wm + 1) / 2;
+    const int nj = (count + 31) / 32;
     if (nj == 2) run(std::integral_constant<int, 2>());
-    else if (nj == 1) run(std::integral_constant<int, 1>());
-    else run(std::integral_constant<int, 0>());
+    else run(std::integral_constant<int, 1>());
     g_wait<0>();                                 // no load still writes LDS below
     lds_barrier();
 
@@ -213,7 +207,7 @@ __global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks,
                 o[q] = cvt_pk_bf16(silu_bf16r(__uint_as_float(g << 16)) * __uint_as_float(u << 16),
                                    silu_bf16r(__uint_as_float(g & 0xffff0000u)) * __uint_as_float(u & 0xffff0000u));
             }
-            *(u32x2*)(smem + (32 * (wm + 2 * j) + l32) * U_ROW + (32 * wn + 2 * r + 4 * h) * 2) = u32x2{o[0], o[1]};
+            *(u32x2*)(smem + (32 * j + l32) * U_ROW + (32 * wave + 2 * r + 4 * h) * 2) = u32x2{o[0], o[1]};
         }
     }
     lds_barrier();
@@ -225,9 +219,9 @@ __global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks,
         const bool nan = byte == 255;            // as f8_rows
         if (nan) byte = 127;
         const float scale = __uint_as_float(byte << 23);
-        unsigned char* y = (unsigned char*)a.y + (int64_t)rid_s[m] * a.N + nb * 128 + 8 * l16;
+        unsigned char* y = (unsigned char*)a.y + (T.start + m) * a.N + nb * 128 + 8 * l16;
         *(u32x2*)y = nan ? u32x2{0x7f7f7f7fu, 0x7f7f7f7fu} : u32x2{v.codes(0, scale), v.codes(1, scale)};
-        if (l16 == 0) a.ys[(int64_t)rid_s[m] * a.ys_ld + nb] = (unsigned char)byte;
+        if (l16 == 0) a.ys[(T.start + m) * a.ys_ld + nb] = (unsigned char)byte;
     }
 }
 

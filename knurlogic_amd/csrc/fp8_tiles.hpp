@@ -46,7 +46,7 @@ __device__ __forceinline__ GTile g_tile(const F8Args& a, int tile) {
 // x row of row m of a tile, or -1
 __device__ __forceinline__ int64_t g_xrow(const F8Args& a, const GTile& t, int m) {
     if (m >= t.count) return -1;
-    if (!a.tiles) return t.start + m;
+    if (!a.tiles || a.in_order) return t.start + m;
     const int rid = a.sorted[t.start + m];
     int p = rid, in = 0;
     if (a.Mper != 1) {
@@ -85,14 +85,14 @@ __device__ __forceinline__ uint32_t g_scale(const unsigned char* sc, int TM, int
 }
 
 // Grouped tiles: workgroup -> (tile, column block).  Workgroups go to the 8 XCDs
-// in turn; 2 neighbouring tiles (often one expert's) of every column block stay on
-// one XCD, whose L2 then serves the second, the next 2 go to the next (tiles at
+// in turn; 4 neighbouring tiles (often one expert's) of every column block stay on
+// one XCD, whose L2 then serves the others, the next 4 go to the next (tiles at
 // the list's end are empty: they must not all fall to one).
 __device__ __forceinline__ void g_place(int id, int nblocks, int& tile, int& nb) {
     const int xcd = id & 7, kk = id >> 3;
-    tile = ((kk / (2 * nblocks)) * 8 + xcd) * 2 + kk % 2;
-    nb = kk / 2 % nblocks;
+    tile = ((kk / (4 * nblocks)) * 8 + xcd) * 4 + kk % 4;
+    nb = kk / 4 % nblocks;
 }
-inline int64_t g_place_grid(int64_t tiles, int64_t nblocks) { return ceil_div(tiles, 16) * 16 * nblocks; }
+inline int64_t g_place_grid(int64_t tiles, int64_t nblocks) { return ceil_div(tiles, 32) * 32 * nblocks; }
 
 }  // namespace kmi
