@@ -31,13 +31,15 @@ struct Shape {
     static_assert(XL * 8 * WAVES == TM && WL * 8 * WAVES == TN, "whole loads per wave");
 };
 
-template <Kind KIND, int NW, int WM, int MB, int S>
+// TAIL: K is not a multiple of 128
+template <Kind KIND, int NW, int WM, int MB, int S, bool TAIL>
 __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks, int tiles) {
     typedef Shape<NW, WM, MB, S> Z;
     constexpr int RB = 4, TN = Z::TN, TM = Z::TM, XL = Z::XL, WL = Z::WL, WAVES = Z::WAVES, WTILE = Z::WTILE;
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ int rid_s[TM];
     unsigned char* const sc = smem + S * Z::STAGE;            // [G_CHUNK / 16][TM][16] scale bytes
+    const uint32_t lds = g_lds(smem), lds_sc = lds + S * Z::STAGE;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave % NW, wm = wave / NW;
     const int l16 = lane & 15, c = lane >> 4;
@@ -78,8 +80,9 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
     // (From here on the compiler's counts miss what is in flight: no load that it
     // would wait for.)
     const int piece = (lane & 7) ^ (lane >> 3);               // (row % 8 == lane / 8)
-    const __amdgpu_buffer_rsrc_t rx = make_rsrc((const unsigned char*)a.x + x0 * a.xld, (a.xrows - x0) * a.xld);
-    const __amdgpu_buffer_rsrc_t rw = make_rsrc(a.w + (T.expert * a.wrows + n0) * a.K, left * a.K);
+    const unsigned char* const xv = (const unsigned char*)a.x + x0 * a.xld;
+    const unsigned char* const wv = a.w + (T.expert * a.wrows + n0) * a.K;
+    const int64_t xbytes = (a.xrows - x0) * a.xld, wbytes = left * a.K;
     uint32_t xoff[XL], woff[WL];
 #pragma unroll
     for (int j = 0; j < XL; j++) {
@@ -91,19 +94,19 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
         const int m = 8 * (wave + WAVES * j) + (lane >> 3);
         woff[j] = m < left ? (uint32_t)m * (uint32_t)K + 16u * piece : G_NONE;
     }
-    auto issue = [&](int t) {                                 // block t (past the last: zeros)
-        unsigned char* dst = smem + (t % S) * Z::STAGE;
-        const bool in = t * F8_BLOCK + 16 * piece < K;        // inputs past the last: zeros
+    auto issue = [&](int t, int at) {                         // block t (past the last: zeros) into place `at`
+        const __amdgpu_buffer_rsrc_t rw = make_rsrc(wv, t < KB ? wbytes : 0), rx = make_rsrc(xv, t < KB ? xbytes : 0);
+        const uint32_t dst = lds + at * Z::STAGE + wave * 1024;
+        const bool in = !TAIL || t * F8_BLOCK + 16 * piece < K;       // inputs past the last: zeros
 #pragma unroll
         for (int j = 0; j < WL; j++)
-            g_dma16(rw, dst + (wave + WAVES * j) * 1024, in ? woff[j] : G_NONE, (uint32_t)t * F8_BLOCK);
+            g_dma16(rw, dst + WAVES * j * 1024, in ? woff[j] : G_NONE, (uint32_t)t * F8_BLOCK);
 #pragma unroll
-        for (int j = 0; j < XL; j++)
-            g_dma16(rx, dst + WTILE + (wave + WAVES * j) * 1024, t < KB ? xoff[j] : G_NONE, (uint32_t)t * F8_BLOCK);
+        for (int j = 0; j < XL; j++) g_dma16(rx, dst + WTILE + WAVES * j * 1024, xoff[j], (uint32_t)t * F8_BLOCK);
     };
-    g_scales<TM, WAVES>(a, T, sc, 0, KB, wave, lane);
+    g_scales<TM, WAVES>(a, T, lds_sc, 0, KB, wave, lane);
 #pragma unroll
-    for (int t = 0; t < S; t++) issue(t);
+    for (int t = 0; t < S; t++) issue(t, t);
 
     // fragment reads: weight row 64 wn + 16 i + l16, pieces c and c + 4; x row
     // 16 (MB wm + j) + l16, the same
@@ -132,17 +135,19 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
     for (int i = 0; i < RB; i++) read_w(smem, i);
     read_b(smem, 0);
     static_assert(MB % 2 == 0, "x fragments alternate");
+    int at = 0;                                  // this block's place in the ring
     for (int t0 = 0; t0 < KB; t0 += G_CHUNK) {
     if (t0) {                                    // every wave is past its reads of the last chunk's scales
         load_scales(t0);
-        g_scales<TM, WAVES>(a, T, sc, t0, KB, wave, lane);
+        g_scales<TM, WAVES>(a, T, lds_sc, t0, KB, wave, lane);
         g_wait<0>();
         lds_barrier();
     }
     const int t1 = t0 + G_CHUNK < KB ? t0 + G_CHUNK : KB;
     for (int t = t0; t < t1; t++) {              // (no branch inside: the compiler would sink products past it)
-        const unsigned char* st = smem + (t % S) * Z::STAGE;
-        const unsigned char* nx = smem + ((t + 1) % S) * Z::STAGE;
+        const int after = at + 1 < S ? at + 1 : 0;
+        const unsigned char* st = smem + at * Z::STAGE;
+        const unsigned char* nx = smem + after * Z::STAGE;
         uint32_t sx[MB];
 #pragma unroll
         for (int j = 0; j < MB; j++) sx[j] = g_scale(sc, TM, 16 * (MB * wm + j) + l16, t);
@@ -152,7 +157,7 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
         auto turn = [&]() {
             g_wait<(S - 2) * (XL + WL)>();
             lds_barrier();
-            issue(t + S);
+            issue(t + S, at);
         };
         {
             // product n = 4 j + i; its sums are scaled two products later
@@ -187,6 +192,7 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
                 apply(NP - 1);
             }
         }
+        at = after;
     }
     }
     g_wait<0>();                                 // no load still writes LDS below
@@ -248,7 +254,7 @@ __global__ __launch_bounds__(256) void f8_rows(const typename T::storage* __rest
     if (l == 0) s[r * sld + b] = (unsigned char)byte;
 }
 
-template <Kind KIND, int NW, int WM, int MB, int S>
+template <Kind KIND, int NW, int WM, int MB, int S, bool TAIL>
 int go(const F8Args& a, int64_t tiles, hipStream_t st) {
     typedef Shape<NW, WM, MB, S> Z;
     if (a.K > FP8_GEMM_MAX_K || a.xld != fp8_row_bytes(a.K) || a.tm > Z::TM) {
@@ -261,15 +267,16 @@ int go(const F8Args& a, int64_t tiles, hipStream_t st) {
         set_error("fp8: grid of %lld workgroups", (long long)wgs);
         return EINVAL_ARG;
     }
-    allow_dynamic_lds_once((const void*)f8_gemm<KIND, NW, WM, MB, S>);
-    f8_gemm<KIND, NW, WM, MB, S><<<(unsigned)wgs, 64 * Z::WAVES, Z::LDS, st>>>(a, nblocks, (int)tiles);
+    allow_dynamic_lds_once((const void*)f8_gemm<KIND, NW, WM, MB, S, TAIL>);
+    f8_gemm<KIND, NW, WM, MB, S, TAIL><<<(unsigned)wgs, 64 * Z::WAVES, Z::LDS, st>>>(a, nblocks, (int)tiles);
     KMI_CHECK_LAUNCH("fp8 tiles");
     return OK;
 }
 
 template <int NW, int WM, int MB, int S>
 int go(const F8Args& a, int64_t tiles, hipStream_t st) {
-    return a.e8 ? go<E8S, NW, WM, MB, S>(a, tiles, st) : go<F32S, NW, WM, MB, S>(a, tiles, st);
+    if (a.K % F8_BLOCK) return a.e8 ? go<E8S, NW, WM, MB, S, true>(a, tiles, st) : go<F32S, NW, WM, MB, S, true>(a, tiles, st);
+    return a.e8 ? go<E8S, NW, WM, MB, S, false>(a, tiles, st) : go<F32S, NW, WM, MB, S, false>(a, tiles, st);
 }
 
 }  // namespace

@@ -37,9 +37,12 @@ __device__ __forceinline__ bf16x8 u_operand(uint32_t lo, uint32_t hi, float scal
     return as_bf16x8(r);
 }
 
+// TAIL: K is not a multiple of 64
+template <bool TAIL>
 __global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks, int tiles) {
     extern __shared__ __align__(16) unsigned char smem[];
     unsigned char* const sc = smem + U_STAGES * U_STAGE;      // [G_CHUNK / 16][U_TM][16] scale bytes
+    const uint32_t lds = g_lds(smem), lds_sc = lds + U_STAGES * U_STAGE;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l32 = lane & 31, h = lane >> 5;
@@ -72,9 +75,9 @@ __global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks,
     // counts miss what is in flight: no load that it would wait for.)
     const int piece = (lane & 3) ^ (lane >> 3 & 3);           // (row / 2 % 4 == lane / 8 % 4)
     const int64_t n0 = (int64_t)nb * 128;                     // N is a multiple of 128
-    const __amdgpu_buffer_rsrc_t rx = make_rsrc(a.x, a.xrows * a.xld);
-    const __amdgpu_buffer_rsrc_t rg = make_rsrc(a.w + (T.expert * a.wrows + n0) * a.K, 128 * a.K);
-    const __amdgpu_buffer_rsrc_t ru = make_rsrc(a.w + (T.expert * a.wrows + n0 + a.N) * a.K, 128 * a.K);
+    const unsigned char* const xv = (const unsigned char*)a.x;
+    const unsigned char* const wv = a.w + (T.expert * a.wrows + n0 + (wave & 2 ? a.N : 0)) * a.K;     // (a wave loads gate or up rows)
+    const int64_t xbytes = a.xrows * a.xld, wbytes = 128 * a.K;
     uint32_t xoff[U_XL], woff[U_WL];
 #pragma unroll
     for (int j = 0; j < U_XL; j++) {
@@ -86,21 +89,21 @@ __global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks,
         const int m = 16 * (wave + U_WAVES * j) + (lane >> 2);
         woff[j] = (uint32_t)((m >> 6) * 32 + (m & 31)) * (uint32_t)K + 16u * piece;
     }
-    auto issue = [&](int t) {                                 // half t (past the last: zeros)
-        unsigned char* dst = smem + (t % U_STAGES) * U_STAGE;
-        const bool in = t * U_K + 16 * piece < K;             // inputs past the last: zeros
+    auto issue = [&](int t, int at) {                         // half t (past the last: zeros) into place `at`
+        const bool on = t * U_K < K;
+        const __amdgpu_buffer_rsrc_t rw = make_rsrc(wv, on ? wbytes : 0), rx = make_rsrc(xv, on ? xbytes : 0);
+        const uint32_t dst = lds + at * U_STAGE + wave * 1024;
+        const bool in = !TAIL || t * U_K + 16 * piece < K;    // inputs past the last: zeros
 #pragma unroll
-        for (int j = 0; j < U_WL; j++) {
-            const int m = 16 * (wave + U_WAVES * j);          // (bit 5: up)
-            g_dma16(m & 32 ? ru : rg, dst + m * U_K, in ? woff[j] : G_NONE, (uint32_t)t * U_K);
-        }
+        for (int j = 0; j < U_WL; j++)
+            g_dma16(rw, dst + U_WAVES * j * 1024, in ? woff[j] : G_NONE, (uint32_t)t * U_K);
 #pragma unroll
         for (int j = 0; j < U_XL; j++)
-            g_dma16(rx, dst + U_WTILE + (wave + U_WAVES * j) * 1024, t < 2 * KB ? xoff[j] : G_NONE, (uint32_t)t * U_K);
+            g_dma16(rx, dst + U_WTILE + U_WAVES * j * 1024, xoff[j], (uint32_t)t * U_K);
     };
-    g_scales<U_TM, U_WAVES>(a, T, sc, 0, KB, wave, lane);
+    g_scales<U_TM, U_WAVES>(a, T, lds_sc, 0, KB, wave, lane);
 #pragma unroll
-    for (int t = 0; t < U_STAGES; t++) issue(t);
+    for (int t = 0; t < U_STAGES; t++) issue(t, t);
 
     // this lane's row of fragment i (weights) or j (x): bytes 32 h .. of a half, in
     // 16-byte pieces 2 h + q
@@ -123,8 +126,8 @@ __global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks,
     auto run = [&](auto nj) {
         constexpr int NJ = decltype(nj)::value;
         u32x4 w[2][2], x[NJ][2];
-        auto read = [&](int t, int q) {                       // piece q of every fragment of half t
-            const unsigned char* st = smem + (t % U_STAGES) * U_STAGE;
+        auto read = [&](int at, int q) {                      // piece q of every fragment of the half at place `at`
+            const unsigned char* st = smem + at * U_STAGE;
 #pragma unroll
             for (int i = 0; i < 2; i++) w[i][q] = *(const u32x4*)(st + i * 32 * U_K + wo[q]);
 #pragma unroll
@@ -134,10 +137,11 @@ __global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks,
         lds_barrier();
 #pragma unroll
         for (int q = 0; q < 2; q++) read(0, q);
+        int at = 0;                                           // this half's place in the ring
         for (int t0 = 0; t0 < KB; t0 += G_CHUNK) {
             if (t0) {                                         // every wave is past its reads of the last chunk's scales
                 load_scales(t0);
-                g_scales<U_TM, U_WAVES>(a, T, sc, t0, KB, wave, lane);
+                g_scales<U_TM, U_WAVES>(a, T, lds_sc, t0, KB, wave, lane);
                 g_wait<0>();
                 lds_barrier();
             }
@@ -158,7 +162,8 @@ __global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks,
                     // this half is in registers everywhere and the next one has landed
                     g_wait<(U_STAGES - 2) * (U_WL + U_XL)>();
                     lds_barrier();
-                    issue(2 * t + half + U_STAGES);
+                    issue(2 * t + half + U_STAGES, at);
+                    at = at + 1 < U_STAGES ? at + 1 : 0;
 #pragma unroll
                     for (int s = 0; s < 4; s++) {
                         bf16x8 wv[2], xv[NJ];
@@ -171,7 +176,7 @@ __global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks,
 #pragma unroll
                             for (int j = 0; j < NJ; j++)
                                 p[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wv[i], xv[j], p[i][j], 0, 0, 0);
-                        if (s % 2) read(2 * t + half + 1, s / 2);
+                        if (s % 2) read(at, s / 2);
                         __builtin_amdgcn_sched_barrier(0);
                     }
                 }
@@ -238,8 +243,9 @@ int launch_fp8_glu(const F8Args& a, int64_t tiles, hipStream_t st) {
         set_error("fp8: grid of %lld workgroups", (long long)wgs);
         return EINVAL_ARG;
     }
-    allow_dynamic_lds_once((const void*)f8_glu);
-    f8_glu<<<(unsigned)wgs, 64 * U_WAVES, U_LDS, st>>>(a, (int)nblocks, (int)tiles);
+    const auto f = a.K % U_K ? f8_glu<true> : f8_glu<false>;
+    allow_dynamic_lds_once((const void*)f);
+    f<<<(unsigned)wgs, 64 * U_WAVES, U_LDS, st>>>(a, (int)nblocks, (int)tiles);
     KMI_CHECK_LAUNCH("fp8 gate|up");
     return OK;
 }

@@ -6,8 +6,6 @@
 
 namespace kmi {
 
-#define KMI_F8_LDS(p) ((__attribute__((address_space(3))) unsigned char*)(p))
-
 constexpr uint32_t G_NONE = 0x80000000u;     // past every view: reads 0
 constexpr int G_CHUNK = 64;                  // blocks whose scales are held at a time
 
@@ -17,14 +15,18 @@ __device__ __forceinline__ void g_wait() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N_) : "memory");
 }
 
-// 16 bytes per lane from the view's offset into LDS at dst + 16 lane.  In asm, as
-// the compiler would wait for the load before any later read of LDS; the kernel
+// 16 bytes per lane from the view's offset into LDS at byte dst + 16 lane.  In asm,
+// as the compiler would wait for the load before any later read of LDS; the kernel
 // waits for it itself (g_wait), and the compiler's own counts, which miss these
 // loads, only wait for more.
-__device__ __forceinline__ void g_dma16(__amdgpu_buffer_rsrc_t r, unsigned char* dst, uint32_t voff, uint32_t soff) {
-    const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)KMI_F8_LDS(dst));
+__device__ __forceinline__ void g_dma16(__amdgpu_buffer_rsrc_t r, uint32_t dst, uint32_t voff, uint32_t soff) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-                 ::"s"(at), "v"(voff), "s"(r), "s"(soff) : "memory", "m0");
+                 ::"s"(dst), "v"(voff), "s"(r), "s"(soff) : "memory", "m0");
+}
+// the byte address of shared memory p (taken once: a generic pointer's conversion
+// tests for null every time)
+__device__ __forceinline__ uint32_t g_lds(const void* p) {
+    return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p);
 }
 
 // A tile: (expert, first row, rows) of the list, or rows [a.tm z, ..) of expert 0.
@@ -64,7 +66,7 @@ __device__ __forceinline__ int64_t g_xrow(const F8Args& a, const GTile& t, int m
 template <int TM, int WAVES>
 constexpr int g_scale_loads = (G_CHUNK / 16 * TM / 64 + WAVES - 1) / WAVES;
 template <int TM, int WAVES>
-__device__ __forceinline__ void g_scales(const F8Args& a, const GTile& tile, unsigned char* sc, int t0, int KB, int wave,
+__device__ __forceinline__ void g_scales(const F8Args& a, const GTile& tile, uint32_t sc, int t0, int KB, int wave,
                                          int lane) {
     constexpr int N = g_scale_loads<TM, WAVES>, G = TM / 64;
     static_assert(N * WAVES == G_CHUNK / 16 * G, "whole loads per wave");
