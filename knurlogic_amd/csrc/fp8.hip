@@ -53,6 +53,8 @@ Plan plan_grouped(int64_t rows, int64_t P, int64_t E, int64_t K, bool glu) {
     return {true, glu || per <= 64 ? 64 : 128};
 }
 
+size_t values_bytes(int64_t rows, int64_t K) { return align256((size_t)rows * fp8_row_bytes(K) * 2); }
+
 size_t rows_bytes(int64_t rows, int64_t K) {
     return align256((size_t)rows * fp8_row_bytes(K)) + align256((size_t)rows * fp8_row_scales(K));
 }
@@ -149,7 +151,7 @@ size_t kmi_switch_glu_fp8_workspace_bytes(int64_t T, int64_t H, int64_t I, int k
     const int64_t P = T * k;
     const Plan p = plan_grouped(P, P, E, H > I ? H : I, true);
     return align256((size_t)P * H * 2) + (p.pairs ? 0 : sort_index_bytes(P, E, p.tm)) +
-           (p.gemm ? rows_bytes(T, H) + rows_bytes(P, I) : align256((size_t)P * I * 2));
+           (p.gemm ? values_bytes(T, H) + rows_bytes(P, I) : align256((size_t)P * I * 2));
 }
 
 int kmi_switch_glu_fp8(const void* x, int64_t T, int64_t H, int64_t I, int k, const int32_t* inds,
@@ -170,7 +172,7 @@ int kmi_switch_glu_fp8(const void* x, int64_t T, int64_t H, int64_t I, int k, co
     KMI_CHECK_ARG(x && inds && w_gu && s_gu && w_down && s_down && out, "%s: null pointer", what);
     const int64_t P = T * k;
     const Plan p = plan_grouped(P, P, E, H > I ? H : I, true);
-    KMI_CHECK_ARG(!p.gemm || (T * fp8_row_bytes(H) < (1LL << 31) && P * I < (1LL << 31)),
+    KMI_CHECK_ARG(!p.gemm || (2 * T * fp8_row_bytes(H) < (1LL << 31) && P * I < (1LL << 31)),
                   "%s: activations past 2 GiB", what);
     rc = check_workspace(what, kmi_switch_glu_fp8_workspace_bytes(T, H, I, k, E), workspace, workspace_bytes);
     if (rc) return rc;
@@ -192,9 +194,10 @@ int kmi_switch_glu_fp8(const void* x, int64_t T, int64_t H, int64_t I, int k, co
     d.w = (const unsigned char*)w_down; d.s = s_down; d.wrows = H; d.K = I; d.N = H; d.xrows = P; d.y = y;
     d.lhs_div = 1; d.lhs_inv = 1.0;
     if (p.gemm) {
-        rc = quantize_rows(g, x, dtype, T, ws, st);
+        rc = launch_fp8_rows(x, dtype, T, H, (unsigned char*)ws, nullptr, st);
         if (rc) return rc;
-        ws += rows_bytes(T, H);
+        g.x = ws; g.xld = 2 * fp8_row_bytes(H);
+        ws += values_bytes(T, H);
         d.x = g.y = ws; d.xld = I; d.in_order = 1; d.xs_ld = g.ys_ld = fp8_row_scales(I);
         d.xs = g.ys = (unsigned char*)ws + align256((size_t)P * I);
         rc = launch_fp8_glu(g, sr.max_tiles, st);

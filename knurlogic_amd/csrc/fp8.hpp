@@ -42,8 +42,8 @@ struct F8Args {
     // f8_stream, instead of tiles: the expert of each of the `rows` pairs; tile z =
     // pair z, of x row (lhs ? lhs[z] : z / lhs_div)
     const int32_t* route;
-    // launch_fp8_gemm: x is rows of codes as launch_fp8_rows writes them (xld
-    // bytes each) with scale bytes xs [xrows, xs_ld]; launch_fp8_glu writes codes y
+    // launch_fp8_gemm, launch_fp8_glu: x is rows as launch_fp8_rows writes them (xld
+    // bytes each), codes with scale bytes xs [xrows, xs_ld] or values; the latter writes codes y
     // [rows, N] and scale bytes ys [rows, ys_ld] of the activations
     int64_t xld;
     const unsigned char* xs;
@@ -64,7 +64,8 @@ bool fp8_combine_supported(int64_t K, int k);
 int launch_fp8_combine(const F8Args& a, const void* scores, int k, int64_t T, void* out, hipStream_t st);
 
 // Rows quantized ahead: codes in rows of fp8_row_bytes (a multiple of 128, the
-// tail zero) and scale bytes in rows of fp8_row_scales.
+// tail zero) and scale bytes in rows of fp8_row_scales; or, without s, what they
+// stand for in bfloat16 (exact) in rows of twice the bytes.
 int64_t fp8_row_bytes(int64_t K);
 int64_t fp8_row_scales(int64_t K);             // (a multiple of 16)
 int launch_fp8_rows(const void* x, int dtype, int64_t rows, int64_t K, unsigned char* q, unsigned char* s,
@@ -72,8 +73,8 @@ int launch_fp8_rows(const void* x, int dtype, int64_t rows, int64_t K, unsigned 
 constexpr int64_t FP8_GEMM_MAX_K = 65536;     // a tile's rows within 32-bit offsets
 // tiles of up to a.tm (64, 128 or 256) rows over such rows
 int launch_fp8_gemm(const F8Args& a, int64_t tiles, hipStream_t st);
-// the gate|up products of expert tiles of up to 64 rows, and their activations as
-// codes and scale bytes, in the order of a.sorted
+// the gate|up products of expert tiles of up to 64 rows over x's values in bfloat16,
+// and their activations as codes and scale bytes, in the order of a.sorted
 int launch_fp8_glu(const F8Args& a, int64_t tiles, hipStream_t st);
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
@@ -96,6 +97,16 @@ __device__ __forceinline__ f32x4 f8_mfma(i32x8 a, i32x8 b, f32x4 c, uint32_t sa,
 
 __device__ __forceinline__ i32x8 f8_operand(u32x4 lo, u32x4 hi) {
     return i32x8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
+}
+
+// 8 codes times a scale (a power of two), in bfloat16, which holds them exactly
+__device__ __forceinline__ bf16x8 f8_values(uint32_t lo, uint32_t hi, float scale) {
+    u32x4 r;
+    r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false));
+    r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true));
+    r.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false));
+    r.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true));
+    return as_bf16x8(r);
 }
 
 // max over each 16 neighbouring lanes, by rotations of a row of lanes (a shuffle

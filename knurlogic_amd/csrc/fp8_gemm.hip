@@ -74,6 +74,8 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
         else swl = ((const uint32_t*)a.s)[i];
         asm volatile("" : "+v"(swl));            // waited for here, not in the loop
     };
+    int64_t xr[XL];                                           // (beside the scales' latency)
+    g_xrows(a, T, 8 * wave + (lane >> 3), 8 * WAVES, xr);
     load_scales(0);
     if (tid < TM) rid_s[tid] = tid >= count ? -1 : a.tiles ? a.sorted[T.start + tid] : (int)(T.start + tid);
     // direct-to-LDS loads: 8 lanes per row, the lane's piece permuted by the row.
@@ -86,8 +88,7 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
     uint32_t xoff[XL], woff[WL];
 #pragma unroll
     for (int j = 0; j < XL; j++) {
-        const int64_t r = g_xrow(a, T, 8 * (wave + WAVES * j) + (lane >> 3));
-        xoff[j] = r < 0 ? G_NONE : (uint32_t)((r - x0) * a.xld) + 16u * piece;
+        xoff[j] = xr[j] < 0 ? G_NONE : (uint32_t)((xr[j] - x0) * a.xld) + 16u * piece;
     }
 #pragma unroll
     for (int j = 0; j < WL; j++) {
@@ -205,7 +206,12 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
             const int m = 16 * (MB * wm + j) + l16;
             const int rid = rid_s[m];
             if (rid < 0) continue;
-            const bool seen = !a.lhs || g_xrow(a, T, m) >= 0;
+            bool seen = true;
+            if (a.lhs) {
+                int64_t row[1];
+                g_xrows(a, T, m, 0, row);
+                seen = row[0] >= 0;
+            }
 #pragma unroll
             for (int i = 0; i < RB; i++) {
                 const int64_t n = n0 + 64 * wn + 16 * i + 4 * c;
@@ -232,8 +238,8 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
 }
 
 // x's rows into codes [rows, ld] (tails zero) and scale bytes [rows, sld]: 16
-// lanes per row and block.
-template <class T>
+// lanes per row and block.  VALUES: what they stand for, in bfloat16, instead.
+template <class T, bool VALUES>
 __global__ __launch_bounds__(256) void f8_rows(const typename T::storage* __restrict__ x, int64_t rows, int K, int KB,
                                                unsigned char* __restrict__ q, int64_t ld,
                                                unsigned char* __restrict__ s, int64_t sld) {
@@ -250,7 +256,12 @@ __global__ __launch_bounds__(256) void f8_rows(const typename T::storage* __rest
     const bool nan = byte == 255;
     if (nan) byte = 127;
     const float scale = __uint_as_float(byte << 23);
-    *(u32x2*)(q + r * ld + k) = nan ? u32x2{0x7f7f7f7fu, 0x7f7f7f7fu} : u32x2{v.codes(0, scale), v.codes(1, scale)};
+    const u32x2 c = nan ? u32x2{0x7f7f7f7fu, 0x7f7f7f7fu} : u32x2{v.codes(0, scale), v.codes(1, scale)};
+    if constexpr (VALUES) {
+        *(bf16x8*)(q + r * ld + 2 * k) = f8_values(c.x, c.y, scale);
+        return;
+    }
+    *(u32x2*)(q + r * ld + k) = c;
     if (l == 0) s[r * sld + b] = (unsigned char)byte;
 }
 
@@ -291,9 +302,10 @@ int launch_fp8_rows(const void* x, int dtype, int64_t rows, int64_t K, unsigned 
         set_error("fp8: %lld rows", (long long)rows);
         return EINVAL_ARG;
     }
-    const int64_t ld = fp8_row_bytes(K), sld = fp8_row_scales(K);
-    if (dtype == BF16) f8_rows<F8BF16><<<(unsigned)grid, 256, 0, st>>>((const uint16_t*)x, rows, (int)K, (int)KB, q, ld, s, sld);
-    else f8_rows<F8F16><<<(unsigned)grid, 256, 0, st>>>((const uint16_t*)x, rows, (int)K, (int)KB, q, ld, s, sld);
+    const int64_t ld = fp8_row_bytes(K) * (s ? 1 : 2), sld = fp8_row_scales(K);
+    const auto f = dtype == BF16 ? s ? f8_rows<F8BF16, false> : f8_rows<F8BF16, true>
+                                 : s ? f8_rows<F8F16, false> : f8_rows<F8F16, true>;
+    f<<<(unsigned)grid, 256, 0, st>>>((const uint16_t*)x, rows, (int)K, (int)KB, q, ld, s, sld);
     KMI_CHECK_LAUNCH("fp8 rows");
     return OK;
 }

@@ -5,15 +5,16 @@
 // What these products are rounded to, E4M3 again, turns a small error of a sum into
 // an eighth of a value where a code falls to its neighbour; the 8-bit matrix
 // instructions drop too much of small products for that (fp8.hpp).  So the codes
-// are turned into bfloat16, which holds them exactly, x's with its row's scale (a
-// power of two), on their way from LDS to v_mfma_f32_32x32x16_bf16; a block's sums
-// meet the weights' scale in float32.
+// are multiplied in bfloat16, which holds them exactly: the weights' turned on their
+// way from LDS to v_mfma_f32_32x32x16_bf16, x's values (codes times the row's scale, a
+// power of two) by the pass before; a block's sums meet the weights' scale in
+// float32.
 //
 // 4 waves: 32 gate and 32 up rows x the tile's one or two blocks of 32 rows each.
 // A workgroup starts with a chain of latencies (its tile, its rows, their first
 // inputs: 4 us) and ends with SwiGLU (5 us) beside some 20 us of products, so two
-// of them share a CU: K goes in halves of a block, 64 inputs, 20 KB of LDS each.  A
-// lane holds its row's 32 bytes of a half in registers, so the half's place is free
+// of them share a CU: K goes in halves of a block, 64 inputs, 24 KB of LDS each.  A
+// lane holds its row's 32 inputs of a half in registers, so the half's place is free
 // once they are read, a half ahead: two halves' loads are in flight beside the one
 // that has landed.
 #include "fp8_tiles.hpp"
@@ -23,26 +24,16 @@ namespace kmi {
 namespace {
 
 constexpr int U_TM = 64, U_WAVES = 4, U_STAGES = 3, U_K = 64;          // U_K: inputs of a half
-constexpr int U_WTILE = 256 * U_K, U_STAGE = U_WTILE + U_TM * U_K;
-constexpr int U_WL = U_WTILE / 1024 / U_WAVES, U_XL = U_TM * U_K / 1024 / U_WAVES;      // loads per wave and half
-constexpr int U_LDS = U_STAGES * U_STAGE + G_CHUNK * U_TM;
+constexpr int U_WTILE = 256 * U_K, U_STAGE = U_WTILE + 2 * U_TM * U_K;
+constexpr int U_WL = U_WTILE / 1024 / U_WAVES, U_XL = 2 * U_TM * U_K / 1024 / U_WAVES;  // loads per wave and half
+constexpr int U_LDS = U_STAGES * U_STAGE;
 constexpr int U_ROW = 272;                                             // bytes of an activation row in LDS, padded
-
-__device__ __forceinline__ bf16x8 u_operand(uint32_t lo, uint32_t hi, float scale) {      // 8 codes times scale
-    u32x4 r;
-    r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false));
-    r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true));
-    r.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false));
-    r.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true));
-    return as_bf16x8(r);
-}
 
 // TAIL: K is not a multiple of 64
 template <bool TAIL>
 __global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks, int tiles) {
     extern __shared__ __align__(16) unsigned char smem[];
-    unsigned char* const sc = smem + U_STAGES * U_STAGE;      // [G_CHUNK / 16][U_TM][16] scale bytes
-    const uint32_t lds = g_lds(smem), lds_sc = lds + U_STAGES * U_STAGE;
+    const uint32_t lds = g_lds(smem);
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l32 = lane & 31, h = lane >> 5;
@@ -59,20 +50,27 @@ __global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks,
     const int64_t sbase = (T.expert * SB + nb) * KB;
     float swl[2];
     auto load_scales = [&](int t) {
-        const int k = t + lane < KB ? t + lane : KB - 1;
-#pragma unroll
-        for (int g = 0; g < 2; g++) {
-            const int64_t i = sbase + (g ? a.N / F8_BLOCK * KB : 0) + k;
-            swl[g] = a.e8 ? e8m0_to_f32(((const unsigned char*)a.s)[i]) : ((const float*)a.s)[i];
+        const int64_t i = sbase + (t + lane < KB ? t + lane : KB - 1), up = a.N / F8_BLOCK * KB;
+        uint32_t v[2];
+        if (a.e8) {
+            v[0] = ((const unsigned char*)a.s)[i];
+            v[1] = ((const unsigned char*)a.s)[i + up];
+        } else {
+            v[0] = ((const uint32_t*)a.s)[i];
+            v[1] = ((const uint32_t*)a.s)[i + up];
         }
+        asm volatile("" : "+v"(v[0]), "+v"(v[1]));            // waited for here, not in the loop
 #pragma unroll
-        for (int g = 0; g < 2; g++) asm volatile("" : "+v"(swl[g]));      // waited for here, not in the loop
+        for (int g = 0; g < 2; g++) swl[g] = a.e8 ? e8m0_to_f32(v[g]) : __uint_as_float(v[g]);
     };
+    int64_t xr[U_XL];                                         // (beside the scales' latency)
+    g_xrows(a, T, 8 * wave + (lane >> 3), 8 * U_WAVES, xr);
     load_scales(0);
-    // direct-to-LDS loads: 4 lanes per row of 64 bytes, the lane's piece permuted by
-    // the row, so that 8 rows' reads fall on distinct banks; LDS weight row 64 v + r:
-    // gate row 32 v + r of the block, r < 32, or up row.  (From here on the compiler's
-    // counts miss what is in flight: no load that it would wait for.)
+    // direct-to-LDS loads: 4 lanes per weight row of 64 bytes, 8 per x row of 128, the
+    // lane's piece permuted by the row, so that 8 rows' reads fall on distinct banks;
+    // LDS weight row 64 v + r: gate row 32 v + r of the block, r < 32, or up row.
+    // (From here on the compiler's counts miss what is in flight: no load that it
+    // would wait for.)
     const int piece = (lane & 3) ^ (lane >> 3 & 3);           // (row / 2 % 4 == lane / 8 % 4)
     const int64_t n0 = (int64_t)nb * 128;                     // N is a multiple of 128
     const unsigned char* const xv = (const unsigned char*)a.x;
@@ -81,8 +79,7 @@ __global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks,
     uint32_t xoff[U_XL], woff[U_WL];
 #pragma unroll
     for (int j = 0; j < U_XL; j++) {
-        const int64_t r = g_xrow(a, T, 16 * (wave + U_WAVES * j) + (lane >> 2));
-        xoff[j] = r < 0 ? G_NONE : (uint32_t)(r * a.xld) + 16u * piece;
+        xoff[j] = xr[j] < 0 ? G_NONE : (uint32_t)(xr[j] * a.xld) + 16u * ((lane & 7) ^ (lane >> 3));
     }
 #pragma unroll
     for (int j = 0; j < U_WL; j++) {
@@ -99,21 +96,18 @@ __global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks,
             g_dma16(rw, dst + U_WAVES * j * 1024, in ? woff[j] : G_NONE, (uint32_t)t * U_K);
 #pragma unroll
         for (int j = 0; j < U_XL; j++)
-            g_dma16(rx, dst + U_WTILE + U_WAVES * j * 1024, xoff[j], (uint32_t)t * U_K);
+            g_dma16(rx, dst + U_WTILE + U_WAVES * j * 1024, xoff[j], (uint32_t)t * U_K * 2);
     };
-    g_scales<U_TM, U_WAVES>(a, T, lds_sc, 0, KB, wave, lane);
 #pragma unroll
     for (int t = 0; t < U_STAGES; t++) issue(t, t);
 
-    // this lane's row of fragment i (weights) or j (x): bytes 32 h .. of a half, in
-    // 16-byte pieces 2 h + q
-    uint32_t wo[2], xo[2];
+    // this lane's row of fragment i (weights) or j (x): inputs 32 h .. of a half, in
+    // 16-byte pieces 2 h + q (x: 4 h + s)
+    uint32_t wo[2], xo[4];
 #pragma unroll
-    for (int q = 0; q < 2; q++) {
-        const uint32_t p = 16u * ((2 * h + q) ^ (l32 >> 1 & 3));
-        wo[q] = (uint32_t)(64 * wave + l32) * U_K + p;
-        xo[q] = U_WTILE + (uint32_t)l32 * U_K + p;
-    }
+    for (int q = 0; q < 2; q++) wo[q] = (uint32_t)(64 * wave + l32) * U_K + 16u * ((2 * h + q) ^ (l32 >> 1 & 3));
+#pragma unroll
+    for (int s = 0; s < 4; s++) xo[s] = U_WTILE + (uint32_t)l32 * 2 * U_K + 16u * ((4 * h + s) ^ (l32 & 7));
     f32x16 acc[2][2];
 #pragma unroll
     for (int i = 0; i < 2; i++)
@@ -125,31 +119,26 @@ __global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks,
     // NJ: the tile's blocks of 32 rows
     auto run = [&](auto nj) {
         constexpr int NJ = decltype(nj)::value;
-        u32x4 w[2][2], x[NJ][2];
-        auto read = [&](int at, int q) {                      // piece q of every fragment of the half at place `at`
+        u32x4 w[2][2];
+        bf16x8 x[NJ][4];
+        // the operands of step s (weights: of two) of the half at place `at`
+        auto read = [&](int at, int s) {
             const unsigned char* st = smem + at * U_STAGE;
+            if (s % 2)
 #pragma unroll
-            for (int i = 0; i < 2; i++) w[i][q] = *(const u32x4*)(st + i * 32 * U_K + wo[q]);
+                for (int i = 0; i < 2; i++) w[i][s / 2] = *(const u32x4*)(st + i * 32 * U_K + wo[s / 2]);
 #pragma unroll
-            for (int j = 0; j < NJ; j++) x[j][q] = *(const u32x4*)(st + j * 32 * U_K + xo[q]);
+            for (int j = 0; j < NJ; j++) x[j][s] = *(const bf16x8*)(st + j * 64 * U_K + xo[s]);
         };
         g_wait<(U_STAGES - 1) * (U_WL + U_XL)>();
         lds_barrier();
 #pragma unroll
-        for (int q = 0; q < 2; q++) read(0, q);
+        for (int s = 0; s < 4; s++) read(0, s);
         int at = 0;                                           // this half's place in the ring
         for (int t0 = 0; t0 < KB; t0 += G_CHUNK) {
-            if (t0) {                                         // every wave is past its reads of the last chunk's scales
-                load_scales(t0);
-                g_scales<U_TM, U_WAVES>(a, T, lds_sc, t0, KB, wave, lane);
-                g_wait<0>();
-                lds_barrier();
-            }
+            if (t0) load_scales(t0);
             const int t1 = t0 + G_CHUNK < KB ? t0 + G_CHUNK : KB;
             for (int t = t0; t < t1; t++) {
-                float sx[NJ];
-#pragma unroll
-                for (int j = 0; j < NJ; j++) sx[j] = __uint_as_float(g_scale(sc, U_TM, 32 * j + l32, t) << 23);
                 f32x16 p[2][NJ];
 #pragma unroll
                 for (int i = 0; i < 2; i++)
@@ -166,17 +155,15 @@ __global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks,
                     at = at + 1 < U_STAGES ? at + 1 : 0;
 #pragma unroll
                     for (int s = 0; s < 4; s++) {
-                        bf16x8 wv[2], xv[NJ];
+                        bf16x8 wv[2];
 #pragma unroll
-                        for (int i = 0; i < 2; i++) wv[i] = u_operand(w[i][s / 2][s % 2 * 2], w[i][s / 2][s % 2 * 2 + 1], 1.f);
-#pragma unroll
-                        for (int j = 0; j < NJ; j++) xv[j] = u_operand(x[j][s / 2][s % 2 * 2], x[j][s / 2][s % 2 * 2 + 1], sx[j]);
+                        for (int i = 0; i < 2; i++) wv[i] = f8_values(w[i][s / 2][s % 2 * 2], w[i][s / 2][s % 2 * 2 + 1], 1.f);
 #pragma unroll
                         for (int i = 0; i < 2; i++)
 #pragma unroll
                             for (int j = 0; j < NJ; j++)
-                                p[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wv[i], xv[j], p[i][j], 0, 0, 0);
-                        if (s % 2) read(at, s / 2);
+                                p[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wv[i], x[j][s], p[i][j], 0, 0, 0);
+                        read(at, s);
                         __builtin_amdgcn_sched_barrier(0);
                     }
                 }
@@ -233,7 +220,7 @@ __global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks,
 }  // namespace
 
 int launch_fp8_glu(const F8Args& a, int64_t tiles, hipStream_t st) {
-    if (!a.tiles || a.K > FP8_GEMM_MAX_K || a.xld != fp8_row_bytes(a.K) || a.tm != U_TM || a.N % 128 ||
+    if (!a.tiles || a.K > FP8_GEMM_MAX_K || a.xld != 2 * fp8_row_bytes(a.K) || a.tm != U_TM || a.N % 128 ||
         a.xrows * a.xld >= (1LL << 31)) {
         set_error("fp8: gate|up tiles of %d rows, K=%lld, N=%lld", a.tm, (long long)a.K, (long long)a.N);
         return EINVAL_ARG;

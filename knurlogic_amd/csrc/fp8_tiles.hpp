@@ -45,20 +45,43 @@ __device__ __forceinline__ GTile g_tile(const F8Args& a, int tile) {
     return {t[0], t[1], t[2]};
 }
 
-// x row of row m of a tile, or -1
-__device__ __forceinline__ int64_t g_xrow(const F8Args& a, const GTile& t, int m) {
-    if (m >= t.count) return -1;
-    if (!a.tiles || a.in_order) return t.start + m;
-    const int rid = a.sorted[t.start + m];
-    int p = rid, in = 0;
-    if (a.Mper != 1) {
-        p = rid / (int)a.Mper;
-        in = rid - p * (int)a.Mper;
+// x rows of rows m0, m0 + by, .. of a tile, or -1: every load of a kind before the
+// first is waited for (a workgroup's start is a chain of such latencies)
+template <int N>
+__device__ __forceinline__ void g_xrows(const F8Args& a, const GTile& t, int m0, int by, int64_t (&row)[N]) {
+    if (!a.tiles || a.in_order) {
+#pragma unroll
+        for (int j = 0; j < N; j++) row[j] = m0 + by * j < t.count ? t.start + m0 + by * j : -1;
+        return;
     }
-    // p / lhs_div: half a step from every border, so exact in float64
-    const int64_t b = a.lhs ? a.lhs[p] : a.lhs_div == 1 ? p : (int)(((double)p + 0.5) * a.lhs_inv);
-    const int64_t r = b * a.Mper + in;
-    return b >= 0 && r < a.xrows ? r : -1;
+    int p[N], in[N], b[N];
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+        const int m = m0 + by * j;
+        p[j] = a.sorted[t.start + (m < t.count ? m : t.count - 1)];
+        in[j] = 0;
+    }
+    if (a.Mper != 1) {
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            const int rid = p[j];
+            p[j] = rid / (int)a.Mper;
+            in[j] = rid - p[j] * (int)a.Mper;
+        }
+    }
+    if (a.lhs) {
+#pragma unroll
+        for (int j = 0; j < N; j++) b[j] = a.lhs[p[j]];
+    } else {
+        // p / lhs_div: half a step from every border, so exact in float64
+#pragma unroll
+        for (int j = 0; j < N; j++) b[j] = (int)(((double)p[j] + 0.5) * a.lhs_inv);
+    }
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+        const int64_t r = (int64_t)b[j] * a.Mper + in[j];
+        row[j] = m0 + by * j < t.count && b[j] >= 0 && r < a.xrows ? r : -1;
+    }
 }
 
 // The scale bytes of a tile's TM rows, G_CHUNK blocks from t0, by direct-to-LDS
@@ -72,12 +95,14 @@ __device__ __forceinline__ void g_scales(const F8Args& a, const GTile& tile, uin
     static_assert(N * WAVES == G_CHUNK / 16 * G, "whole loads per wave");
     const int64_t x0 = a.tiles ? 0 : tile.start;
     const __amdgpu_buffer_rsrc_t r = make_rsrc(a.xs + x0 * a.xs_ld, (a.xrows - x0) * a.xs_ld);
+    static_assert(G == 1 || WAVES % G == 0, "a wave's loads are of the same rows");
+    int64_t row[1];
+    g_xrows(a, tile, 64 * (wave % G) + lane, 0, row);
     uint32_t off[N];
 #pragma unroll
     for (int i = 0; i < N; i++) {                // 16 blocks' piece u / G, 64 rows u % G
-        const int u = wave + WAVES * i, t = t0 + 16 * (u / G);
-        const int64_t row = g_xrow(a, tile, 64 * (u % G) + lane);
-        off[i] = row >= 0 && t < KB ? (uint32_t)((row - x0) * a.xs_ld) + t : G_NONE;
+        const int t = t0 + 16 * ((wave + WAVES * i) / G);
+        off[i] = row[0] >= 0 && t < KB ? (uint32_t)((row[0] - x0) * a.xs_ld) + t : G_NONE;
     }
 #pragma unroll
     for (int i = 0; i < N; i++) g_dma16(r, sc + (wave + WAVES * i) * 1024, off[i], 0);
