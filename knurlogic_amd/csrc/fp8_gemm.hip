@@ -31,11 +31,13 @@ struct Shape {
     static_assert(XL * 8 * WAVES == TM && WL * 8 * WAVES == TN, "whole loads per wave");
 };
 
-// TAIL: K is not a multiple of 128
-template <Kind KIND, int NW, int WM, int MB, int S, bool TAIL>
-__global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks, int tiles) {
+// TAIL: K is not a multiple of 128; MANY: several column blocks per workgroup
+template <Kind KIND, int NW, int WM, int MB, int S, bool TAIL, bool MANY>
+__global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks, int tiles, int many) {
     typedef Shape<NW, WM, MB, S> Z;
     constexpr int RB = 4, TN = Z::TN, TM = Z::TM, XL = Z::XL, WL = Z::WL, WAVES = Z::WAVES, WTILE = Z::WTILE;
+    static_assert(!MANY || S == 2, "stores among the loads in flight: their wait is for all of them");
+    const int nl = MANY ? many : 1;
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ int rid_s[TM];
     unsigned char* const sc = smem + S * Z::STAGE;            // [G_CHUNK / 16][TM][16] scale bytes
@@ -43,7 +45,7 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave % NW, wm = wave / NW;
     const int l16 = lane & 15, c = lane >> 4;
-    // workgroup -> (tile, column block): grouped as g_place; dense, each XCD takes
+    // workgroup -> (tile, nl column blocks from nb nl): grouped as g_place; dense, each XCD takes
     // an eighth of the pairs, in strips of 8 tiles (weights and x shared in its L2)
     int tile, nb;
     if (a.tiles) {
@@ -64,12 +66,18 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
     const int K = (int)a.K, KB = (K + F8_BLOCK - 1) / F8_BLOCK;
     const int64_t x0 = a.tiles ? 0 : T.start;                 // the x view's first row
     // the weights' scales of the wave's rows, 64 blocks, one per lane
-    const int64_t n0 = (int64_t)nb * TN, left = a.N - n0 < TN ? a.N - n0 : TN;
-    const int64_t SB = (a.wrows + F8_BLOCK - 1) / F8_BLOCK, nw = n0 + 64 * wn;
-    const int64_t sbase = (T.expert * SB + (nw < a.N ? nw : n0) / F8_BLOCK) * KB;
+    // (several column blocks: KB nl <= 64, all of theirs)
+    const int64_t first = (int64_t)nb * nl * TN;              // the first column
+    const int64_t SB = (a.wrows + F8_BLOCK - 1) / F8_BLOCK;
     uint32_t swl;
     auto load_scales = [&](int t) {
-        const int64_t i = sbase + (t + lane < KB ? t + lane : KB - 1);
+        int kb = t + lane, b = 0;
+        if (MANY) {
+            b = kb / KB;
+            kb -= b * KB;
+        }
+        const int64_t n = first + (int64_t)b * TN + 64 * wn;
+        const int64_t i = (T.expert * SB + (n < a.N ? n : first) / F8_BLOCK) * KB + (kb < KB ? kb : KB - 1);
         if (KIND == E8S) swl = ((const unsigned char*)a.s)[i];
         else swl = ((const uint32_t*)a.s)[i];
         asm volatile("" : "+v"(swl));            // waited for here, not in the loop
@@ -83,8 +91,7 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
     // would wait for.)
     const int piece = (lane & 7) ^ (lane >> 3);               // (row % 8 == lane / 8)
     const unsigned char* const xv = (const unsigned char*)a.x + x0 * a.xld;
-    const unsigned char* const wv = a.w + (T.expert * a.wrows + n0) * a.K;
-    const int64_t xbytes = (a.xrows - x0) * a.xld, wbytes = left * a.K;
+    const int64_t xbytes = (a.xrows - x0) * a.xld;
     uint32_t xoff[XL], woff[WL];
 #pragma unroll
     for (int j = 0; j < XL; j++) {
@@ -92,22 +99,28 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
     }
 #pragma unroll
     for (int j = 0; j < WL; j++) {
-        const int m = 8 * (wave + WAVES * j) + (lane >> 3);
-        woff[j] = m < left ? (uint32_t)m * (uint32_t)K + 16u * piece : G_NONE;
+        woff[j] = (uint32_t)(8 * (wave + WAVES * j) + (lane >> 3)) * (uint32_t)K + 16u * piece;   // (past the view: zeros)
     }
-    auto issue = [&](int t, int at) {                         // block t (past the last: zeros) into place `at`
-        const __amdgpu_buffer_rsrc_t rw = make_rsrc(wv, t < KB ? wbytes : 0), rx = make_rsrc(xv, t < KB ? xbytes : 0);
+    // the next block in turn, of this column block or the next (past the last: zeros)
+    int it = 0, rows = (int)(a.N - first < (int64_t)nl * TN ? a.N - first : (int64_t)nl * TN);
+    const unsigned char* wv = a.w + (T.expert * a.wrows + first) * a.K;
+    auto issue = [&](int at) {
+        const __amdgpu_buffer_rsrc_t rw = make_rsrc(wv, rows > 0 ? (rows < TN ? rows : TN) * K : 0);
+        const __amdgpu_buffer_rsrc_t rx = make_rsrc(xv, rows > 0 ? xbytes : 0);
         const uint32_t dst = lds + at * Z::STAGE + wave * 1024;
-        const bool in = !TAIL || t * F8_BLOCK + 16 * piece < K;       // inputs past the last: zeros
+        const bool in = !TAIL || it * F8_BLOCK + 16 * piece < K;      // inputs past the last: zeros
 #pragma unroll
         for (int j = 0; j < WL; j++)
-            g_dma16(rw, dst + WAVES * j * 1024, in ? woff[j] : G_NONE, (uint32_t)t * F8_BLOCK);
+            g_dma16(rw, dst + WAVES * j * 1024, in ? woff[j] : G_NONE, (uint32_t)it * F8_BLOCK);
 #pragma unroll
-        for (int j = 0; j < XL; j++) g_dma16(rx, dst + WTILE + WAVES * j * 1024, xoff[j], (uint32_t)t * F8_BLOCK);
+        for (int j = 0; j < XL; j++) g_dma16(rx, dst + WTILE + WAVES * j * 1024, xoff[j], (uint32_t)it * F8_BLOCK);
+        it = it + 1 < KB ? it + 1 : 0;
+        rows -= it ? 0 : TN;
+        wv += it ? 0 : TN * K;                                // (not read past the last)
     };
     g_scales<TM, WAVES>(a, T, lds_sc, 0, KB, wave, lane);
 #pragma unroll
-    for (int t = 0; t < S; t++) issue(t, t);
+    for (int t = 0; t < S; t++) issue(t);
 
     // fragment reads: weight row 64 wn + 16 i + l16, pieces c and c + 4; x row
     // 16 (MB wm + j) + l16, the same
@@ -125,11 +138,6 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
         b[j & 1] = f8_operand(*(const u32x4*)(st + j * 2048 + xo[0]), *(const u32x4*)(st + j * 2048 + xo[1]));
     };
     f32x4 acc[RB][MB];
-#pragma unroll
-    for (int i = 0; i < RB; i++)
-#pragma unroll
-        for (int j = 0; j < MB; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
     g_wait<(S - 1) * (XL + WL)>();
     lds_barrier();
 #pragma unroll
@@ -137,6 +145,13 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
     read_b(smem, 0);
     static_assert(MB % 2 == 0, "x fragments alternate");
     int at = 0;                                  // this block's place in the ring
+    for (int cb = 0; cb < nl; cb++) {
+    const int64_t n0 = first + (int64_t)cb * TN;
+    if (n0 >= a.N) break;
+#pragma unroll
+    for (int i = 0; i < RB; i++)
+#pragma unroll
+        for (int j = 0; j < MB; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int t0 = 0; t0 < KB; t0 += G_CHUNK) {
     if (t0) {                                    // every wave is past its reads of the last chunk's scales
         load_scales(t0);
@@ -152,13 +167,13 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
         uint32_t sx[MB];
 #pragma unroll
         for (int j = 0; j < MB; j++) sx[j] = g_scale(sc, TM, 16 * (MB * wm + j) + l16, t);
-        const uint32_t sw = (uint32_t)__builtin_amdgcn_readlane((int)swl, t % G_CHUNK);
+        const uint32_t sw = (uint32_t)__builtin_amdgcn_readlane((int)swl, (cb * KB + t) % G_CHUNK);
         // after the block's last LDS read: the next block has landed, and this
         // one's place is free
         auto turn = [&]() {
             g_wait<(S - 2) * (XL + WL)>();
             lds_barrier();
-            issue(t + S, at);
+            issue(at);
         };
         {
             // product n = 4 j + i; its sums are scaled two products later
@@ -196,8 +211,6 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
         at = after;
     }
     }
-    g_wait<0>();                                 // no load still writes LDS below
-
     {
         uint16_t* y = (uint16_t*)a.y;
         const bool wide = a.N % 4 == 0 && ((uintptr_t)a.y & 7) == 0;
@@ -235,6 +248,8 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
             }
         }
     }
+    }
+    g_wait<0>();                                 // no load still writes LDS when the workgroup ends
 }
 
 // x's rows into codes [rows, ld] (tails zero) and scale bytes [rows, sld]: 16
@@ -265,29 +280,40 @@ __global__ __launch_bounds__(256) void f8_rows(const typename T::storage* __rest
     if (l == 0) s[r * sld + b] = (unsigned char)byte;
 }
 
-template <Kind KIND, int NW, int WM, int MB, int S, bool TAIL>
+template <Kind KIND, int NW, int WM, int MB, int S, bool TAIL, bool MANY>
 int go(const F8Args& a, int64_t tiles, hipStream_t st) {
     typedef Shape<NW, WM, MB, S> Z;
     if (a.K > FP8_GEMM_MAX_K || a.xld != fp8_row_bytes(a.K) || a.tm > Z::TM) {
         set_error("fp8: K=%lld in tiles of %d", (long long)a.K, a.tm);
         return EINVAL_ARG;
     }
-    const int nblocks = (int)ceil_div(a.N, Z::TN);
+    // Column blocks per workgroup.  A workgroup's start (its tile, its rows, their
+    // first inputs) takes as long as some ten blocks of K: a short K takes several
+    // column blocks, their weights streaming on, while the grid keeps twice what
+    // runs at once
+    int many = 1;
+    if (MANY) {
+        const int64_t KB = ceil_div(a.K, F8_BLOCK), active = ceil_div(a.rows, a.tm) + (a.E < a.rows ? a.E : a.rows) / 2;
+        while (2 * many * KB <= 24 && active * ceil_div(a.N, 2 * many * Z::TN) >= 1536) many *= 2;
+    }
+    const int nblocks = (int)ceil_div(a.N, (int64_t)many * Z::TN);
     const int64_t wgs = a.tiles ? g_place_grid(tiles, nblocks) : ceil_div(tiles * nblocks, 8) * 8;
     if (wgs >= (1LL << 31)) {
         set_error("fp8: grid of %lld workgroups", (long long)wgs);
         return EINVAL_ARG;
     }
-    allow_dynamic_lds_once((const void*)f8_gemm<KIND, NW, WM, MB, S, TAIL>);
-    f8_gemm<KIND, NW, WM, MB, S, TAIL><<<(unsigned)wgs, 64 * Z::WAVES, Z::LDS, st>>>(a, nblocks, (int)tiles);
+    const auto f = f8_gemm<KIND, NW, WM, MB, S, TAIL, MANY>;
+    allow_dynamic_lds_once((const void*)f);
+    f<<<(unsigned)wgs, 64 * Z::WAVES, Z::LDS, st>>>(a, nblocks, (int)tiles, many);
     KMI_CHECK_LAUNCH("fp8 tiles");
     return OK;
 }
 
-template <int NW, int WM, int MB, int S>
+template <int NW, int WM, int MB, int S, bool MANY>
 int go(const F8Args& a, int64_t tiles, hipStream_t st) {
-    if (a.K % F8_BLOCK) return a.e8 ? go<E8S, NW, WM, MB, S, true>(a, tiles, st) : go<F32S, NW, WM, MB, S, true>(a, tiles, st);
-    return a.e8 ? go<E8S, NW, WM, MB, S, false>(a, tiles, st) : go<F32S, NW, WM, MB, S, false>(a, tiles, st);
+    if (a.K % F8_BLOCK)
+        return a.e8 ? go<E8S, NW, WM, MB, S, true, MANY>(a, tiles, st) : go<F32S, NW, WM, MB, S, true, MANY>(a, tiles, st);
+    return a.e8 ? go<E8S, NW, WM, MB, S, false, MANY>(a, tiles, st) : go<F32S, NW, WM, MB, S, false, MANY>(a, tiles, st);
 }
 
 }  // namespace
@@ -311,9 +337,10 @@ int launch_fp8_rows(const void* x, int dtype, int64_t rows, int64_t K, unsigned 
 }
 
 int launch_fp8_gemm(const F8Args& a, int64_t tiles, hipStream_t st) {
-    if (a.tm <= 64) return go<2, 2, 2, 3>(a, tiles, st);
-    if (a.tm <= 128) return go<2, 2, 4, 2>(a, tiles, st);
-    return go<4, 2, 8, 2>(a, tiles, st);
+    if (a.tiles) return a.tm <= 64 ? go<2, 2, 2, 2, true>(a, tiles, st) : go<2, 2, 4, 2, true>(a, tiles, st);
+    if (a.tm <= 64) return go<2, 2, 2, 3, false>(a, tiles, st);
+    if (a.tm <= 128) return go<2, 2, 4, 2, false>(a, tiles, st);
+    return go<4, 2, 8, 2, false>(a, tiles, st);
 }
 
 }  // namespace kmi
