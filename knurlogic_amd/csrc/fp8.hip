@@ -30,7 +30,7 @@ int check_workspace(const char* what, size_t need, const void* ws, size_t bytes)
     return OK;
 }
 
-// How a call runs: on f8_skinny, which quantizes x itself, or with x quantized
+// How a call runs: on f8_stream, which quantizes x itself, or with x quantized
 // ahead on f8_gemm's tiles; and the rows per tile.
 struct Plan {
     bool gemm;
@@ -38,25 +38,51 @@ struct Plan {
     bool pairs;        // f8_stream pair by pair, without the sort
 };
 
-Plan plan_dense(int64_t M, int64_t K) {
-    if (M <= 32) {
-        const int tm = M <= 16 ? 16 : 32;
-        if (K <= fp8_skinny_max_k(tm, false)) return {false, tm};
-    }
-    return {true, M <= 64 ? 64 : M <= 128 ? 128 : 256};
+//
+// Dense: the stream up to 16 rows ([4096, 4096] x 16 rows: 11 us, tiles 14.4;
+// [14336, 4096]: 20.8, 20.6), then the tiles with the least rounds x time of a
+// round.  A block of 128 inputs takes 0.5 us in tiles of 64 rows where each is
+// alone on its CU, 0.8 two to a CU; 0.9 and 1.2 in tiles of 128; 1.5 in tiles of 256
+// x 256, one to a CU.  [4096, 4096], tiles of 64 / 128 / 256: 512 rows 23 / 35 / 59
+// us, 1024 35 / 38 / 60, 2048 63 / 50 / 65, 4096 117 / 94 / 75; [14336, 4096]: 256
+// rows 37 / 38 / 62, 512 64 / 49 / 64, 1024 106 / 90 / 67.
+Plan plan_dense(int64_t M, int64_t K, int64_t N) {
+    if (M <= 16 && K <= fp8_skinny_max_k(false)) return {false, 16};
+    const auto rounds = [&](int64_t tm, int64_t tn, int64_t at_once) {
+        return ceil_div(ceil_div(M, tm) * ceil_div(N, tn), at_once);
+    };
+    const int64_t t64 = rounds(64, 128, 256) == 1 ? 5 : 8 * rounds(64, 128, 512);
+    const int64_t t128 = rounds(128, 128, 256) == 1 ? 9 : 12 * rounds(128, 128, 512);
+    const int64_t t256 = 15 * rounds(256, 256, 256);
+    return {true, t64 <= t128 && t64 <= t256 ? 64 : t128 <= t256 ? 128 : 256};
 }
 
-// rows grouped by expert: by the average rows of an active one
-Plan plan_grouped(int64_t rows, int64_t P, int64_t E, int64_t K, bool glu) {
-    const int64_t per = ceil_div(rows, P < E ? P : E);
-    if (per <= 16 && K <= fp8_skinny_max_k(16, glu)) return {false, 16, rows == P && (P <= 16 || 4 * P <= E)};
+// Grouped.  Pair by pair (no sort, no tile list; an expert's weights once per pair)
+// while few pairs share an expert: 64 experts [2048, 2048], 16 pairs 17.8 us,
+// streamed by the sorted list 25.5, tiles 22.1; 32: 28.2, 38.6, 32.3; 48: 43.0, 46.6,
+// 34.6; 8 experts [4096, 4096], 8 pairs 28.2, 37.1, 43.5, 12: 45.0, 39.0, 42.3.
+// Then the stream while the tiles would be few (8 experts [2048, 2048], 64 rows:
+// 18.0, tiles 24.6; [4096, 4096]: 64 rows 45.3, 45.2, 96 rows 52.5, 45.1; but 64
+// experts [2048, 2048], 128 rows: 56.6, 52.6), or an expert's few rows are long
+// (128 experts [1536, 4096], 256 rows: 142, 151, 512 rows: 148, 173; 128: 136, 131,
+// 768: 186, 174).  Tiles of 64 rows (gate|up's only size) up to 64 rows to an
+// expert, then 128: 64 experts [2048, 2048], 96 rows each: 97 us, in tiles of 64 104;
+// 8 experts [4096, 4096], 64 rows each: 54 both.
+Plan plan_grouped(int64_t rows, int64_t P, int64_t E, int64_t K, int64_t N, bool glu) {
+    const int64_t experts = P < E ? P : E, per = ceil_div(rows, experts);
+    if (K <= fp8_skinny_max_k(glu)) {
+        if (rows == P && (2 * P <= E || P <= (E < 8 ? E : 8))) return {false, 16, true};
+        if (per <= 8 && experts * ceil_div(N, 128) <= 512) return {false, 16};
+        if (2 <= per && per <= 4 && K > 2048) return {false, 16};
+    }
     return {true, glu || per <= 64 ? 64 : 128};
 }
 
 size_t values_bytes(int64_t rows, int64_t K) { return align256((size_t)rows * fp8_row_bytes(K) * 2); }
 
+// (a part of K may read 16 scale bytes from any word of a row)
 size_t rows_bytes(int64_t rows, int64_t K) {
-    return align256((size_t)rows * fp8_row_bytes(K)) + align256((size_t)rows * fp8_row_scales(K));
+    return align256((size_t)rows * fp8_row_bytes(K)) + align256((size_t)rows * fp8_row_scales(K) + 16);
 }
 
 // x quantized at ws (rows_bytes), as a's x
@@ -76,8 +102,11 @@ using namespace kmi;
 extern "C" {
 
 size_t kmi_qmm_fp8_workspace_bytes(int64_t M, int64_t K, int64_t N, int dtype) {
-    if (M <= 0 || K <= 0 || N <= 0 || !plan_dense(M, K).gemm) return 0;
-    return rows_bytes(M, K);
+    if (M <= 0 || K <= 0 || N <= 0) return 0;
+    const Plan p = plan_dense(M, K, N);
+    if (!p.gemm) return 0;
+    const int parts = fp8_gemm_parts(M, K, N, p.tm);
+    return rows_bytes(M, K) + (parts > 1 ? (size_t)parts * M * ceil_div(N, 4) * 16 : 0);
 }
 
 int kmi_qmm_fp8(const void* x, int64_t M, int64_t K, int64_t N, const uint32_t* w, const void* scales, int e8m0,
@@ -91,20 +120,24 @@ int kmi_qmm_fp8(const void* x, int64_t M, int64_t K, int64_t N, const uint32_t* 
     KMI_CHECK_ARG(x && w && scales && y, "%s: null pointer", what);
     rc = check_workspace(what, kmi_qmm_fp8_workspace_bytes(M, K, N, dtype), workspace, workspace_bytes);
     if (rc) return rc;
-    const Plan p = plan_dense(M, K);
+    const Plan p = plan_dense(M, K, N);
     hipStream_t st = (hipStream_t)stream;
     F8Args a = {};
     a.w = (const unsigned char*)w; a.s = scales; a.e8 = e8m0; a.E = 1; a.wrows = N; a.K = K; a.N = N;
     a.x = x; a.xrows = M; a.y = y; a.rows = M; a.tm = p.tm; a.half = dtype == F16;
     if (!p.gemm) return launch_fp8_skinny(a, dtype, false, ceil_div(M, a.tm), st);
     rc = quantize_rows(a, x, dtype, M, (char*)workspace, st);
-    return rc ? rc : launch_fp8_gemm(a, ceil_div(M, a.tm), st);
+    if (rc) return rc;
+    const int parts = fp8_gemm_parts(M, K, N, p.tm);
+    a.partial = (float*)((char*)workspace + rows_bytes(M, K));
+    a.part_ld = ceil_div(N, 4) * 4;
+    return launch_fp8_gemm(a, ceil_div(M, a.tm), parts, st);
 }
 
 size_t kmi_gather_qmm_fp8_workspace_bytes(int64_t P, int64_t X, int64_t M, int64_t E, int64_t K, int64_t N,
                                           int dtype) {
     if (P <= 0 || X <= 0 || M <= 0 || E <= 0 || K <= 0 || N <= 0) return 0;
-    const Plan p = plan_grouped(P * M, P, E, K, false);
+    const Plan p = plan_grouped(P * M, P, E, K, N, false);
     if (p.pairs) return 0;
     return sort_index_bytes(P * M, E, p.tm) + (p.gemm ? rows_bytes(X * M, K) : 0);
 }
@@ -121,7 +154,7 @@ int kmi_gather_qmm_fp8(const void* x, int64_t X, int64_t M, int64_t K, const uin
                   X < (1LL << 31) && X * M < (1LL << 31), "%s: too many rows", what);
     if (P == 0) return OK;
     KMI_CHECK_ARG(x && w && scales && lhs && rhs && y, "%s: null pointer", what);
-    const Plan p = plan_grouped(P * M, P, E, K, false);
+    const Plan p = plan_grouped(P * M, P, E, K, N, false);
     KMI_CHECK_ARG(!p.gemm || X * M * fp8_row_bytes(K) < (1LL << 31), "%s: x past 2 GiB of codes", what);
     rc = check_workspace(what, kmi_gather_qmm_fp8_workspace_bytes(P, X, M, E, K, N, dtype), workspace,
                          workspace_bytes);
@@ -143,13 +176,13 @@ int kmi_gather_qmm_fp8(const void* x, int64_t X, int64_t M, int64_t K, const uin
     }
     if (!p.gemm) return launch_fp8_skinny(a, dtype, false, sr.max_tiles, st);
     rc = quantize_rows(a, x, dtype, X * M, (char*)workspace + sort_index_bytes(P * M, E, p.tm), st);
-    return rc ? rc : launch_fp8_gemm(a, sr.max_tiles, st);
+    return rc ? rc : launch_fp8_gemm(a, sr.max_tiles, 1, st);
 }
 
 size_t kmi_switch_glu_fp8_workspace_bytes(int64_t T, int64_t H, int64_t I, int k, int64_t E) {
     if (T <= 0 || H <= 0 || I <= 0 || k <= 0 || E <= 0) return 0;
     const int64_t P = T * k;
-    const Plan p = plan_grouped(P, P, E, H > I ? H : I, true);
+    const Plan p = plan_grouped(P, P, E, H > I ? H : I, I, true);
     return align256((size_t)P * H * 2) + (p.pairs ? 0 : sort_index_bytes(P, E, p.tm)) +
            (p.gemm ? values_bytes(T, H) + rows_bytes(P, I) : align256((size_t)P * I * 2));
 }
@@ -171,7 +204,7 @@ int kmi_switch_glu_fp8(const void* x, int64_t T, int64_t H, int64_t I, int k, co
     if (T == 0) return OK;
     KMI_CHECK_ARG(x && inds && w_gu && s_gu && w_down && s_down && out, "%s: null pointer", what);
     const int64_t P = T * k;
-    const Plan p = plan_grouped(P, P, E, H > I ? H : I, true);
+    const Plan p = plan_grouped(P, P, E, H > I ? H : I, I, true);
     KMI_CHECK_ARG(!p.gemm || (2 * T * fp8_row_bytes(H) < (1LL << 31) && P * I < (1LL << 31)),
                   "%s: activations past 2 GiB", what);
     rc = check_workspace(what, kmi_switch_glu_fp8_workspace_bytes(T, H, I, k, E), workspace, workspace_bytes);
@@ -202,7 +235,7 @@ int kmi_switch_glu_fp8(const void* x, int64_t T, int64_t H, int64_t I, int k, co
         d.xs = g.ys = (unsigned char*)ws + align256((size_t)P * I);
         rc = launch_fp8_glu(g, sr.max_tiles, st);
         if (rc) return rc;
-        rc = launch_fp8_gemm(d, sr.max_tiles, st);
+        rc = launch_fp8_gemm(d, sr.max_tiles, 1, st);
     } else {
         if (p.pairs) {
             g.route = d.route = inds;

@@ -51,10 +51,12 @@ struct F8Args {
     unsigned char* ys;
     int64_t ys_ld;
     int half;                   // y is float16
+    float* partial;
+    int64_t part_ld;            // a multiple of 4, at least N
 };
 
 // tiles of up to a.tm (16 or 32; gate|up 16) rows; dtype BF16 or F16
-int64_t fp8_skinny_max_k(int tm, bool glu);
+int64_t fp8_skinny_max_k(bool glu);
 int launch_fp8_skinny(const F8Args& a, int dtype, bool glu, int64_t tiles, hipStream_t st);
 
 // out [T, N] = the combine of every token's k pairs over a's weights (bf16): pair
@@ -72,7 +74,11 @@ int launch_fp8_rows(const void* x, int dtype, int64_t rows, int64_t K, unsigned 
                     hipStream_t st);
 constexpr int64_t FP8_GEMM_MAX_K = 65536;     // a tile's rows within 32-bit offsets
 // tiles of up to a.tm (64, 128 or 256) rows over such rows
-int launch_fp8_gemm(const F8Args& a, int64_t tiles, hipStream_t st);
+// parts > 1 (dense; fp8_gemm_parts): K in parts of fp8_part_blocks blocks, their
+// sums through a.partial [parts, rows, a.part_ld]
+int fp8_gemm_parts(int64_t M, int64_t K, int64_t N, int tm);
+int fp8_part_blocks(int64_t K, int parts);
+int launch_fp8_gemm(const F8Args& a, int64_t tiles, int parts, hipStream_t st);
 // the gate|up products of expert tiles of up to 64 rows over x's values in bfloat16,
 // and their activations as codes and scale bytes, in the order of a.sorted
 int launch_fp8_glu(const F8Args& a, int64_t tiles, hipStream_t st);

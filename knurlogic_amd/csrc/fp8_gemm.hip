@@ -31,9 +31,10 @@ struct Shape {
     static_assert(XL * 8 * WAVES == TM && WL * 8 * WAVES == TN, "whole loads per wave");
 };
 
-// TAIL: K is not a multiple of 128; MANY: several column blocks per workgroup
-template <Kind KIND, int NW, int WM, int MB, int S, bool TAIL, bool MANY>
-__global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks, int tiles, int many) {
+// TAIL: K is not a multiple of 128; MANY: several column blocks per workgroup;
+// PART: blocks [per z, per z + per) of K (grid z), sums to a.partial
+template <Kind KIND, int NW, int WM, int MB, int S, bool TAIL, bool MANY, bool PART>
+__global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks, GPlace place, int tiles, int many, int per) {
     typedef Shape<NW, WM, MB, S> Z;
     constexpr int RB = 4, TN = Z::TN, TM = Z::TM, XL = Z::XL, WL = Z::WL, WAVES = Z::WAVES, WTILE = Z::WTILE;
     static_assert(!MANY || S == 2, "stores among the loads in flight: their wait is for all of them");
@@ -49,8 +50,8 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
     // an eighth of the pairs, in strips of 8 tiles (weights and x shared in its L2)
     int tile, nb;
     if (a.tiles) {
-        g_place((int)blockIdx.x, nblocks, tile, nb);
-        if (tile >= tiles) return;
+        g_place((int)blockIdx.x, place, tile, nb);
+        if (tile >= tiles || nb >= nblocks) return;
     } else {
         const int xcd = (int)blockIdx.x & 7, kk = (int)blockIdx.x >> 3;
         const int idx = xcd * ((int)gridDim.x >> 3) + kk, strip = idx / (8 * nblocks), in = idx - strip * 8 * nblocks;
@@ -63,7 +64,9 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
     const int count = T.count;
     if (count <= 0) return;
 
-    const int K = (int)a.K, KB = (K + F8_BLOCK - 1) / F8_BLOCK;
+    const int K = (int)a.K, KBs = (K + F8_BLOCK - 1) / F8_BLOCK;
+    const int kb0 = PART ? (int)blockIdx.y * per : 0, KB = PART ? KBs - kb0 < per ? KBs - kb0 : per : KBs;
+    if (PART) a.xs += kb0;
     const int64_t x0 = a.tiles ? 0 : T.start;                 // the x view's first row
     // the weights' scales of the wave's rows, 64 blocks, one per lane
     // (several column blocks: KB nl <= 64, all of theirs)
@@ -77,7 +80,7 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
             kb -= b * KB;
         }
         const int64_t n = first + (int64_t)b * TN + 64 * wn;
-        const int64_t i = (T.expert * SB + (n < a.N ? n : first) / F8_BLOCK) * KB + (kb < KB ? kb : KB - 1);
+        const int64_t i = (T.expert * SB + (n < a.N ? n : first) / F8_BLOCK) * KBs + kb0 + (kb < KB ? kb : KB - 1);
         if (KIND == E8S) swl = ((const unsigned char*)a.s)[i];
         else swl = ((const uint32_t*)a.s)[i];
         asm volatile("" : "+v"(swl));            // waited for here, not in the loop
@@ -90,8 +93,9 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
     // (From here on the compiler's counts miss what is in flight: no load that it
     // would wait for.)
     const int piece = (lane & 7) ^ (lane >> 3);               // (row % 8 == lane / 8)
-    const unsigned char* const xv = (const unsigned char*)a.x + x0 * a.xld;
-    const int64_t xbytes = (a.xrows - x0) * a.xld;
+    const int k0 = kb0 * F8_BLOCK;
+    const unsigned char* const xv = (const unsigned char*)a.x + x0 * a.xld + k0;
+    const int64_t xbytes = (a.xrows - x0) * a.xld - k0;
     uint32_t xoff[XL], woff[WL];
 #pragma unroll
     for (int j = 0; j < XL; j++) {
@@ -103,12 +107,12 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
     }
     // the next block in turn, of this column block or the next (past the last: zeros)
     int it = 0, rows = (int)(a.N - first < (int64_t)nl * TN ? a.N - first : (int64_t)nl * TN);
-    const unsigned char* wv = a.w + (T.expert * a.wrows + first) * a.K;
+    const unsigned char* wv = a.w + (T.expert * a.wrows + first) * a.K + k0;
     auto issue = [&](int at) {
-        const __amdgpu_buffer_rsrc_t rw = make_rsrc(wv, rows > 0 ? (rows < TN ? rows : TN) * K : 0);
+        const __amdgpu_buffer_rsrc_t rw = make_rsrc(wv, rows > 0 ? (rows < TN ? rows : TN) * K - k0 : 0);
         const __amdgpu_buffer_rsrc_t rx = make_rsrc(xv, rows > 0 ? xbytes : 0);
         const uint32_t dst = lds + at * Z::STAGE + wave * 1024;
-        const bool in = !TAIL || it * F8_BLOCK + 16 * piece < K;      // inputs past the last: zeros
+        const bool in = !TAIL || k0 + it * F8_BLOCK + 16 * piece < K;      // inputs past the last: zeros
 #pragma unroll
         for (int j = 0; j < WL; j++)
             g_dma16(rw, dst + WAVES * j * 1024, in ? woff[j] : G_NONE, (uint32_t)it * F8_BLOCK);
@@ -228,6 +232,10 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
 #pragma unroll
             for (int i = 0; i < RB; i++) {
                 const int64_t n = n0 + 64 * wn + 16 * i + 4 * c;
+                if constexpr (PART) {            // rows of whole blocks of 4
+                    if (n < a.N) *(f32x4*)(a.partial + ((int64_t)blockIdx.y * a.rows + rid) * a.part_ld + n) = acc[i][j];
+                    continue;
+                }
                 u32x2 o;
                 if (a.half) {
                     o.x = f32_to_f16(acc[i][j][0]) | (uint32_t)f32_to_f16(acc[i][j][1]) << 16;
@@ -250,6 +258,23 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
     }
     }
     g_wait<0>();                                 // no load still writes LDS when the workgroup ends
+}
+
+// y[m, n] = the parts' sums, in order, rounded once: 4 columns per thread
+__global__ __launch_bounds__(256) void f8_reduce(const float* __restrict__ part, int parts, int64_t rows, int64_t ld,
+                                                 int64_t N, int half, uint16_t* __restrict__ y) {
+    const int64_t per = ld / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= rows * per) return;
+    const int64_t m = i / per, n = i % per * 4;
+    f32x4 v = *(const f32x4*)(part + m * ld + n);
+    for (int p = 1; p < parts; p++) {
+        const f32x4 o = *(const f32x4*)(part + (p * rows + m) * ld + n);
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] += o[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (n + e < N) y[m * N + n + e] = half ? f32_to_f16(v[e]) : f32_to_bf16(v[e]);
 }
 
 // x's rows into codes [rows, ld] (tails zero) and scale bytes [rows, sld]: 16
@@ -280,40 +305,55 @@ __global__ __launch_bounds__(256) void f8_rows(const typename T::storage* __rest
     if (l == 0) s[r * sld + b] = (unsigned char)byte;
 }
 
-template <Kind KIND, int NW, int WM, int MB, int S, bool TAIL, bool MANY>
-int go(const F8Args& a, int64_t tiles, hipStream_t st) {
+template <Kind KIND, int NW, int WM, int MB, int S, bool TAIL, bool MANY, bool PART>
+int go(const F8Args& a, int64_t tiles, int parts, hipStream_t st) {
     typedef Shape<NW, WM, MB, S> Z;
     if (a.K > FP8_GEMM_MAX_K || a.xld != fp8_row_bytes(a.K) || a.tm > Z::TM) {
         set_error("fp8: K=%lld in tiles of %d", (long long)a.K, a.tm);
         return EINVAL_ARG;
     }
     // Column blocks per workgroup.  A workgroup's start (its tile, its rows, their
-    // first inputs) takes as long as some ten blocks of K: a short K takes several
-    // column blocks, their weights streaming on, while the grid keeps twice what
-    // runs at once
+    // first inputs) takes as long as some ten blocks of K, so a short K takes
+    // several column blocks, their weights streaming on, while the grid keeps twice
+    // what runs at once (16384 rows of 128 experts [2048, 768]: 4 blocks 84 us, 1
+    // 105); so does any K where most of a tile is empty, and the weights' stream is
+    // all there is, while two workgroups come to a CU (512 rows of 64 experts
+    // [2048, 2048]: 2 blocks 61.9 us, 1 65.7, 4 78.0; 4096 rows: 88.2, 89.1, 101.8).
+    const int64_t KB = ceil_div(a.K, F8_BLOCK);
     int many = 1;
     if (MANY) {
-        const int64_t KB = ceil_div(a.K, F8_BLOCK), active = ceil_div(a.rows, a.tm) + (a.E < a.rows ? a.E : a.rows) / 2;
+        const int64_t experts = a.E < a.rows ? a.E : a.rows, some = ceil_div(a.rows, a.tm) + experts / 2;
+        const int64_t active = some > experts ? some : experts;
         while (2 * many * KB <= 24 && active * ceil_div(a.N, 2 * many * Z::TN) >= 1536) many *= 2;
+        if (many == 1 && 2 * KB <= G_CHUNK && a.rows < 64 * a.E && active * ceil_div(a.N, 2 * Z::TN) >= 512) many = 2;
     }
     const int nblocks = (int)ceil_div(a.N, (int64_t)many * Z::TN);
-    const int64_t wgs = a.tiles ? g_place_grid(tiles, nblocks) : ceil_div(tiles * nblocks, 8) * 8;
+    const GPlace place = g_place_of(nblocks);
+    const int64_t wgs = a.tiles ? g_place_grid(tiles, place) : ceil_div(tiles * nblocks, 8) * 8;
     if (wgs >= (1LL << 31)) {
         set_error("fp8: grid of %lld workgroups", (long long)wgs);
         return EINVAL_ARG;
     }
-    const auto f = f8_gemm<KIND, NW, WM, MB, S, TAIL, MANY>;
+    const auto f = f8_gemm<KIND, NW, WM, MB, S, TAIL, MANY, PART>;
     allow_dynamic_lds_once((const void*)f);
-    f<<<(unsigned)wgs, 64 * Z::WAVES, Z::LDS, st>>>(a, nblocks, (int)tiles, many);
+    const int per = PART ? fp8_part_blocks(a.K, parts) : 0;
+    f<<<dim3((unsigned)wgs, (unsigned)parts), 64 * Z::WAVES, Z::LDS, st>>>(a, nblocks, place, (int)tiles, many, per);
     KMI_CHECK_LAUNCH("fp8 tiles");
+    if (PART) {
+        const int64_t n = ceil_div(a.rows * (a.part_ld / 4), 256);
+        f8_reduce<<<(unsigned)n, 256, 0, st>>>(a.partial, parts, a.rows, a.part_ld, a.N, a.half, (uint16_t*)a.y);
+        KMI_CHECK_LAUNCH("fp8 parts");
+    }
     return OK;
 }
 
-template <int NW, int WM, int MB, int S, bool MANY>
-int go(const F8Args& a, int64_t tiles, hipStream_t st) {
+template <int NW, int WM, int MB, int S, bool MANY, bool PART>
+int go(const F8Args& a, int64_t tiles, int parts, hipStream_t st) {
     if (a.K % F8_BLOCK)
-        return a.e8 ? go<E8S, NW, WM, MB, S, true, MANY>(a, tiles, st) : go<F32S, NW, WM, MB, S, true, MANY>(a, tiles, st);
-    return a.e8 ? go<E8S, NW, WM, MB, S, false, MANY>(a, tiles, st) : go<F32S, NW, WM, MB, S, false, MANY>(a, tiles, st);
+        return a.e8 ? go<E8S, NW, WM, MB, S, true, MANY, PART>(a, tiles, parts, st)
+                    : go<F32S, NW, WM, MB, S, true, MANY, PART>(a, tiles, parts, st);
+    return a.e8 ? go<E8S, NW, WM, MB, S, false, MANY, PART>(a, tiles, parts, st)
+                : go<F32S, NW, WM, MB, S, false, MANY, PART>(a, tiles, parts, st);
 }
 
 }  // namespace
@@ -336,11 +376,29 @@ int launch_fp8_rows(const void* x, int dtype, int64_t rows, int64_t K, unsigned 
     return OK;
 }
 
-int launch_fp8_gemm(const F8Args& a, int64_t tiles, hipStream_t st) {
-    if (a.tiles) return a.tm <= 64 ? go<2, 2, 2, 2, true>(a, tiles, st) : go<2, 2, 4, 2, true>(a, tiles, st);
-    if (a.tm <= 64) return go<2, 2, 2, 3, false>(a, tiles, st);
-    if (a.tm <= 128) return go<2, 2, 4, 2, false>(a, tiles, st);
-    return go<4, 2, 8, 2, false>(a, tiles, st);
+int fp8_part_blocks(int64_t K, int parts) {
+    return (int)(ceil_div(ceil_div(ceil_div(K, F8_BLOCK), parts), 4) * 4);       // (scale bytes in words)
+}
+
+// Dense products of few tiles split K into parts of at least 8 blocks, while a CU
+// has no workgroup.  [4096, 14336] x 33 rows (32 tiles): 8 parts 22.5 us, 4 27.0,
+// whole 56.1; [14336, 4096] x 64 (112): 2 parts 23.9, 4 28.0, whole 26.0; [4096,
+// 4096] x 256 (128): 2 parts 22.0, whole 21.7.  A K of 17 blocks: 2 parts 14.4,
+// whole 14.2.
+int fp8_gemm_parts(int64_t M, int64_t K, int64_t N, int tm) {
+    const int64_t wgs = ceil_div(M, tm) * ceil_div(N, 128), KB = ceil_div(K, F8_BLOCK);
+    if (tm > 64 || KB < 32) return 1;
+    const int64_t idle = 256 / wgs, most = KB / 8;
+    const int parts = (int)(idle < most ? idle : most);
+    return parts < 2 ? 1 : (int)ceil_div(KB, fp8_part_blocks(K, parts));
+}
+
+int launch_fp8_gemm(const F8Args& a, int64_t tiles, int parts, hipStream_t st) {
+    if (a.tiles) return a.tm <= 64 ? go<2, 2, 2, 2, true, false>(a, tiles, 1, st) : go<2, 2, 4, 2, true, false>(a, tiles, 1, st);
+    if (parts > 1) return go<2, 2, 2, 3, false, true>(a, tiles, parts, st);
+    if (a.tm <= 64) return go<2, 2, 2, 3, false, false>(a, tiles, 1, st);
+    if (a.tm <= 128) return go<2, 2, 4, 2, false, false>(a, tiles, 1, st);
+    return go<4, 2, 8, 2, false, false>(a, tiles, 1, st);
 }
 
 }  // namespace kmi

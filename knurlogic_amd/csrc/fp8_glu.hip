@@ -31,15 +31,15 @@ constexpr int U_ROW = 272;                                             // bytes 
 
 // TAIL: K is not a multiple of 64
 template <bool TAIL>
-__global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks, int tiles) {
+__global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks, GPlace place, int tiles) {
     extern __shared__ __align__(16) unsigned char smem[];
     const uint32_t lds = g_lds(smem);
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l32 = lane & 31, h = lane >> 5;
     int tile, nb;
-    g_place((int)blockIdx.x, nblocks, tile, nb);
-    if (tile >= tiles) return;
+    g_place((int)blockIdx.x, place, tile, nb);
+    if (tile >= tiles || nb >= nblocks) return;
     const GTile T = g_tile(a, tile);
     const int count = T.count;
     if (count <= 0) return;
@@ -225,14 +225,16 @@ int launch_fp8_glu(const F8Args& a, int64_t tiles, hipStream_t st) {
         set_error("fp8: gate|up tiles of %d rows, K=%lld, N=%lld", a.tm, (long long)a.K, (long long)a.N);
         return EINVAL_ARG;
     }
-    const int64_t nblocks = a.N / 128, wgs = g_place_grid(tiles, nblocks);
+    const int64_t nblocks = a.N / 128;
+    const GPlace place = g_place_of(nblocks);
+    const int64_t wgs = g_place_grid(tiles, place);
     if (wgs >= (1LL << 31)) {
         set_error("fp8: grid of %lld workgroups", (long long)wgs);
         return EINVAL_ARG;
     }
     const auto f = a.K % U_K ? f8_glu<true> : f8_glu<false>;
     allow_dynamic_lds_once((const void*)f);
-    f<<<(unsigned)wgs, 64 * U_WAVES, U_LDS, st>>>(a, (int)nblocks, (int)tiles);
+    f<<<(unsigned)wgs, 64 * U_WAVES, U_LDS, st>>>(a, (int)nblocks, place, (int)tiles);
     KMI_CHECK_LAUNCH("fp8 gate|up");
     return OK;
 }

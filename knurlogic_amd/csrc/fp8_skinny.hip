@@ -1,4 +1,4 @@
-// Block-scaled E4M3 products of few rows: tiles of up to 16 or 32 activation rows
+// Block-scaled E4M3 products of few rows: tiles of up to 16 activation rows
 // against 16-row blocks of weights.
 //
 // The 8 waves of a workgroup split into KP parts of K (part v takes the 128-input
@@ -45,19 +45,19 @@ __device__ __forceinline__ f32x4 st_times(const i32x8& w, const i32x8& x) {
 
 // R row blocks per wave and step; KPW blocks of K per wave at most
 // and W waves (GLU: 3 workgroups of 4 on a CU, or one of 8; else 2 or 1 of 8)
-template <class T, int MB, int KP, int KPW, int R, bool GLU, int W>
-__global__ __launch_bounds__(64 * W, W == 4 ? 3 : GLU || KPW * MB >= 8 ? 2 : 4) void f8_stream(F8Args a, int steps) {
+template <class T, int KP, int KPW, int R, bool GLU, int W>
+__global__ __launch_bounds__(64 * W, W == 4 ? 3 : GLU || KPW >= 8 ? 2 : 4) void f8_stream(F8Args a, int steps) {
     constexpr int RB = GLU ? 2 : 1, NP = W / KP, F = R * RB * KPW;
     // weight blocks (2 KB) in flight per wave: 8, or 4 where x, or gate|up's float16
     // operands, take the registers
-    constexpr int DEPTH = GLU || KPW * MB >= 16 ? 4 : 8, D = F < DEPTH ? F : DEPTH;
-    constexpr int BATCH = KPW * MB < 4 ? KPW : 4 / MB;       // x blocks quantized at a time
+    constexpr int DEPTH = GLU || KPW >= 16 ? 4 : 8, D = F < DEPTH ? F : DEPTH;
+    constexpr int BATCH = KPW < 4 ? KPW : 4;       // x blocks quantized at a time
     static_assert(F % D == 0 && KPW % BATCH == 0, "ring");
     // a wave's x codes, and after them its sums (two steps'), in turn
-    constexpr int SUMS = R * RB * MB * 1024, AREA = 2 * SUMS > BATCH * MB * 2048 ? 2 * SUMS : BATCH * MB * 2048;
+    constexpr int SUMS = R * RB * 1024, AREA = 2 * SUMS > BATCH * 2048 ? 2 * SUMS : BATCH * 2048;
     __shared__ __align__(16) unsigned char area[W][AREA];
-    __shared__ unsigned char xe[W][BATCH * MB * 16];
-    __shared__ int rid_s[16 * MB], xrow_s[16 * MB];
+    __shared__ unsigned char xe[W][BATCH * 16];
+    __shared__ int rid_s[16], xrow_s[16];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kp = wave % KP, np = wave / KP;
     const int l16 = lane & 15, c = lane >> 4;
@@ -119,7 +119,7 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : GLU || KPW * MB >= 8 ? 2 : 4) 
 #pragma unroll
     for (int q = 0; q < D; q++) load(q, step);
 
-    if (tid < 16 * MB) {
+    if (tid < 16) {
         int rid = -1, xr = -1;
         if (tid < count) {
             rid = a.tiles ? a.sorted[start + tid] : (int)(start + tid);
@@ -138,19 +138,17 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : GLU || KPW * MB >= 8 ? 2 : 4) 
 
     // x blocks of this part: 16 lanes quantize 128 inputs of a row, BATCH blocks of
     // a row at once, through LDS (pieces permuted by the row) into the operand
-    i32x8 x[KPW][MB];
-    float xf[KPW][MB];
+    i32x8 x[KPW];
+    float xf[KPW];
 #pragma unroll
     for (int b0 = 0; b0 < KPW; b0 += BATCH) {
         const int kb = kp + KP * (b0 + c), k = kb * F8_BLOCK + 8 * l16;
         if (kp + KP * b0 >= KB) {                            // (no block of this batch)
 #pragma unroll
-            for (int i = b0; i < b0 + BATCH; i++)
-#pragma unroll
-                for (int j = 0; j < MB; j++) {
-                    x[i][j] = i32x8{0, 0, 0, 0, 0, 0, 0, 0};
-                    xf[i][j] = 0.f;
-                }
+            for (int i = b0; i < b0 + BATCH; i++) {
+                x[i] = i32x8{0, 0, 0, 0, 0, 0, 0, 0};
+                xf[i] = 0.f;
+            }
             continue;
         }
         auto rows = [&](int m0, auto many) {                 // several rows' loads before the first is used
@@ -171,8 +169,8 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : GLU || KPW * MB >= 8 ? 2 : 4) 
                 const u32x2 o = nan ? u32x2{0x7f7f7f7fu, 0x7f7f7f7fu} : u32x2{v[g].codes(0, scale), v[g].codes(1, scale)};
                 const int m = m0 + g;
                 if (c < BATCH && m < count) {
-                    *(u32x2*)(area[wave] + (c * MB * 16 + m) * 128 + 16 * ((l16 >> 1) ^ (m & 7)) + 8 * (l16 & 1)) = o;
-                    if (l16 == 0) xe[wave][c * MB * 16 + m] = (unsigned char)byte;
+                    *(u32x2*)(area[wave] + (c * 16 + m) * 128 + 16 * ((l16 >> 1) ^ (m & 7)) + 8 * (l16 & 1)) = o;
+                    if (l16 == 0) xe[wave][c * 16 + m] = (unsigned char)byte;
                 }
             }
         };
@@ -181,70 +179,59 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : GLU || KPW * MB >= 8 ? 2 : 4) 
             for (int m = 0; m < count; m += 8) rows(m, std::integral_constant<int, 8>());
         // (a wave reads what it wrote: LDS is in order within it)
 #pragma unroll
-        for (int i = 0; i < BATCH; i++)
+        for (int i = 0; i < BATCH; i++) {
+            const int m = l16;
+            const bool on = m < count && kp + KP * (b0 + i) < KB;
+            const unsigned char* row = area[wave] + (i * 16 + m) * 128;
+            i32x8 v = f8_operand(*(const u32x4*)(row + 16 * (c ^ (m & 7))), *(const u32x4*)(row + 16 * ((c + 4) ^ (m & 7))));
 #pragma unroll
-            for (int j = 0; j < MB; j++) {
-                const int m = 16 * j + l16;
-                const bool on = m < count && kp + KP * (b0 + i) < KB;
-                const unsigned char* row = area[wave] + (i * MB * 16 + m) * 128;
-                i32x8 v = f8_operand(*(const u32x4*)(row + 16 * (c ^ (m & 7))), *(const u32x4*)(row + 16 * ((c + 4) ^ (m & 7))));
-#pragma unroll
-                for (int q = 0; q < 8; q++) v[q] = on ? v[q] : 0;
-                x[b0 + i][j] = v;
-                xf[b0 + i][j] = on ? __uint_as_float((uint32_t)xe[wave][i * MB * 16 + m] << 23) : 0.f;
-            }
+            for (int q = 0; q < 8; q++) v[q] = on ? v[q] : 0;
+            x[b0 + i] = v;
+            xf[b0 + i] = on ? __uint_as_float((uint32_t)xe[wave][i * 16 + m] << 23) : 0.f;
+        }
     }
 
     for (int buf = 0; step < steps; buf ^= 1) {
         const int next = step + (int)gridDim.x;
         // (opaque: float16 operands are made where they are used, not kept)
 #pragma unroll
-        for (int i = 0; i < KPW; i++)
-#pragma unroll
-            for (int j = 0; j < MB; j++) asm volatile("" : "+v"(x[i][j]));
+        for (int i = 0; i < KPW; i++) asm volatile("" : "+v"(x[i]));
         float s[RB];
 #pragma unroll
         for (int g = 0; g < RB; g++) s[g] = a.e8 ? e8m0_to_f32(sv[g]) : __uint_as_float(sv[g]);
         load_scales(next);
-        f32x4 acc[R][RB][MB];
+        f32x4 acc[R][RB];
 #pragma unroll
         for (int r = 0; r < R; r++)
 #pragma unroll
-            for (int g = 0; g < RB; g++)
-#pragma unroll
-                for (int j = 0; j < MB; j++) acc[r][g][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int g = 0; g < RB; g++) acc[r][g] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int q = 0; q < F; q++) {
             const int g = q % RB, i = q / RB % KPW, r = q / RB / KPW;
             const float sw = __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(s[g]), i));
+            // codes' products first, then both scales at once: no step leaves
+            // float32's range that the result does not
+            const f32x4 p = st_times<GLU>(wr[q % D], x[i]);
+            const float f = kp + KP * i < KB ? sw * xf[i] : 0.f;
 #pragma unroll
-            for (int j = 0; j < MB; j++) {
-                // codes' products first, then both scales at once: no step leaves
-                // float32's range that the result does not
-                const f32x4 p = st_times<GLU>(wr[q % D], x[i][j]);
-                const float f = kp + KP * i < KB ? sw * xf[i][j] : 0.f;
-#pragma unroll
-                for (int e = 0; e < 4; e++) acc[r][g][j][e] = __builtin_fmaf(p[e], f, acc[r][g][j][e]);
-            }
+            for (int e = 0; e < 4; e++) acc[r][g][e] = __builtin_fmaf(p[e], f, acc[r][g][e]);
             load((q + D) % F, q + D < F ? step : next);
             if constexpr (GLU) __builtin_amdgcn_sched_barrier(0);    // one block's float16 operands at a time
         }
 #pragma unroll
         for (int r = 0; r < R; r++)
 #pragma unroll
-            for (int g = 0; g < RB; g++)
-#pragma unroll
-                for (int j = 0; j < MB; j++) *(f32x4*)(area[wave] + buf * SUMS + ((r * RB + g) * MB + j) * 1024 + 16 * lane) = acc[r][g][j];
+            for (int g = 0; g < RB; g++) *(f32x4*)(area[wave] + buf * SUMS + (r * RB + g) * 1024 + 16 * lane) = acc[r][g];
         lds_barrier();
         // D: row 4 (l / 16) + e of the block, activation row l % 16
-        for (int idx = tid; idx < NP * R * MB * 64; idx += 64 * W) {
-            const int l = idx & 63, j = idx / 64 % MB, r = idx / 64 / MB % R, p = idx / 64 / MB / R;
-            const int tok = 16 * j + (l & 15), rid = rid_s[tok];
+        for (int idx = tid; idx < NP * R * 64; idx += 64 * W) {
+            const int l = idx & 63, r = idx / 64 % R, p = idx / 64 / R;
+            const int tok = l & 15, rid = rid_s[tok];
             if (rid < 0) continue;
             f32x4 v[RB];
 #pragma unroll
             for (int g = 0; g < RB; g++) {
-                const int at = buf * SUMS + ((r * RB + g) * MB + j) * 1024 + 16 * l;
+                const int at = buf * SUMS + (r * RB + g) * 1024 + 16 * l;
                 v[g] = *(const f32x4*)(area[p * KP] + at);
 #pragma unroll
                 for (int w = 1; w < KP; w++) {
@@ -352,58 +339,61 @@ __global__ __launch_bounds__(64 * ST_WAVES) void f8_combine(F8Args a, const uint
 // workgroups of 8 waves that stream at once: two on each CU
 constexpr int64_t ST_GRID = 512;
 
-template <class T, int MB, int KP, int KPW, int R, bool GLU, int W = ST_WAVES>
+template <class T, int KP, int KPW, int R, bool GLU, int W = ST_WAVES>
 int go(const F8Args& a, int64_t tiles, hipStream_t st) {
     const int64_t steps = ceil_div(a.N, 16 * R * (W / KP));
     if (steps >= (1LL << 31)) {
         set_error("fp8: N=%lld", (long long)a.N);
         return EINVAL_ARG;
     }
-    // as many workgroups per tile as keep every one's steps alike
-    const int64_t per = ceil_div(steps * tiles, W == 4 ? 3 * ST_GRID / 2 : ST_GRID);
-    const int64_t gx = ceil_div(steps, per < steps ? per : steps);
-    f8_stream<T, MB, KP, KPW, R, GLU, W><<<dim3((unsigned)gx, (unsigned)tiles), 64 * W, 0, st>>>(a, (int)steps);
+    // as many workgroups per tile as keep every one's steps alike and run at once
+    // (16 more than that are a second round: 24 pairs [2048, 4096], 528 workgroups
+    // 52.1 us, 456 43.1); of sorted tiles some are empty, and a few more run
+    // (512 rows of 128 experts [1536, 4096]: 148 us, 181 with the first rule)
+    constexpr int64_t most = W == 4 ? 3 * ST_GRID / 2 : ST_GRID;
+    int64_t per = ceil_div(steps, tiles < most ? most / tiles : 1);
+    if (a.tiles) per = ceil_div(steps * tiles, most) < steps ? ceil_div(steps * tiles, most) : steps;
+    const int64_t gx = ceil_div(steps, per);
+    f8_stream<T, KP, KPW, R, GLU, W><<<dim3((unsigned)gx, (unsigned)tiles), 64 * W, 0, st>>>(a, (int)steps);
     KMI_CHECK_LAUNCH("fp8 stream");
     return OK;
 }
 
 // The parts of K: as few as leave a wave's x in its registers (KPW blocks), so that
 // a part with no block is rare.
-template <class T, int MB, bool GLU>
+template <class T, bool GLU>
 int parts(const F8Args& a, int64_t tiles, hipStream_t st) {
     const int64_t KB = ceil_div(a.K, F8_BLOCK);
     if constexpr (GLU) {
-        if (KB <= 4) return go<T, MB, 2, 2, 1, GLU, 4>(a, tiles, st);
-        if (KB <= 8) return go<T, MB, 2, 4, 1, GLU, 4>(a, tiles, st);
-        if (KB <= 16) return go<T, MB, 4, 4, 1, GLU, 4>(a, tiles, st);
-        if (KB <= 32) return go<T, MB, 8, 4, 1, GLU>(a, tiles, st);
-        if (KB <= 64) return go<T, MB, 8, 8, 1, GLU>(a, tiles, st);
+        if (KB <= 4) return go<T, 2, 2, 1, GLU, 4>(a, tiles, st);
+        if (KB <= 8) return go<T, 2, 4, 1, GLU, 4>(a, tiles, st);
+        if (KB <= 16) return go<T, 4, 4, 1, GLU, 4>(a, tiles, st);
+        if (KB <= 32) return go<T, 8, 4, 1, GLU>(a, tiles, st);
+        if (KB <= 64) return go<T, 8, 8, 1, GLU>(a, tiles, st);
     } else {
-        if (KB <= 2) return go<T, MB, 2, 1, 4, GLU>(a, tiles, st);
-        if (KB <= 4) return go<T, MB, 2, 2, 2, GLU>(a, tiles, st);
-        if (KB <= 8) return go<T, MB, 2, 4, 1, GLU>(a, tiles, st);
-        if (KB <= 16) return go<T, MB, 4, 4, 1, GLU>(a, tiles, st);
-        if (KB <= 32) return go<T, MB, 8, 4, 1, GLU>(a, tiles, st);
-        if (KB <= 64) return go<T, MB, 8, 8, 1, GLU>(a, tiles, st);
+        if (KB <= 2) return go<T, 2, 1, 4, GLU>(a, tiles, st);
+        if (KB <= 4) return go<T, 2, 2, 2, GLU>(a, tiles, st);
+        if (KB <= 8) return go<T, 2, 4, 1, GLU>(a, tiles, st);
+        if (KB <= 16) return go<T, 4, 4, 1, GLU>(a, tiles, st);
+        if (KB <= 32) return go<T, 8, 4, 1, GLU>(a, tiles, st);
+        if (KB <= 64) return go<T, 8, 8, 1, GLU>(a, tiles, st);
     }
-    if constexpr (MB == 1 && !GLU) return go<T, MB, 8, 16, 1, GLU>(a, tiles, st);
+    if constexpr (!GLU) return go<T, 8, 16, 1, GLU>(a, tiles, st);
     set_error("fp8: K=%lld for tiles of %d rows", (long long)a.K, a.tm);
     return EINVAL_ARG;
 }
 
 }  // namespace
 
-int64_t fp8_skinny_max_k(int tm, bool glu) { return tm <= 16 && !glu ? 16384 : 8192; }
+int64_t fp8_skinny_max_k(bool glu) { return glu ? 8192 : 16384; }
 
 int launch_fp8_skinny(const F8Args& a, int dtype, bool glu, int64_t tiles, hipStream_t st) {
-    if (tiles <= 0 || tiles >= 65536 || a.tm < 1 || a.tm > (glu ? 16 : 32) || (glu && dtype != BF16) ||
-        a.K > fp8_skinny_max_k(a.tm, glu)) {
+    if (tiles <= 0 || tiles >= 65536 || a.tm < 1 || a.tm > 16 || (glu && dtype != BF16) || a.K > fp8_skinny_max_k(glu)) {
         set_error("fp8: %lld tiles of %d rows, K=%lld", (long long)tiles, a.tm, (long long)a.K);
         return EINVAL_ARG;
     }
-    if (glu) return parts<F8BF16, 1, true>(a, tiles, st);
-    if (a.tm <= 16) return dtype == BF16 ? parts<F8BF16, 1, false>(a, tiles, st) : parts<F8F16, 1, false>(a, tiles, st);
-    return dtype == BF16 ? parts<F8BF16, 2, false>(a, tiles, st) : parts<F8F16, 2, false>(a, tiles, st);
+    if (glu) return parts<F8BF16, true>(a, tiles, st);
+    return dtype == BF16 ? parts<F8BF16, false>(a, tiles, st) : parts<F8F16, false>(a, tiles, st);
 }
 
 bool fp8_combine_supported(int64_t K, int k) { return K <= CB_MAX_K && k <= CB_MAX_SLOTS; }

@@ -112,14 +112,27 @@ __device__ __forceinline__ uint32_t g_scale(const unsigned char* sc, int TM, int
 }
 
 // Grouped tiles: workgroup -> (tile, column block).  Workgroups go to the 8 XCDs
-// in turn; 4 neighbouring tiles (often one expert's) of every column block stay on
-// one XCD, whose L2 then serves the others, the next 4 go to the next (tiles at
-// the list's end are empty: they must not all fall to one).
-__device__ __forceinline__ void g_place(int id, int nblocks, int& tile, int& nb) {
-    const int xcd = id & 7, kk = id >> 3;
-    tile = ((kk / (4 * nblocks)) * 8 + xcd) * 4 + kk % 4;
-    nb = kk / 4 % nblocks;
+// in turn.  A unit is 4 neighbouring tiles (often one expert's) x `cols` column
+// blocks: it stays on one XCD, whose L2 then serves its weights to the other tiles
+// and its rows to the other columns; the next unit goes to the next XCD.  Units of
+// up to 4, all alike (a last one of 2 of 6 columns left half the XCDs a third less:
+// 302 us for 276): with all columns in one, few tiles fill few XCDs (512 rows of 8 experts
+// [4096, 4096]: 92.6 us, 53.8 so); with 1, many tiles' rows go through every L2
+// (32768 rows of 128 experts [1536, 4096]: 500 us, 474 so).
+struct GPlace {
+    int units, cols;            // units to a group of 4 tiles, column blocks to a unit
+};
+__device__ __forceinline__ void g_place(int id, GPlace p, int& tile, int& nb) {
+    const int kk = id >> 3, v = kk / (4 * p.cols), u = v * 8 + (id & 7), in = kk - 4 * p.cols * v;
+    tile = u / p.units * 4 + in % 4;
+    nb = u % p.units * p.cols + in / 4;
 }
-inline int64_t g_place_grid(int64_t tiles, int64_t nblocks) { return ceil_div(tiles, 32) * 32 * nblocks; }
+inline GPlace g_place_of(int64_t nblocks) {
+    const int64_t cols = nblocks % 4 == 0 ? 4 : nblocks % 3 == 0 ? 3 : nblocks % 2 == 0 ? 2 : 1;
+    return {(int)ceil_div(nblocks, cols), (int)cols};
+}
+inline int64_t g_place_grid(int64_t tiles, GPlace p) {
+    return ceil_div(ceil_div(tiles, 4) * p.units, 8) * 32 * p.cols;
+}
 
 }  // namespace kmi
