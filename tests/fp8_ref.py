@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import numpy as np
+import torch
 
 BLOCK = 128
 
@@ -33,29 +34,24 @@ def nearest(v):
 
 
 def exponent(amax):
-    """The smallest e >= -126 with amax <= 448 * 2^e."""
-    e = -126
-    while amax > 448 * 2.0 ** e:
-        e += 1
-    return e
+    """The smallest e >= -126 with amax <= 448 * 2^e (448 = 0.875 * 2^9)."""
+    f, x = np.frexp(amax)
+    return np.where(np.asarray(amax) > 0, np.maximum(x - np.where(f <= 0.875, 9, 8), -126), -126)
 
 
 def block_scales(w, bn, bk):
     """Codes uint8 [N, K] and scale bytes [N/bn, K/bk] of w (float64)."""
     N, K = w.shape
-    q = np.zeros((N, K), np.uint8)
-    s = np.zeros((-(-N // bn), -(-K // bk)), np.uint8)
-    for i in range(s.shape[0]):
-        for j in range(s.shape[1]):
-            at = (slice(i * bn, (i + 1) * bn), slice(j * bk, (j + 1) * bk))
-            top = np.abs(w[at]).max()
-            if not np.isfinite(top):
-                s[i, j] = 255
-                continue
-            e = exponent(top)
-            s[i, j] = e + 127
-            q[at] = nearest(w[at] / 2.0 ** e)
-    return q, s
+    n, k = -(-N // bn), -(-K // bk)
+    p = np.zeros((n * bn, k * bk))
+    p[:N, :K] = w
+    top = np.abs(p).reshape(n, bn, k, bk).max((1, 3))
+    bad = ~np.isfinite(top)
+    e = exponent(np.where(bad, 1.0, top))
+    wide = lambda v: np.repeat(np.repeat(v, bn, 0)[:N], bk, 1)[:, :K]
+    with np.errstate(invalid="ignore"):
+        q = np.where(wide(bad), 0, nearest(np.where(wide(bad), 0, w) / 2.0 ** wide(e)))
+    return q.astype(np.uint8), np.where(bad, 255, e + 127).astype(np.uint8)
 
 
 def scale_values(s):
@@ -84,12 +80,12 @@ def product(x, q, s):
     """(y, sum of the products' magnitudes, sum over the runs of 8 inputs of
     the largest product's) of x against one weight."""
     a, b = rows(x), weights(q, s)
-    m, n = np.abs(a), np.abs(b)
-    cut = np.zeros((a.shape[0], b.shape[0]))
+    m, n = torch.from_numpy(np.abs(a)), torch.from_numpy(np.abs(b))
+    cut = torch.zeros(len(a), len(b), dtype=torch.float64)
+    for k in range(0, a.shape[1], 8):
+        cut += (m[:, None, k:k + 8] * n[None, :, k:k + 8]).amax(-1)
     with np.errstate(invalid="ignore"):
-        for k in range(0, a.shape[1], 8):
-            cut += (m[:, None, k:k + 8] * n[None, :, k:k + 8]).max(-1)
-        return a @ b.T, m @ n.T, cut
+        return a @ b.T, (m @ n.T).numpy(), cut.numpy()
 
 
 def bound(y, mag, cut, K, eps):

@@ -134,6 +134,39 @@ def test_matmul_types(dev, M, kind, dtype):
     _check(got, x, q, s)
 
 
+def _check_some(got, x, q, s, rows, cols, what=""):
+    """The given rows, at ranges of columns that begin on a scale block."""
+    got, x, rows = to_numpy(got), to_numpy(x), list(rows)
+    for c0, c1 in cols:
+        _check(torch.from_numpy(got[rows, c0:c1]).to(BF), torch.from_numpy(x[rows]), q[c0:c1], s[c0 // 128:], what)
+
+
+@pytest.mark.parametrize("M,N,Kd", [(384, 14336, 144), (384, 14300, 8208), (900, 14332, 256), (1030, 14340, 400),
+                                    (769, 14336, 8320)])
+def test_matmul_of_many_tiles(dev, M, N, Kd):
+    """The large tiles, their last rows and columns in part, scales in more
+    than one chunk."""
+    kind = "e8m0" if M % 2 else "f32"
+    (q, s), (wq, sc) = _w(M, (N, Kd), kind, dev)
+    x = _x(N, (M, Kd), BF, dev)
+    got = K.quantized_matmul(x, wq, sc, mode="fp8")
+    at = N // 128 * 128 - 128
+    _check_some(got, x, q, s, [0, 63, 64, 255, 256, M - 1], [(0, 140), (at, N)])
+    assert torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, FH])
+@pytest.mark.parametrize("M,N,Kd", [(17, 66, 4096), (64, 127, 8208), (100, 200, 4112), (33, 4, 16384), (130, 130, 5120)])
+def test_matmul_in_parts_of_k(dev, dtype, M, N, Kd):
+    """Few tiles of a long K: sums of parts, the last of them shorter."""
+    kind = "e8m0" if M % 2 else "f32"
+    (q, s), (wq, sc) = _w(N, (N, Kd), kind, dev)
+    x = _x(M + 2, (M, Kd), dtype, dev, 0.25)
+    got = K.quantized_matmul(x, wq, sc, mode="fp8")
+    _check(got, x, q, s)
+    assert torch.equal(got, K.quantized_matmul(x, wq, sc, mode="fp8"))
+
+
 @pytest.mark.parametrize("M", [2, 40, 256])
 def test_matmul_row_scales_follow_each_row_and_block(dev, M):
     """Rows and blocks of very different size, zero rows, zero blocks."""
@@ -242,6 +275,26 @@ def test_gather_sizes(dev, P, E, M, N, Kd):
     _gather_check(got, x, range(P), rhs, q, s)
 
 
+@pytest.mark.parametrize("P,E,N,Kd", [(300, 64, 2048, 144), (700, 64, 2040, 1040), (4200, 64, 1280, 272), (300, 3, 700, 400),
+                                      (9, 9, 300, 8208), (40, 16, 260, 2304), (70, 2, 260, 16400)])
+def test_gather_in_groups(dev, P, E, N, Kd):
+    """Several column blocks to a workgroup, units of every size, K past the
+    stream's; experts without rows, rows of one expert only."""
+    kind = "e8m0" if P % 3 else "f32"
+    (q, s), (wq, sc) = _w(P + E, (E, N, Kd), kind, dev)
+    x = _x(P, (P, 1, Kd), BF, dev)
+    rng = np.random.default_rng(P)
+    for rhs in (rng.integers(0, E, P), np.full(P, E - 1), rng.integers(0, E, P) // 2 * 2):
+        got = K.gather_qmm(x, wq, sc, rhs_indices=torch.from_numpy(rhs).to(dev), mode="fp8")
+        at = N // 128 * 128 - 128
+        for p in (0, 1, P // 2, P - 1):
+            if rhs[p] < E:
+                _check_some(got[p], x[p], q[rhs[p]], s[rhs[p]], [0], [(0, N if N < 300 else 300), (at, N)], f"pair {p}")
+            else:
+                assert (got[p] == 0).all()
+        assert torch.isfinite(got).all()
+
+
 @pytest.mark.parametrize("dtype", [BF, FH])
 @pytest.mark.parametrize("P", [5, 150])
 def test_gather_types_and_lhs(dev, dtype, P):
@@ -319,7 +372,7 @@ def _experts(seed, E, H, I, kind, dev):
 
 
 @pytest.mark.parametrize("T,k,E", [(1, 1, 1), (1, 8, 16), (3, 2, 4), (16, 4, 8), (50, 2, 3), (200, 2, 3), (70, 10, 12)])
-@pytest.mark.parametrize("H,I", [(256, 128), (400, 384), (1040, 640), (4160, 256)])
+@pytest.mark.parametrize("H,I", [(256, 128), (400, 384), (528, 640), (2064, 256)])
 def test_switch_glu(dev, T, k, E, H, I):
     kind = "e8m0" if T % 2 == 0 else "f32"
     hg, hd, wg, wd = _experts(T + H, E, H, I, kind, dev)
