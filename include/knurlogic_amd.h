@@ -300,8 +300,10 @@ int kmi_dequantize_fp8(const uint32_t* wq, const void* scales, int e8m0, int64_t
  * block (power-of-two scales; a row with an infinity or a NaN gives NaN).
  * fp32 accumulation (the matrix instruction lines up each run of 8 products with
  * its largest and keeps 13 binary places below it), y rounded once to x's dtype
- * (bfloat16 or float16).  K % 16 == 0; x and w 16-byte aligned; scales [ceil(N/128), ceil(K/128)] float32 (any
- * values) or E8M0 bytes.  Each output row depends only on its own input row.
+ * (bfloat16 or float16).  K % 16 == 0 and at most 65536, M < 2^21; x and w
+ * 16-byte aligned; scales [ceil(N/128), ceil(K/128)] float32 (any values) or E8M0
+ * bytes.  Each output row depends only on its own input row; its last bits may
+ * differ with the number of rows beside it (K in parts for few tiles).
  * `workspace` (kmi_qmm_fp8_workspace_bytes) may be NULL when that is 0.
  */
 size_t kmi_qmm_fp8_workspace_bytes(int64_t M, int64_t K, int64_t N, int dtype);
@@ -310,7 +312,8 @@ int kmi_qmm_fp8(const void* x, int64_t M, int64_t K, int64_t N, const uint32_t* 
 
 /*
  * kmi_gather_qmm over such weights: y[p, m] = xhat[lhs[p], m] @ What[rhs[p]]^T,
- * x [X, M, K], w [E, N, K/4], scales [E, ceil(N/128), ceil(K/128)], E <= 4096.
+ * x [X, M, K], w [E, N, K/4], scales [E, ceil(N/128), ceil(K/128)], E <= 4096,
+ * K <= 65536; rows of more than 2 GiB of codes are refused.
  * Rows are grouped by expert on the GPU.  An index out of range gives a zero row.
  */
 size_t kmi_gather_qmm_fp8_workspace_bytes(int64_t P, int64_t X, int64_t M, int64_t E, int64_t K, int64_t N,
@@ -321,7 +324,7 @@ int kmi_gather_qmm_fp8(const void* x, int64_t X, int64_t M, int64_t K, const uin
 
 /*
  * kmi_switch_glu over such experts: w_gu [E, 2I, H/4] (gate rows, then up rows;
- * I % 128 == 0), w_down [E, H, I/4], H % 16 == 0, k <= 64.  The activations
+ * I % 128 == 0), w_down [E, H, I/4], H % 16 == 0, H and I <= 65536, k <= 64.  The activations
  * round(round(silu(gate)) * up) are quantized per row and 128 of I on their
  * way into the down product.  bf16.  out [T, k, H], or [T, H] with scores.
  */

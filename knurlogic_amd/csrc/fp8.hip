@@ -15,7 +15,8 @@ constexpr int64_t MAX_E = 4096;        // of the GPU sort
 
 int check_operands(const char* what, int dtype, int64_t K, int64_t N, const void* x, const void* w) {
     KMI_CHECK_ARG(dtype == BF16 || dtype == F16, "%s: dtype %d (bfloat16 or float16)", what, dtype);
-    KMI_CHECK_ARG(K > 0 && K % 16 == 0 && K < (1 << 24), "%s: K=%lld (a multiple of 16 below 2^24)", what, (long long)K);
+    KMI_CHECK_ARG(K > 0 && K % 16 == 0 && K <= FP8_GEMM_MAX_K, "%s: K=%lld (a multiple of 16 up to %lld)", what,
+                  (long long)K, (long long)FP8_GEMM_MAX_K);
     KMI_CHECK_ARG(N > 0 && N < (1LL << 31), "%s: N=%lld", what, (long long)N);
     KMI_CHECK_ARG((((uintptr_t)x | (uintptr_t)w) & 15) == 0, "%s: x and w on 16 bytes", what);
     return OK;

@@ -51,11 +51,11 @@ struct F8Args {
     unsigned char* ys;
     int64_t ys_ld;
     int half;                   // y is float16
-    float* partial;
+    float* partial;             // launch_fp8_gemm's parts of K
     int64_t part_ld;            // a multiple of 4, at least N
 };
 
-// tiles of up to a.tm (16 or 32; gate|up 16) rows; dtype BF16 or F16
+// f8_stream: tiles of up to 16 rows; dtype BF16 or F16 (gate|up: BF16)
 int64_t fp8_skinny_max_k(bool glu);
 int launch_fp8_skinny(const F8Args& a, int dtype, bool glu, int64_t tiles, hipStream_t st);
 
@@ -73,7 +73,7 @@ int64_t fp8_row_scales(int64_t K);             // (a multiple of 16)
 int launch_fp8_rows(const void* x, int dtype, int64_t rows, int64_t K, unsigned char* q, unsigned char* s,
                     hipStream_t st);
 constexpr int64_t FP8_GEMM_MAX_K = 65536;     // a tile's rows within 32-bit offsets
-// tiles of up to a.tm (64, 128 or 256) rows over such rows
+// tiles of up to a.tm (64, 128 or, dense, 256) rows over such rows;
 // parts > 1 (dense; fp8_gemm_parts): K in parts of fp8_part_blocks blocks, their
 // sums through a.partial [parts, rows, a.part_ld]
 int fp8_gemm_parts(int64_t M, int64_t K, int64_t N, int tm);

@@ -90,6 +90,8 @@ def test_c_entries_refuse_on_the_host():
         return L.kmi_qmm_fp8(*{**ok, **kw}.values())
     assert qmm(K=250) == -1 and b"multiple of 16" in L.kmi_last_error()
     assert qmm(K=0) == -1 and qmm(N=0) == -1 and qmm(dt=2) == -1 and qmm(M=-1) == -1
+    assert qmm(K=65552) == -1 and b"65536" in L.kmi_last_error() and qmm(M=1 << 21) == -1
+    assert qmm(M=64, K=65536) == -3 and qmm(M=17) == -3 and qmm(M=1, K=16400) == -3
     assert qmm(x=8) == -1 and b"16 bytes" in L.kmi_last_error()
     assert qmm(w=4) == -1 and qmm(y=None) == -1 and b"null" in L.kmi_last_error()
     assert qmm(M=0) == 0
@@ -98,6 +100,7 @@ def test_c_entries_refuse_on_the_host():
     def gather(**kw):
         return L.kmi_gather_qmm_fp8(*{**g, **kw}.values())
     assert gather(P=400) == -3 and b"workspace" in L.kmi_last_error()
+    assert gather(K=65552) == -1 and gather(X=1 << 20, K=4096, P=1 << 20) == -1 and b"2 GiB" in L.kmi_last_error()
     assert gather(E=5000) == -1 and gather(E=0) == -1 and gather(K=8) == -1 and gather(P=1 << 40) == -1
     assert gather(l=None) == -1 and gather(P=0) == 0
     assert L.kmi_gather_qmm_fp8_workspace_bytes(400, 4, 1, 4, 256, 64, 0) > 0
@@ -107,6 +110,7 @@ def test_c_entries_refuse_on_the_host():
     def glu(**kw):
         return L.kmi_switch_glu_fp8(*{**u, **kw}.values())
     assert glu() == -3 and glu(I=144) == -1 and b"blocks of 128" in L.kmi_last_error()
+    assert glu(H=65552) == -1 and glu(I=65664) == -1
     assert glu(H=250) == -1 and glu(k=0) == -1 and glu(k=65) == -1 and glu(dt=1) == -1 and glu(E=0) == -1
     assert glu(wd=None) == -1 and glu(T=0) == 0 and glu(T=1 << 30, k=64) == -1
     assert L.kmi_quantize_fp8(16, 0, 1, 4, 24, 16, 16, None) == -1

@@ -389,6 +389,20 @@ def test_switch_glu(dev, T, k, E, H, I):
     _glu_check(got, _glu_ref(to_numpy(x), inds, hg, hd, to_numpy(sc)))
 
 
+@pytest.mark.parametrize("T,k,E,H,I", [(1, 2, 4, 256, 4224), (3, 2, 3, 8208, 128), (40, 2, 3, 8208, 128), (40, 1, 2, 128, 8320),
+                                       (13, 4, 64, 144, 256), (90, 6, 65, 144, 1408)])
+def test_switch_glu_long_and_wide(dev, T, k, E, H, I):
+    """Scales in more than one chunk, both ways round; pairs past the combining
+    kernel's depth; columns in units of every size."""
+    hg, hd, wg, wd = _experts(T + I, E, H, I, "f32" if T % 2 else "e8m0", dev)
+    rng = np.random.default_rng(T)
+    inds = np.stack([rng.choice(E, k, replace=False) for _ in range(T)])
+    x = _x(T, (T, H), BF, dev)
+    sc = torch.softmax(_x(T + 1, (T, k), FS, dev), -1).to(BF)
+    got = K.switch_glu_fp8(x, torch.from_numpy(inds).to(dev), *wg, *wd, sc)
+    _glu_check(got, _glu_ref(to_numpy(x), inds, hg, hd, to_numpy(sc)))
+
+
 def test_switch_glu_out_of_range_and_repeated_experts(dev):
     hg, hd, wg, wd = _experts(3, 4, 256, 128, "f32", dev)
     inds = np.array([[0, 0, 4], [-1, 2, 2], [7, 9, -3], [3, 1, 0]])
