@@ -17,6 +17,11 @@
 // lane holds its row's 32 inputs of a half in registers, so the half's place is free
 // once they are read, a half ahead: two halves' loads are in flight beside the one
 // that has landed.
+//
+// 16384 rows of 128 experts, 2048 -> 768: 156-188 us (103 GFLOP: 0.66 PFLOP/s of the
+// 1.84 that these instructions reach on the whole chip).  Without the products
+// 143 us, without the loads 120, without either 104: data and products are of like
+// length and hide each other only in part.
 #include "fp8_tiles.hpp"
 
 namespace kmi {

@@ -1,5 +1,6 @@
 // E4M3 with one E8M0 scale per block of 128 x 128: weights into codes and
-// scales, and back.
+// scales, and back.  Bound by HBM: bf16 [14336, 4096] 34.4 us, 5.1 TB/s read and
+// written (a large copy: 4.8).
 #include "fp8.hpp"
 #include "../../include/knurlogic_amd.h"
 
