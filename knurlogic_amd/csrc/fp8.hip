@@ -41,7 +41,7 @@ struct Plan {
 
 //
 // Dense: the stream up to 16 rows ([4096, 4096] x 16 rows: 11 us, tiles 14.4;
-// [14336, 4096]: 20.8, 20.6), then the tiles with the least rounds x time of a
+// [14336, 4096]: 19.3, 20.6), then the tiles with the least rounds x time of a
 // round.  A block of 128 inputs takes 0.5 us in tiles of 64 rows where each is
 // alone on its CU, 0.8 two to a CU; 0.9 and 1.2 in tiles of 128; 1.5 in tiles of 256
 // x 256, one to a CU.  [4096, 4096], tiles of 64 / 128 / 256: 512 rows 23 / 35 / 59

@@ -323,8 +323,8 @@ int go(const F8Args& a, int64_t tiles, int parts, hipStream_t st) {
     // Column blocks per workgroup.  A workgroup's start (its tile, its rows, their
     // first inputs) takes as long as some ten blocks of K, so a short K takes
     // several column blocks, their weights streaming on, while the grid keeps twice
-    // what runs at once (16384 rows of 128 experts [2048, 768]: 4 blocks 84 us, 1
-    // 105); so does any K where most of a tile is empty, and the weights' stream is
+    // what runs at once (the expert block of 2048 tokens, down [2048, 768]: 2 or 4 blocks
+    // 271 us, 1 278, 8 285); so does any K where most of a tile is empty, and the weights' stream is
     // all there is, while two workgroups come to a CU (512 rows of 64 experts
     // [2048, 2048]: 2 blocks 61.9 us, 1 65.7, 4 78.0; 4096 rows: 88.2, 89.1, 101.8).
     const int64_t KB = ceil_div(a.K, F8_BLOCK);

@@ -11,7 +11,7 @@
 // before, no partial sums in memory.  gate|up takes a block of gate rows and the
 // up rows beside it, in float16 operands (its results are rounded to E4M3 again).
 //
-// Bound by HBM where the weights are large (16 rows of [14336, 4096] 19.5 us, 3.0
+// Bound by HBM where the weights are large (16 rows of [14336, 4096] 16.6 us, 3.6
 // TB/s: each wave quantizes its part of x before its first product), by the launch
 // and one chain of latencies where they are not (1 row of [4096, 4096] 7 us).
 #include "fp8.hpp"
@@ -47,10 +47,17 @@ __device__ __forceinline__ f32x4 st_times(const i32x8& w, const i32x8& x) {
     }
 }
 
-// R row blocks per wave and step; KPW blocks of K per wave at most
-// and W waves (GLU: 3 workgroups of 4 on a CU, or one of 8; else 2 or 1 of 8)
+// workgroups of W waves that run at once on a CU: 3 of 4 waves (GLU), else 2 of 8,
+// or 1 where K has 8 parts, with twice the registers (16 rows [8192, 4096]: 14.7 us, 18.1
+// with 2; [14336, 4096]: 19.3, 20.7)
+template <int KP, int W>
+constexpr int st_at_once = W == 4 ? 3 : KP == 8 ? 1 : 2;
+
+// R row blocks per wave and step; KPW blocks of K per wave at most.
+// The weights' loads are ordinary ones: non-temporal, [28672, 4096] x 1 row took 28.8 us
+// for 26.0, 8 pairs of 64 experts [2048, 2048] 13.0 for 11.6 ([4096, 4096] x 1 row: 7.3 for 7.7).
 template <class T, int KP, int KPW, int R, bool GLU, int W>
-__global__ __launch_bounds__(64 * W, W == 4 ? 3 : GLU || KPW >= 8 ? 2 : 4) void f8_stream(F8Args a, int steps) {
+__global__ __launch_bounds__(64 * W, (st_at_once<KP, W> * W / 4)) void f8_stream(F8Args a, int steps) {
     constexpr int RB = GLU ? 2 : 1, NP = W / KP, F = R * RB * KPW;
     // weight blocks (2 KB) in flight per wave: 8, or 4 where x, or gate|up's float16
     // operands, take the registers
@@ -113,9 +120,9 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : GLU || KPW >= 8 ? 2 : 4) void 
         asm volatile("" : "+s"(in));
         const uint32_t off = (uint32_t)l16 * (uint32_t)K + 16u * c;
         const u32x4 lo = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-            rs, (int)(16 * c < in ? off : ST_NONE), kb * F8_BLOCK, AUX_NT));
+            rs, (int)(16 * c < in ? off : ST_NONE), kb * F8_BLOCK, 0));
         const u32x4 hi = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-            rs, (int)(64 + 16 * c < in ? off : ST_NONE), kb * F8_BLOCK + 64, AUX_NT));
+            rs, (int)(64 + 16 * c < in ? off : ST_NONE), kb * F8_BLOCK + 64, 0));
         wr[q % D] = f8_operand(lo, hi);
     };
     int step = (int)blockIdx.x;
@@ -289,9 +296,9 @@ __global__ __launch_bounds__(64 * ST_WAVES) void f8_combine(F8Args a, const uint
                 const int in = K - kb * F8_BLOCK;
                 w[d] = f8_operand(
                     __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                        rs, (int)(16 * c < in ? off : ST_NONE), kb * F8_BLOCK, AUX_NT)),
+                        rs, (int)(16 * c < in ? off : ST_NONE), kb * F8_BLOCK, 0)),
                     __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                        rs, (int)(64 + 16 * c < in ? off : ST_NONE), kb * F8_BLOCK + 64, AUX_NT)));
+                        rs, (int)(64 + 16 * c < in ? off : ST_NONE), kb * F8_BLOCK + 64, 0)));
             };
 #pragma unroll
             for (int d = 0; d < CB_DEPTH; d++) load(d, d);
@@ -340,9 +347,6 @@ __global__ __launch_bounds__(64 * ST_WAVES) void f8_combine(F8Args a, const uint
     }
 }
 
-// workgroups of 8 waves that stream at once: two on each CU
-constexpr int64_t ST_GRID = 512;
-
 template <class T, int KP, int KPW, int R, bool GLU, int W = ST_WAVES>
 int go(const F8Args& a, int64_t tiles, hipStream_t st) {
     const int64_t steps = ceil_div(a.N, 16 * R * (W / KP));
@@ -354,7 +358,7 @@ int go(const F8Args& a, int64_t tiles, hipStream_t st) {
     // (16 more than that are a second round: 24 pairs [2048, 4096], 528 workgroups
     // 52.1 us, 456 43.1); of sorted tiles some are empty, and a few more run
     // (512 rows of 128 experts [1536, 4096]: 148 us, 181 with the first rule)
-    constexpr int64_t most = W == 4 ? 3 * ST_GRID / 2 : ST_GRID;
+    constexpr int64_t most = 256 * st_at_once<KP, W>;
     int64_t per = ceil_div(steps, tiles < most ? most / tiles : 1);
     if (a.tiles) per = ceil_div(steps * tiles, most) < steps ? ceil_div(steps * tiles, most) : steps;
     const int64_t gx = ceil_div(steps, per);
