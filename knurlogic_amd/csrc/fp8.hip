@@ -59,16 +59,16 @@ Plan plan_dense(int64_t M, int64_t K, int64_t N) {
 }
 
 // Grouped.  Pair by pair (no sort, no tile list; an expert's weights once per pair)
-// while few pairs share an expert: 64 experts [2048, 2048], 16 pairs 17.8 us,
-// streamed by the sorted list 25.5, tiles 22.1; 32: 28.2, 38.6, 32.3; 48: 43.0, 46.6,
-// 34.6; 8 experts [4096, 4096], 8 pairs 28.2, 37.1, 43.5, 12: 45.0, 39.0, 42.3.
-// Then the stream while the tiles would be few (8 experts [2048, 2048], 64 rows:
-// 18.0, tiles 24.6; [4096, 4096]: 64 rows 45.3, 45.2, 96 rows 52.5, 45.1; but 64
-// experts [2048, 2048], 128 rows: 56.6, 52.6), or an expert's few rows are long
-// (128 experts [1536, 4096], 256 rows: 142, 151, 512 rows: 148, 173; 128: 136, 131,
-// 768: 186, 174).  Tiles of 64 rows (gate|up's only size) up to 64 rows to an
-// expert, then 128: 64 experts [2048, 2048], 96 rows each: 97 us, in tiles of 64 104;
-// 8 experts [4096, 4096], 64 rows each: 54 both.
+// while few pairs share an expert: 64 experts [2048, 2048], 16 pairs 15.7 us,
+// streamed by the sorted list 24.5, tiles 22.5; 32: 25.3, 34.6, 31.7; 64: 42.5,
+// 50.5, 47.0; 96: 61.5, 51.1, 48.6; 8 experts [4096, 4096], 8 pairs 22.1, 29.7, 35.1,
+// 12: 35.7, 33.4, 43.6.  Then the stream while the tiles would be few (8 experts
+// [4096, 4096], 64 rows: 42.8, tiles 45.5, 128 rows 51.3, 48.8; but 64 experts
+// [2048, 2048], 256 rows: 61.9, 58.8), or an expert's few rows are long (128 experts
+// [1536, 4096], 256 rows: 126, 156, 512 rows: 148, 184; 768: 186, 174; 256 experts
+// [2048, 4096], 256 rows, one each: 287, 253).  Tiles of 64 rows (gate|up's only
+// size) up to 64 rows to an expert, then 128: 64 experts [2048, 2048], 96 rows each:
+// 97 us, in tiles of 64 104; 8 experts [4096, 4096], 64 rows each: 54 both.
 Plan plan_grouped(int64_t rows, int64_t P, int64_t E, int64_t K, int64_t N, bool glu) {
     const int64_t experts = P < E ? P : E, per = ceil_div(rows, experts);
     if (K <= fp8_skinny_max_k(glu)) {
