@@ -97,6 +97,16 @@ __device__ __forceinline__ uint32_t f8_scale_byte(uint32_t amax_bits) {
     return amax_bits >= 0x7f800000u ? 255u : (uint32_t)(e < 1 ? 1 : e);
 }
 
+// A weights' scale (any float32) as m * 2^(byte - 127), m in [1, 2) in magnitude
+// (a subnormal scale's is smaller, an infinite or NaN one's is itself).  The power
+// joins the block's sum before m does: the two scales' own product may leave
+// float32's range where the result does not.
+__device__ __forceinline__ void f8_split(float s, uint32_t& byte, float& m) {
+    const uint32_t e = __float_as_uint(s) >> 23 & 0xffu;
+    byte = e == 0 ? 1u : e == 255 ? 127u : e;
+    m = __builtin_amdgcn_ldexpf(s, 127 - (int)byte);
+}
+
 __device__ __forceinline__ f32x4 f8_mfma(i32x8 a, i32x8 b, f32x4 c, uint32_t sa, uint32_t sb) {
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, (int)sa, 0, (int)sb);
 }

@@ -25,8 +25,8 @@ namespace kmi {
 
 namespace {
 
-// how the scales meet the sums: both applied to each block's in float32 (weights'
-// scales in float32), or by the instruction (E8M0)
+// how the scales meet the sums: powers of two by the instruction, and float32
+// scales' mantissas after it, in float32, block by block
 enum Kind { F32S, E8S };
 
 // NW x WM waves: 64 weight rows x MB 16-row blocks of activations each
@@ -80,7 +80,8 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
     // (several column blocks: KB nl <= 64, all of theirs)
     const int64_t first = (int64_t)nb * nl * TN;              // the first column
     const int64_t SB = (a.wrows + F8_BLOCK - 1) / F8_BLOCK;
-    uint32_t swl;
+    uint32_t swl;                                // the scale's byte
+    float sml = 1.f;                             // and its mantissa (F32S)
     auto load_scales = [&](int t) {
         int kb = t + lane, b = 0;
         if (MANY) {
@@ -90,8 +91,8 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
         const int64_t n = first + (int64_t)b * TN + 64 * wn;
         const int64_t i = (T.expert * SB + (n < a.N ? n : first) / F8_BLOCK) * KBs + kb0 + (kb < KB ? kb : KB - 1);
         if (KIND == E8S) swl = ((const unsigned char*)a.s)[i];
-        else swl = ((const uint32_t*)a.s)[i];
-        asm volatile("" : "+v"(swl));            // waited for here, not in the loop
+        else f8_split(((const float*)a.s)[i], swl, sml);
+        asm volatile("" : "+v"(swl), "+v"(sml));              // waited for here, not in the loop
     };
     int64_t xr[XL];                                           // (beside the scales' latency)
     g_xrows(a, T, 8 * wave + (lane >> 3), 8 * WAVES, xr);
@@ -180,6 +181,7 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
 #pragma unroll
         for (int j = 0; j < MB; j++) sx[j] = g_scale(sc, TM, 16 * (MB * wm + j) + l16, t);
         const uint32_t sw = (uint32_t)__builtin_amdgcn_readlane((int)swl, (cb * KB + t) % G_CHUNK);
+        const float sm = __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(sml), (cb * KB + t) % G_CHUNK));
         // after the block's last LDS read: the next block has landed, and this
         // one's place is free
         auto turn = [&]() {
@@ -188,14 +190,13 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
             issue(at);
         };
         {
-            // product n = 4 j + i; its sums are scaled two products later
+            // product n = 4 j + i; its sums meet the mantissa two products later
             constexpr int NP = RB * MB;
             f32x4 p[3];
-            float f[2];
             auto apply = [&](int n) {
                 const int i = n % RB, j = n / RB;
 #pragma unroll
-                for (int q = 0; q < 4; q++) acc[i][j][q] = __builtin_fmaf(p[n % 3][q], f[j & 1], acc[i][j][q]);
+                for (int q = 0; q < 4; q++) acc[i][j][q] = __builtin_fmaf(p[n % 3][q], sm, acc[i][j][q]);
             };
 #pragma unroll
             for (int n = 0; n < NP; n++) {
@@ -208,8 +209,7 @@ __global__ __launch_bounds__(64 * NW * WM, 2) void f8_gemm(F8Args a, int nblocks
                 if constexpr (KIND == E8S) {
                     acc[i][j] = f8_mfma(w[i], b[j & 1], acc[i][j], sw, sx[j]);
                 } else {
-                    if (i == 0) f[j & 1] = __uint_as_float(sx[j] << 23) * __uint_as_float(sw);
-                    p[n % 3] = f8_mfma(w[i], b[j & 1], f32x4{0.f, 0.f, 0.f, 0.f}, 127u, 127u);
+                    p[n % 3] = f8_mfma(w[i], b[j & 1], f32x4{0.f, 0.f, 0.f, 0.f}, sw, sx[j]);
                     if (n >= 2) apply(n - 2);
                 }
                 if (j == MB - 1) read_w(nx, i);

@@ -7,8 +7,8 @@
 // instructions drop too much of small products for that (fp8.hpp).  So the codes
 // are multiplied in bfloat16, which holds them exactly: the weights' turned on their
 // way from LDS to v_mfma_f32_32x32x16_bf16, x's values (codes times the row's scale, a
-// power of two) by the pass before; a block's sums meet the weights' scale in
-// float32.
+// power of two) by the pass before.  The weights' scale joins its codes as a power of
+// two (exact), and its mantissa the block's sums, in float32.
 //
 // 4 waves: 32 gate and 32 up rows x the tile's one or two blocks of 32 rows each.
 // A workgroup starts with a chain of latencies (its tile, its rows, their first
@@ -53,7 +53,7 @@ __global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks,
     // the weights' scales, 64 blocks, one per lane (gate, up)
     const int64_t SB = (a.wrows + F8_BLOCK - 1) / F8_BLOCK;
     const int64_t sbase = (T.expert * SB + nb) * KB;
-    float swl[2];
+    float swl[2], spl[2];                                     // the scale is swl * spl, spl a power of two
     auto load_scales = [&](int t) {
         const int64_t i = sbase + (t + lane < KB ? t + lane : KB - 1), up = a.N / F8_BLOCK * KB;
         uint32_t v[2];
@@ -66,7 +66,15 @@ __global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks,
         }
         asm volatile("" : "+v"(v[0]), "+v"(v[1]));            // waited for here, not in the loop
 #pragma unroll
-        for (int g = 0; g < 2; g++) swl[g] = a.e8 ? e8m0_to_f32(v[g]) : __uint_as_float(v[g]);
+        for (int g = 0; g < 2; g++) {
+            uint32_t e;
+            f8_split(a.e8 ? e8m0_to_f32(v[g]) : __uint_as_float(v[g]), e, swl[g]);
+            // no further than bfloat16 holds a code's multiple; past that, none of
+            // the rest leaves float32's range that the result does not
+            const uint32_t in = e < 63 ? 63 : e > 191 ? 191 : e;
+            swl[g] = __builtin_amdgcn_ldexpf(swl[g], (int)e - (int)in);
+            spl[g] = __uint_as_float(in << 23);
+        }
     };
     int64_t xr[U_XL];                                         // (beside the scales' latency)
     g_xrows(a, T, 8 * wave + (lane >> 3), 8 * U_WAVES, xr);
@@ -145,6 +153,10 @@ __global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks,
             const int t1 = t0 + G_CHUNK < KB ? t0 + G_CHUNK : KB;
             for (int t = t0; t < t1; t++) {
                 f32x16 p[2][NJ];
+                float sp[2];
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+                    sp[i] = __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(spl[i]), t % G_CHUNK));
 #pragma unroll
                 for (int i = 0; i < 2; i++)
 #pragma unroll
@@ -162,7 +174,7 @@ __global__ __launch_bounds__(64 * U_WAVES, 2) void f8_glu(F8Args a, int nblocks,
                     for (int s = 0; s < 4; s++) {
                         bf16x8 wv[2];
 #pragma unroll
-                        for (int i = 0; i < 2; i++) wv[i] = f8_values(w[i][s / 2][s % 2 * 2], w[i][s / 2][s % 2 * 2 + 1], 1.f);
+                        for (int i = 0; i < 2; i++) wv[i] = f8_values(w[i][s / 2][s % 2 * 2], w[i][s / 2][s % 2 * 2 + 1], sp[i]);
 #pragma unroll
                         for (int i = 0; i < 2; i++)
 #pragma unroll

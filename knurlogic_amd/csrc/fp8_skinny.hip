@@ -34,16 +34,19 @@ __device__ __forceinline__ f16x8 st_halves(const i32x8& v, int q) {      // code
     return f16x8{p0.x, p0.y, p1.x, p1.y, p2.x, p2.y, p3.x, p3.y};
 }
 
-// the 16 x 16 products' sums of one block
+// the 16 x 16 products' sums of one block, times 2^(sw - 127) 2^(sx - 127)
 template <bool HALF>
-__device__ __forceinline__ f32x4 st_times(const i32x8& w, const i32x8& x) {
+__device__ __forceinline__ f32x4 st_times(const i32x8& w, const i32x8& x, uint32_t sw, uint32_t sx) {
     f32x4 p = {0.f, 0.f, 0.f, 0.f};
     if constexpr (HALF) {
 #pragma unroll
         for (int q = 0; q < 4; q++) p = __builtin_amdgcn_mfma_f32_16x16x32_f16(st_halves(w, q), st_halves(x, q), p, 0, 0, 0);
+        const int e = (int)(sw + sx) - 254;
+#pragma unroll
+        for (int i = 0; i < 4; i++) p[i] = __builtin_amdgcn_ldexpf(p[i], e);
         return p;
     } else {
-        return f8_mfma(w, x, p, 127u, 127u);
+        return f8_mfma(w, x, p, sw, sx);
     }
 }
 
@@ -150,7 +153,7 @@ __global__ __launch_bounds__(64 * W, (st_at_once<KP, W> * W / 4)) void f8_stream
     // x blocks of this part: 16 lanes quantize 128 inputs of a row, BATCH blocks of
     // a row at once, through LDS (pieces permuted by the row) into the operand
     i32x8 x[KPW];
-    float xf[KPW];
+    uint32_t xb[KPW];                                        // the blocks' scale bytes
 #pragma unroll
     for (int b0 = 0; b0 < KPW; b0 += BATCH) {
         const int kb = kp + KP * (b0 + c), k = kb * F8_BLOCK + 8 * l16;
@@ -158,7 +161,7 @@ __global__ __launch_bounds__(64 * W, (st_at_once<KP, W> * W / 4)) void f8_stream
 #pragma unroll
             for (int i = b0; i < b0 + BATCH; i++) {
                 x[i] = i32x8{0, 0, 0, 0, 0, 0, 0, 0};
-                xf[i] = 0.f;
+                xb[i] = 127;
             }
             continue;
         }
@@ -198,7 +201,7 @@ __global__ __launch_bounds__(64 * W, (st_at_once<KP, W> * W / 4)) void f8_stream
 #pragma unroll
             for (int q = 0; q < 8; q++) v[q] = on ? v[q] : 0;
             x[b0 + i] = v;
-            xf[b0 + i] = on ? __uint_as_float((uint32_t)xe[wave][i * 16 + m] << 23) : 0.f;
+            xb[b0 + i] = on ? xe[wave][i * 16 + m] : 127;
         }
     }
 
@@ -207,9 +210,10 @@ __global__ __launch_bounds__(64 * W, (st_at_once<KP, W> * W / 4)) void f8_stream
         // (opaque: float16 operands are made where they are used, not kept)
 #pragma unroll
         for (int i = 0; i < KPW; i++) asm volatile("" : "+v"(x[i]));
+        uint32_t se[RB];                                     // the step's scales: bytes and mantissas
         float s[RB];
 #pragma unroll
-        for (int g = 0; g < RB; g++) s[g] = a.e8 ? e8m0_to_f32(sv[g]) : __uint_as_float(sv[g]);
+        for (int g = 0; g < RB; g++) f8_split(a.e8 ? e8m0_to_f32(sv[g]) : __uint_as_float(sv[g]), se[g], s[g]);
         load_scales(next);
         f32x4 acc[R][RB];
 #pragma unroll
@@ -219,11 +223,10 @@ __global__ __launch_bounds__(64 * W, (st_at_once<KP, W> * W / 4)) void f8_stream
 #pragma unroll
         for (int q = 0; q < F; q++) {
             const int g = q % RB, i = q / RB % KPW, r = q / RB / KPW;
-            const float sw = __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(s[g]), i));
-            // codes' products first, then both scales at once: no step leaves
-            // float32's range that the result does not
-            const f32x4 p = st_times<GLU>(wr[q % D], x[i]);
-            const float f = kp + KP * i < KB ? sw * xf[i] : 0.f;
+            const float sm = __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(s[g]), i));
+            const uint32_t sw = (uint32_t)__builtin_amdgcn_readlane((int)se[g], i);
+            const f32x4 p = st_times<GLU>(wr[q % D], x[i], sw, xb[i]);
+            const float f = kp + KP * i < KB ? sm : 0.f;
 #pragma unroll
             for (int e = 0; e < 4; e++) acc[r][g][e] = __builtin_fmaf(p[e], f, acc[r][g][e]);
             load((q + D) % F, q + D < F ? step : next);
@@ -290,7 +293,9 @@ __global__ __launch_bounds__(64 * ST_WAVES) void f8_combine(F8Args a, const uint
             const __amdgpu_buffer_rsrc_t rs = make_rsrc(a.w + (expert * a.wrows + n0) * a.K, left * a.K);
             const uint32_t off = (uint32_t)l16 * (uint32_t)K + 16u * c;
             const int64_t si = (expert * SB + n0 / F8_BLOCK) * KB + (lane < KB ? lane : 0);
-            const float sw = a.e8 ? e8m0_to_f32(((const unsigned char*)a.s)[si]) : ((const float*)a.s)[si];
+            uint32_t sw;
+            float sm;
+            f8_split(a.e8 ? e8m0_to_f32(((const unsigned char*)a.s)[si]) : ((const float*)a.s)[si], sw, sm);
             i32x8 w[CB_DEPTH];
             auto load = [&](int kb, int d) {
                 const int in = K - kb * F8_BLOCK;
@@ -324,9 +329,9 @@ __global__ __launch_bounds__(64 * ST_WAVES) void f8_combine(F8Args a, const uint
                     // every column the same row: column 0 is used
                     const i32x8 x = f8_operand(*(const u32x4*)(xs[wave] + at * F8_BLOCK + 16 * c),
                                                *(const u32x4*)(xs[wave] + at * F8_BLOCK + 64 + 16 * c));
-                    const f32x4 p = f8_mfma(w[d], x, f32x4{0.f, 0.f, 0.f, 0.f}, 127u, 127u);
-                    const float s = __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(sw), at)) *
-                                    __uint_as_float((uint32_t)xe[wave][at] << 23);
+                    const f32x4 p = f8_mfma(w[d], x, f32x4{0.f, 0.f, 0.f, 0.f},
+                                            (uint32_t)__builtin_amdgcn_readlane((int)sw, at), xe[wave][at]);
+                    const float s = __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(sm), at));
                     const float f = kb < KB ? s : 0.f;
 #pragma unroll
                     for (int e = 0; e < 4; e++) acc[e] = __builtin_fmaf(kb < KB ? p[e] : 0.f, f, acc[e]);
