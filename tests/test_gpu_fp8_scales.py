@@ -162,3 +162,93 @@ def test_block_scales_against_large_and_small_rows(dev, T, E, by):
     want = _block(dev, x, inds, None, g, sg, d, sd)
     got = _block(dev, (x.float() * 2.0 ** by).to(BF), inds, None, g, np.ldexp(sg, -by).astype(np.float32), d, sd)
     assert torch.isfinite(want).all() and torch.equal(got, want)
+
+
+# --- E8M0 bytes at their ends, and NaN ----------------------------------------------
+
+def _bytes(seed, shape):
+    return np.random.default_rng(seed).integers(112, 120, shape).astype(np.uint8)
+
+
+@pytest.mark.parametrize("M,N", DENSE)
+@pytest.mark.parametrize("lo", [1, 30, 200])
+def test_matmul_of_far_bytes(dev, M, N, lo):
+    """One block's byte away from the others', as far as x stays in its type."""
+    q = _codes(12, (N, 272))
+    s = np.full((-(-N // 128), 3), lo, np.uint8)
+    s[0, 1], s[-1, 2] = lo + 3, max(lo - 3, 0)
+    x = _rows(13, (M, 272), dev, std=2.0 ** (119 - lo))
+    got = K.quantized_matmul(x, _up(q, dev).view(torch.uint32), _up(s, dev), mode="fp8")
+    rows, cols = [0, 1, M // 2, M - 1], np.r_[0:20, N - 20:N]
+    sel = torch.from_numpy(cols).to(dev)
+    y, mag, cut = R.product(to_numpy(x[rows]), q, s)
+    d = np.abs(to_numpy(got[rows][:, sel]).astype(np.float64) - y[:, cols])
+    assert (d <= R.bound(y, mag, cut, 272, torch.finfo(BF).eps)[:, cols]).all() and torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("M,N,Kd", [(*d, 512) for d in DENSE] + [(40, 200, 4096)])
+def test_matmul_nan_byte(dev, M, N, Kd):
+    """A byte of 255 makes its own 128 rows of weights NaN and no others,
+    zeros in x or not; one that kmi_quantize_fp8 wrote, too."""
+    w = _rows(14, (N, Kd), dev, std=0.02)
+    clean = K.quantize(w, mode="fp8")
+    w[130, Kd - 1] = float("inf")
+    bad = K.quantize(w, mode="fp8")
+    assert int(bad[1][1, -1]) == 255
+    x = _rows(15, (M, Kd), dev)
+    x[M // 2, -128:] = 0
+    a, b = (K.quantized_matmul(x, *t, mode="fp8") for t in (clean, bad))
+    hit = slice(128, min(256, N))
+    assert b[:, hit].isnan().all() and torch.isfinite(a).all()
+    assert torch.equal(a[:, :128], b[:, :128]) and torch.equal(a[:, 256:], b[:, 256:])
+
+
+@pytest.mark.parametrize("P,E", GROUPED)
+def test_gather_far_and_nan_bytes(dev, P, E):
+    q, s = _codes(16, (E, 200, 272)), _bytes(17, (E, 2, 3))
+    for lo in (1, 200):
+        s[0] = lo
+        s[1, :, 1] = 117
+        x = _rows(18, (P, 1, 272), dev)
+        rhs = torch.arange(P, device=dev) % E
+        x[rhs == 0] *= 2.0 ** (119 - lo)
+        got = K.gather_qmm(x, _up(q, dev).view(torch.uint32), _up(s, dev), rhs_indices=rhs, mode="fp8")
+        for p in (0, 1, P - 2, P - 1):
+            e = p % E
+            y, mag, cut = R.product(to_numpy(x[p]), q[e], s[e])
+            d = np.abs(to_numpy(got[p]).astype(np.float64) - y)
+            assert (d <= R.bound(y, mag, cut, 272, torch.finfo(BF).eps)).all()
+        s[1, 1, 1] = 255
+        bad = K.gather_qmm(x, _up(q, dev).view(torch.uint32), _up(s, dev), rhs_indices=rhs, mode="fp8")
+        of = rhs == 1
+        assert bad[of][:, 0, 128:].isnan().all() and torch.equal(bad[of][:, 0, :128], got[of][:, 0, :128])
+        assert torch.equal(bad[~of], got[~of])
+
+
+@pytest.mark.parametrize("T,E", BLOCK)
+@pytest.mark.parametrize("with_scores", [True, False])
+def test_block_far_and_nan_bytes(dev, T, E, with_scores):
+    """Bytes 100 lower against x 2^100 times as large; then 255 in one expert's
+    gate, and in one block of its down rows."""
+    H, I, k = 512, 256, 2
+    g, d = _codes(19, (E, 2 * I, H)), _codes(20, (E, H, I))
+    sg, sd = _bytes(21, (E, 2 * I // 128, H // 128)), _bytes(22, (E, H // 128, I // 128)) - 5
+    x = _rows(23, (T, H), dev)
+    inds = torch.stack([torch.randperm(E, generator=torch.Generator().manual_seed(t))[:k] for t in range(T)]).to(dev)
+    scores = torch.full((T, k), 0.5, dtype=BF, device=dev) if with_scores else None
+    want = _block(dev, x, inds, scores, g, sg, d, sd)
+    assert torch.isfinite(want).all()
+    assert torch.equal(_block(dev, (x.float() * 2.0 ** 100).to(BF), inds, scores, g, sg - 100, d, sd), want)
+    e = int(inds[0, 0])
+    of = (inds == e).any(-1) if with_scores else inds == e
+    for at in ("gate", "down"):
+        a, b = sg.copy(), sd.copy()
+        if at == "gate":
+            a[e, 1, 2] = 255
+        else:
+            b[e, 2, 1] = 255
+        got = _block(dev, x, inds, scores, g, a, d, b)
+        cols = slice(0, H) if at == "gate" else slice(256, 384)
+        assert got[of][:, cols].isnan().all() and torch.equal(got[~of], want[~of])
+        if at == "down":
+            assert torch.equal(got[of][:, :256], want[of][:, :256]) and torch.equal(got[of][:, 384:], want[of][:, 384:])
