@@ -216,7 +216,8 @@ def build(weights: dict, path: str, in_dims: int | None = None, quant: dict | No
         w = weights[f"{path}.weight"].contiguous().view(torch.uint8).view(torch.uint32).to(device)
         s = weights[f"{path}.weight_scale_inv"].to(device=device, dtype=torch.float32)
         bias = weights.get(f"{path}.bias")
-        bias = bias.to(device) if bias is not None else None
+        if bias is not None:                               # one of the products' two types
+            bias = bias.to(device=device, dtype=torch.float16 if bias.dtype == torch.float16 else torch.bfloat16)
         cls = QuantizedLinear if w.dim() == 2 else QuantizedSwitchLinear
         return cls(w, s, None, bias, **fp8)
     vq = vq_recipe(weights, path, in_dims=in_dims)

@@ -56,6 +56,11 @@ def _input_dims(layer):
     return layer.scales.shape[-1] * layer.group_size
 
 
+def _bias(layer, y):
+    # fp8 products come in x's type, either 16-bit one, whatever the checkpoint's
+    return layer.bias.to(y.dtype) if layer.mode == "fp8" else layer.bias
+
+
 class QuantizedLinear:
     """nn.QuantizedLinear: y = quantized_matmul(x, w, scales, biases) (+ bias)."""
 
@@ -80,7 +85,7 @@ class QuantizedLinear:
     def __call__(self, x):
         y = quantized_matmul(x, self.weight, self.scales, self.biases, transpose=True,
                              group_size=self.group_size, bits=self.bits, mode=self.mode)
-        return add_bias(y, self.bias) if self.bias is not None else y
+        return add_bias(y, _bias(self, y)) if self.bias is not None else y
 
 
 class QuantizedSwitchLinear:
@@ -115,7 +120,7 @@ class QuantizedSwitchLinear:
                        transpose=True, group_size=self.group_size, bits=self.bits,
                        mode=self.mode, sorted_indices=sorted_indices)
         if self.bias is not None:
-            y = add_bias(y, self.bias, indices)
+            y = add_bias(y, _bias(self, y), indices)
         return y
 
 
