@@ -204,14 +204,30 @@ def fp8_recipe(weights: dict, path: str) -> dict | None:
     return {"group_size": 128, "bits": 8, "mode": "fp8"}
 
 
+def _fp8_layers(weights: dict) -> set:
+    """The paths ``fp8_recipe`` takes (other forms of float8 are not packed
+    layers of this package)."""
+    out = set()
+    for k in weights:
+        if k.endswith(".weight_scale_inv"):
+            path = k.rsplit(".", 1)[0]
+            try:
+                fp8_recipe(weights, path)
+            except ValueError:
+                continue
+            out.add(path)
+    return out
+
+
 def build(weights: dict, path: str, in_dims: int | None = None, quant: dict | None = None,
           device="cuda", prefix: str = ""):
     """This package's module for the packed (or VQ) layer ``path``: a
     QuantizedLinear (2-D weight), QuantizedSwitchLinear (3-D) or
     VQSwitchLinear; None when ``path`` is stored unpacked.  A float8 weight
-    with block scales (``fp8_recipe``) becomes a layer of mode fp8, its scales
-    in float32."""
-    fp8 = fp8_recipe(weights, path)
+    with block scales (``fp8_recipe``, which refuses other forms) becomes a
+    layer of mode fp8, its scales in float32."""
+    packed = any(f"{path}.{n}" in weights for n in ("scales", "codes", "vq_scales"))
+    fp8 = None if packed else fp8_recipe(weights, path)
     if fp8 is not None:
         w = weights[f"{path}.weight"].contiguous().view(torch.uint8).view(torch.uint32).to(device)
         s = weights[f"{path}.weight_scale_inv"].to(device=device, dtype=torch.float32)
@@ -266,7 +282,8 @@ def build(weights: dict, path: str, in_dims: int | None = None, quant: dict | No
 def load_quantized(model_path=None, files=None, shapes: dict | None = None, device="cuda") -> dict:
     """Every packed, VQ or block-scaled float8 layer of an mlx-format artifact (``model*.safetensors``
     and config.json under ``model_path``, or explicit ``files``) as this
-    package's modules, {path: module}.  ``shapes`` maps a layer path to its
+    package's modules, {path: module} (float8 in other forms than blocks of
+    128 x 128 is left out, as unpacked layers are).  ``shapes`` maps a layer path to its
     dense weight shape (the module skeleton's), else input sizes come from
     the config's quantization block.  VQ layers described in a file's
     ``vq_modules`` metadata are checked against it."""
@@ -277,8 +294,8 @@ def load_quantized(model_path=None, files=None, shapes: dict | None = None, devi
     weights, meta = read_safetensors(files)
     quant = artifact_quantization(model_path) if model_path is not None else {}
     declared = json.loads(meta["vq_modules"]) if "vq_modules" in meta else {}
-    paths = sorted({k.rsplit(".", 1)[0] for k in weights
-                    if k.endswith((".scales", ".codes", ".vq_scales", ".weight_scale_inv"))})
+    paths = sorted({k.rsplit(".", 1)[0] for k in weights if k.endswith((".scales", ".codes", ".vq_scales"))}
+                   | _fp8_layers(weights))
     out = {}
     for p in paths:
         in_dims = None

@@ -55,3 +55,32 @@ def test_a_layer_with_a_bias_runs(dev, lead, bias, x):
         return
     y = m(torch.ones(4, 1, 144, dtype=x, device=dev), torch.tensor([0, 1, 2, 1], device=dev))
     assert y.dtype == x and y[:, 0, 0].tolist() == [1.25, 2.5, 1.25, 2.5] and torch.equal(y, y[..., :1].expand_as(y))
+
+
+@pytest.mark.parametrize("other", ["per tensor", "inputs", "not float8", "blocks of 64", "alone"])
+def test_layers_of_other_forms_stay_out(tmp_path, other):
+    """A float8 layer that is not in blocks of 128 x 128 is left out, as any
+    layer without packed weights, and keeps nothing else from loading; build
+    refuses it by name."""
+    w, s = {"per tensor": _float8(128, 128, blocks=False), "inputs": _float8(128, 24),
+            "not float8": (torch.zeros(128, 128, dtype=BF), torch.ones(1, 1)),
+            "blocks of 64": (torch.zeros(128, 128).to(F8), torch.ones(2, 2)),
+            "alone": (None, torch.ones(1, 1))}[other]
+    t = {f"a.{n}": v for n, v in _packed().items()}
+    t["b.weight_scale_inv"] = s
+    if w is not None:
+        t["b.weight"] = w
+    fw, fs = _float8(128, 144)
+    t["c.weight"], t["c.weight_scale_inv"] = fw, fs
+    m = C.load_quantized(_save(tmp_path, t), device="cpu")
+    assert set(m) == {"a", "c"} and m["a"].mode == "affine" and m["c"].mode == "fp8"
+    with pytest.raises(ValueError, match="b: weight_scale_inv"):
+        C.build(t, "b", device="cpu")
+
+
+@pytest.mark.parametrize("shape", [(1, 2), (1,)])
+def test_packed_weights_go_before_a_scale_left_beside_them(tmp_path, shape):
+    t = {f"a.{n}": v for n, v in _packed().items()} | {"a.weight_scale_inv": torch.ones(shape)}
+    m = C.load_quantized(_save(tmp_path, t), device="cpu")
+    assert m["a"].mode == "affine"
+    assert C.build(t, "a", 128, device="cpu").mode == "affine"
