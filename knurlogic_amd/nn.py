@@ -184,9 +184,13 @@ class SwitchGLU:
                 and d.mode == f.mode and x.dtype == torch.bfloat16
                 and x.shape[-1] % 64 == 0 and (f.weight.shape[1] // 2) % 64 == 0)
 
-    def _one_call_fp8(self, x: torch.Tensor) -> bool:
-        """E4M3 experts in blocks of 128 in one call (kmi_switch_glu_fp8)."""
+    def _one_call_fp8(self, x: torch.Tensor, k: int) -> bool:
+        """E4M3 experts in blocks of 128 in one call (kmi_switch_glu_fp8: up to
+        64 pairs a token, x's values in bfloat16 within 2 GiB)."""
         f, d = self.fused, self.down_proj
+        H = x.shape[-1]
+        if k > 64 or x.numel() // max(H, 1) * -(-H // FP8_BLOCK) * FP8_BLOCK >= 2 ** 30:
+            return False
         return (f is not None and d.bias is None and f.mode == "fp8" and d.mode == "fp8"
                 and d.scales.dtype == f.scales.dtype and x.dtype == torch.bfloat16)
 
@@ -207,7 +211,7 @@ class SwitchGLU:
                               scores, f.group_size, f.bits)
         if self._one_call_mx(x, k):
             return switch_glu_mx(x, indices, f.weight, f.scales, d.weight, d.scales, scores, f.mode)
-        if self._one_call_fp8(x):
+        if self._one_call_fp8(x, k):
             return switch_glu_fp8(x, indices, f.weight, f.scales, d.weight, d.scales, scores)
         y = self.gathered(x, indices)
         return y if scores is None else moe_combine(y, scores)

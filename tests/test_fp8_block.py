@@ -1,0 +1,38 @@
+"""SwitchGLU over block-scaled E4M3 experts: which calls take the one-call
+kernels, and what the separate products give elsewhere."""
+import pytest
+import torch
+
+from knurlogic_amd import nn
+
+BF = torch.bfloat16
+
+
+def _layer(E, N, Kd, device):
+    return nn.QuantizedSwitchLinear(torch.zeros(E, N, Kd // 4, dtype=torch.int32, device=device).view(torch.uint32),
+                                    torch.ones(E, -(-N // 128), -(-Kd // 128), device=device), None, None, 128, 8, "fp8")
+
+
+def test_one_call_within_its_limits():
+    """64 pairs a token and 2^30 activations are the entry's limits; past them
+    the block goes through the separate products."""
+    glu = nn.SwitchGLU(_layer(2, 128, 272, "cpu"), _layer(2, 128, 272, "cpu"), _layer(2, 272, 128, "cpu"))
+    x = torch.empty(3, 272, dtype=BF, device="meta")
+    assert glu._one_call_fp8(x, 64) and not glu._one_call_fp8(x, 65)
+    # a row of 272 takes 384 codes
+    most = (2 ** 30 - 1) // 384
+    assert glu._one_call_fp8(torch.empty(most, 272, dtype=BF, device="meta"), 1)
+    assert not glu._one_call_fp8(torch.empty(7, most // 7 + 1, 272, dtype=BF, device="meta"), 1)
+    assert not glu._one_call_fp8(x.half(), 2)
+
+
+@pytest.mark.gpu
+def test_more_pairs_than_the_one_call_takes(dev):
+    g = torch.Generator().manual_seed(1)
+    w = lambda *s: (torch.randn(*s, generator=g) * 0.05).to(BF).to(dev)
+    glu = nn.SwitchGLU.from_float(w(70, 128, 256), w(70, 128, 256), w(70, 256, 128), mode="fp8")
+    x = w(3, 256) * 20
+    inds = torch.stack([torch.randperm(70, generator=g)[:65] for _ in range(3)]).to(dev)
+    y = glu(x, inds)
+    assert y.shape == (3, 65, 256) and torch.equal(y, glu.gathered(x, inds))
+    assert torch.isfinite(y).all() and (y != 0).any()
