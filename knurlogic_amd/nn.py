@@ -217,7 +217,8 @@ class SwitchGLU:
         return y if scores is None else moe_combine(y, scores)
 
     def gathered(self, x: torch.Tensor, indices: torch.Tensor) -> torch.Tensor:
-        """The same through separate gather_qmm calls (any layer mix)."""
+        """The same through separate gather_qmm calls (any layer mix, with the
+        layers' biases)."""
         lead, H = x.shape[:-1], x.shape[-1]
         k = indices.shape[-1]
         T = math.prod(lead)
@@ -225,7 +226,8 @@ class SwitchGLU:
         x3 = x.reshape(T, 1, H)
         rhs = indices.reshape(P).to(torch.int32)
         tok = torch.arange(P, device=x.device, dtype=torch.int32) // k
-        if self.fused is not None:
+        biased = lambda layer, y: y if layer.bias is None else add_bias(y, _bias(layer, y), rhs)
+        if self.fused is not None:                        # (stacked layers have no biases)
             f = self.fused
             gu = gather_qmm(x3, f.weight, f.scales, f.biases, lhs_indices=tok, rhs_indices=rhs,
                             group_size=f.group_size, bits=f.bits, mode=f.mode)  # [P, 1, 2I]
@@ -236,11 +238,12 @@ class SwitchGLU:
                               group_size=g.group_size, bits=g.bits, mode=g.mode)
             up = gather_qmm(x3, u.weight, u.scales, u.biases, lhs_indices=tok, rhs_indices=rhs,
                             group_size=u.group_size, bits=u.bits, mode=u.mode)
-            act = swiglu(gate, up)
+            act = swiglu(biased(g, gate), biased(u, up))
         d = self.down_proj
         pairs = torch.arange(P, device=x.device, dtype=torch.int32)
         y = gather_qmm(act, d.weight, d.scales, d.biases, lhs_indices=pairs, rhs_indices=rhs,
                        group_size=d.group_size, bits=d.bits, mode=d.mode)      # [P, 1, H]
+        y = biased(d, y)
         return y.reshape(*lead, k, y.shape[-1])
 
 

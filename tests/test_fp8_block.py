@@ -3,7 +3,9 @@ kernels, and what the separate products give elsewhere."""
 import pytest
 import torch
 
+import knurlogic_amd as K
 from knurlogic_amd import nn
+from tests.util import assert_close, to_numpy
 
 BF = torch.bfloat16
 
@@ -36,3 +38,23 @@ def test_more_pairs_than_the_one_call_takes(dev):
     y = glu(x, inds)
     assert y.shape == (3, 65, 256) and torch.equal(y, glu.gathered(x, inds))
     assert torch.isfinite(y).all() and (y != 0).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", ["affine", "mxfp8", "fp8"])
+@pytest.mark.parametrize("has", ["gud", "d", "g"])
+def test_biases_of_the_projections(dev, mode, has):
+    """A block whose layers have biases is its layers called one by one."""
+    g = torch.Generator().manual_seed(2)
+    w = lambda *s: (torch.randn(*s, generator=g) * 0.05).to(BF).to(dev)
+    E, H, I, T, k = 5, 256, 128, 9, 2
+    layer = lambda n, N, Kd: nn.QuantizedSwitchLinear.from_float(w(E, N, Kd), w(E, N) * 20 if n in has else None, mode=mode)
+    gate, up, down = layer("g", I, H), layer("u", I, H), layer("d", H, I)
+    x = w(T, H) * 20
+    inds = torch.randint(0, E, (T, k), generator=g).to(dev)
+    scores = torch.full((T, k), 0.5, dtype=BF, device=dev)
+    rows, of = x.repeat_interleave(k, 0)[:, None], inds.reshape(-1)
+    want = down(K.swiglu(gate(rows, of), up(rows, of)), of).view(T, k, H)
+    glu = nn.SwitchGLU(gate, up, down)
+    assert_close(to_numpy(glu(x, inds)), to_numpy(want), what="pairs")
+    assert_close(to_numpy(glu.combine(x, inds, scores)), to_numpy(K.moe_combine(want, scores)), what="combined")
