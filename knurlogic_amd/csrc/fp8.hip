@@ -126,7 +126,7 @@ int kmi_qmm_fp8(const void* x, int64_t M, int64_t K, int64_t N, const uint32_t* 
     F8Args a = {};
     a.w = (const unsigned char*)w; a.s = scales; a.e8 = e8m0; a.E = 1; a.wrows = N; a.K = K; a.N = N;
     a.x = x; a.xrows = M; a.y = y; a.rows = M; a.tm = p.tm; a.half = dtype == F16;
-    if (!p.gemm) return launch_fp8_skinny(a, dtype, false, ceil_div(M, a.tm), st);
+    if (!p.gemm) return launch_fp8_skinny(a, dtype, F8_PRODUCT, ceil_div(M, a.tm), st);
     rc = quantize_rows(a, x, dtype, M, (char*)workspace, st);
     if (rc) return rc;
     const int parts = fp8_gemm_parts(M, K, N, p.tm);
@@ -173,9 +173,9 @@ int kmi_gather_qmm_fp8(const void* x, int64_t X, int64_t M, int64_t K, const uin
     if (p.pairs) {
         a.route = rhs;
         a.tm = 1;
-        return launch_fp8_skinny(a, dtype, false, P, st);
+        return launch_fp8_skinny(a, dtype, F8_PRODUCT, P, st);
     }
-    if (!p.gemm) return launch_fp8_skinny(a, dtype, false, sr.max_tiles, st);
+    if (!p.gemm) return launch_fp8_skinny(a, dtype, F8_PRODUCT, sr.max_tiles, st);
     rc = quantize_rows(a, x, dtype, X * M, (char*)workspace + sort_index_bytes(P * M, E, p.tm), st);
     return rc ? rc : launch_fp8_gemm(a, sr.max_tiles, 1, st);
 }
@@ -243,10 +243,10 @@ int kmi_switch_glu_fp8(const void* x, int64_t T, int64_t H, int64_t I, int k, co
             g.tm = d.tm = 1;
         }
         d.x = g.y = ws;
-        rc = launch_fp8_skinny(g, dtype, true, p.pairs ? P : sr.max_tiles, st);
+        rc = launch_fp8_skinny(g, dtype, F8_GLU, p.pairs ? P : sr.max_tiles, st);
         if (rc) return rc;
         if (p.pairs && scores && fp8_combine_supported(I, k)) return launch_fp8_combine(d, scores, k, T, out, st);
-        rc = launch_fp8_skinny(d, dtype, false, p.pairs ? P : sr.max_tiles, st);
+        rc = launch_fp8_skinny(d, dtype, F8_DOWN, p.pairs ? P : sr.max_tiles, st);
     }
     if (rc) return rc;
     if (scores) return kmi_moe_combine(y, scores, dtype, T, k, H, out, stream);

@@ -9,7 +9,12 @@
 // bytes 16 (l / 16) .. + 15 and the same 64 further, x laid out alike).  The parts'
 // sums are added in LDS, in order, and one launch does it all: no pass over x
 // before, no partial sums in memory.  gate|up takes a block of gate rows and the
-// up rows beside it, in float16 operands (its results are rounded to E4M3 again).
+// up rows beside it.  An expert block's products have float16 operands, which hold
+// the codes exactly: gate|up's results are rounded to E4M3 again, and the down
+// product's to bfloat16 before the combine, where the 8-bit instruction's 1.2e-5
+// moved 1 result in 200 to its neighbour (the block's error against float64 0.00170,
+// 0.00165 so; 1 token of 128 experts [2048, 768] 20.9 us with either, 4 tokens of top 2
+// of 8 [4096, 4096] 76.8 for 73.7).
 //
 // Bound by HBM where the weights are large (16 rows of [14336, 4096] 16.6 us, 3.6
 // TB/s: each wave quantizes its part of x before its first product), by the launch
@@ -23,24 +28,13 @@ namespace {
 constexpr int ST_WAVES = 8;
 constexpr uint32_t ST_NONE = 0x80000000u;
 
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-
-__device__ __forceinline__ f16x8 st_halves(const i32x8& v, int q) {      // codes 8 q .. 8 q + 7
-    const uint32_t d0 = (uint32_t)v[2 * q], d1 = (uint32_t)v[2 * q + 1];
-    const f16x2 p0 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(d0, 1.f, false);
-    const f16x2 p1 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(d0, 1.f, true);
-    const f16x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(d1, 1.f, false);
-    const f16x2 p3 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(d1, 1.f, true);
-    return f16x8{p0.x, p0.y, p1.x, p1.y, p2.x, p2.y, p3.x, p3.y};
-}
-
 // the 16 x 16 products' sums of one block, times 2^(sw - 127) 2^(sx - 127)
-template <bool HALF>
+template <bool EXACT>
 __device__ __forceinline__ f32x4 st_times(const i32x8& w, const i32x8& x, uint32_t sw, uint32_t sx) {
     f32x4 p = {0.f, 0.f, 0.f, 0.f};
-    if constexpr (HALF) {
+    if constexpr (EXACT) {
 #pragma unroll
-        for (int q = 0; q < 4; q++) p = __builtin_amdgcn_mfma_f32_16x16x32_f16(st_halves(w, q), st_halves(x, q), p, 0, 0, 0);
+        for (int q = 0; q < 4; q++) p = __builtin_amdgcn_mfma_f32_16x16x32_f16(f8_halves(w, q), f8_halves(x, q), p, 0, 0, 0);
         const int e = (int)(sw + sx) - 254;
 #pragma unroll
         for (int i = 0; i < 4; i++) p[i] = __builtin_amdgcn_ldexpf(p[i], e);
@@ -59,12 +53,12 @@ constexpr int st_at_once = W == 4 ? 3 : KP == 8 ? 1 : 2;
 // R row blocks per wave and step; KPW blocks of K per wave at most.
 // The weights' loads are ordinary ones: non-temporal, [28672, 4096] x 1 row took 28.8 us
 // for 26.0, 8 pairs of 64 experts [2048, 2048] 13.0 for 11.6 ([4096, 4096] x 1 row: 7.3 for 7.7).
-template <class T, int KP, int KPW, int R, bool GLU, int W>
+template <class T, int KP, int KPW, int R, bool GLU, bool EXACT, int W>
 __global__ __launch_bounds__(64 * W, (st_at_once<KP, W> * W / 4)) void f8_stream(F8Args a, int steps) {
     constexpr int RB = GLU ? 2 : 1, NP = W / KP, F = R * RB * KPW;
-    // weight blocks (2 KB) in flight per wave: 8, or 4 where x, or gate|up's float16
-    // operands, take the registers
-    constexpr int DEPTH = GLU || KPW >= 16 ? 4 : 8, D = F < DEPTH ? F : DEPTH;
+    // weight blocks (2 KB) in flight per wave: 8, or 4 where x, or float16 operands,
+    // take the registers
+    constexpr int DEPTH = GLU || KPW >= 16 || (EXACT && KP < 8) ? 4 : 8, D = F < DEPTH ? F : DEPTH;
     constexpr int BATCH = KPW < 4 ? KPW : 4;       // x blocks quantized at a time
     static_assert(F % D == 0 && KPW % BATCH == 0, "ring");
     // a wave's x codes, and after them its sums (two steps'), in turn
@@ -225,12 +219,12 @@ __global__ __launch_bounds__(64 * W, (st_at_once<KP, W> * W / 4)) void f8_stream
             const int g = q % RB, i = q / RB % KPW, r = q / RB / KPW;
             const float sm = __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(s[g]), i));
             const uint32_t sw = (uint32_t)__builtin_amdgcn_readlane((int)se[g], i);
-            const f32x4 p = st_times<GLU>(wr[q % D], x[i], sw, xb[i]);
+            const f32x4 p = st_times<EXACT>(wr[q % D], x[i], sw, xb[i]);
             const float f = kp + KP * i < KB ? sm : 0.f;
 #pragma unroll
             for (int e = 0; e < 4; e++) acc[r][g][e] = __builtin_fmaf(p[e], f, acc[r][g][e]);
             load((q + D) % F, q + D < F ? step : next);
-            if constexpr (GLU) __builtin_amdgcn_sched_barrier(0);    // one block's float16 operands at a time
+            if constexpr (EXACT) __builtin_amdgcn_sched_barrier(0);    // one block's float16 operands at a time
         }
 #pragma unroll
         for (int r = 0; r < R; r++)
@@ -270,14 +264,17 @@ __global__ __launch_bounds__(64 * W, (st_at_once<KP, W> * W / 4)) void f8_stream
 
 // The down product and the weighted combine of a token's pairs: one workgroup per
 // 16 output columns and token, one wave per pair (in turn past 8), so that no
-// product leaves the workgroup before it is summed.  K up to CB_MAX_K.
+// product leaves the workgroup before it is summed.  K up to CB_MAX_K.  The last
+// blocks, fewer than are in flight, go by a branch each: 6 blocks of 768 inputs as 8
+// with two empty ones made the block of 1 token 21.5 us for 20.5.
 constexpr int CB_MAX_K = 4096, CB_MAX_SLOTS = 64, CB_DEPTH = 8;
 
 __global__ __launch_bounds__(64 * ST_WAVES) void f8_combine(F8Args a, const uint16_t* __restrict__ scores, int k,
                                                             uint16_t* __restrict__ out) {
     __shared__ __align__(16) unsigned char xs[ST_WAVES][CB_MAX_K];
     __shared__ unsigned char xe[ST_WAVES][CB_MAX_K / F8_BLOCK];
-    __shared__ float sums[CB_MAX_SLOTS][16], weight[CB_MAX_SLOTS];
+    __shared__ __align__(16) float sums[CB_MAX_SLOTS][16];
+    __shared__ float weight[CB_MAX_SLOTS];
     const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, c = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int K = (int)a.K, KB = (K + F8_BLOCK - 1) / F8_BLOCK;
@@ -322,21 +319,27 @@ __global__ __launch_bounds__(64 * ST_WAVES) void f8_combine(F8Args a, const uint
                     if (l16 == 0) xe[wave][b0 + c] = (unsigned char)byte;
                 }
             }
-            for (int b0 = 0; b0 < KB; b0 += CB_DEPTH) {
+            auto block = [&](int kb, int d) {
+                // every column the same row: column 0 is used
+                const i32x8 x = f8_operand(*(const u32x4*)(xs[wave] + kb * F8_BLOCK + 16 * c),
+                                           *(const u32x4*)(xs[wave] + kb * F8_BLOCK + 64 + 16 * c));
+                const f32x4 p = st_times<true>(w[d], x, (uint32_t)__builtin_amdgcn_readlane((int)sw, kb), xe[wave][kb]);
+                const float s = __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(sm), kb));
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[e] = __builtin_fmaf(p[e], s, acc[e]);
+            };
+            int b0 = 0;
+            for (; b0 + CB_DEPTH <= KB; b0 += CB_DEPTH) {
 #pragma unroll
                 for (int d = 0; d < CB_DEPTH; d++) {
-                    const int kb = b0 + d, at = kb < KB ? kb : 0;
-                    // every column the same row: column 0 is used
-                    const i32x8 x = f8_operand(*(const u32x4*)(xs[wave] + at * F8_BLOCK + 16 * c),
-                                               *(const u32x4*)(xs[wave] + at * F8_BLOCK + 64 + 16 * c));
-                    const f32x4 p = f8_mfma(w[d], x, f32x4{0.f, 0.f, 0.f, 0.f},
-                                            (uint32_t)__builtin_amdgcn_readlane((int)sw, at), xe[wave][at]);
-                    const float s = __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(sm), at));
-                    const float f = kb < KB ? s : 0.f;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) acc[e] = __builtin_fmaf(kb < KB ? p[e] : 0.f, f, acc[e]);
-                    load(kb + CB_DEPTH, d);
+                    block(b0 + d, d);
+                    load(b0 + d + CB_DEPTH, d);
                 }
+            }
+#pragma unroll
+            for (int d = 0; d < CB_DEPTH; d++) {             // (few: a branch costs less than an empty block)
+                if (b0 + d >= KB) break;
+                block(b0 + d, d);
             }
         }
         if (l16 == 0) *(f32x4*)&sums[slot][4 * c] = acc;
@@ -352,7 +355,7 @@ __global__ __launch_bounds__(64 * ST_WAVES) void f8_combine(F8Args a, const uint
     }
 }
 
-template <class T, int KP, int KPW, int R, bool GLU, int W = ST_WAVES>
+template <class T, int KP, int KPW, int R, bool GLU, bool EXACT, int W = ST_WAVES>
 int go(const F8Args& a, int64_t tiles, hipStream_t st) {
     const int64_t steps = ceil_div(a.N, 16 * R * (W / KP));
     if (steps >= (1LL << 31)) {
@@ -367,46 +370,47 @@ int go(const F8Args& a, int64_t tiles, hipStream_t st) {
     int64_t per = ceil_div(steps, tiles < most ? most / tiles : 1);
     if (a.tiles) per = ceil_div(steps * tiles, most) < steps ? ceil_div(steps * tiles, most) : steps;
     const int64_t gx = ceil_div(steps, per);
-    f8_stream<T, KP, KPW, R, GLU, W><<<dim3((unsigned)gx, (unsigned)tiles), 64 * W, 0, st>>>(a, (int)steps);
+    f8_stream<T, KP, KPW, R, GLU, EXACT, W><<<dim3((unsigned)gx, (unsigned)tiles), 64 * W, 0, st>>>(a, (int)steps);
     KMI_CHECK_LAUNCH("fp8 stream");
     return OK;
 }
 
 // The parts of K: as few as leave a wave's x in its registers (KPW blocks), so that
 // a part with no block is rare.
-template <class T, bool GLU>
+template <class T, bool GLU, bool EXACT>
 int parts(const F8Args& a, int64_t tiles, hipStream_t st) {
     const int64_t KB = ceil_div(a.K, F8_BLOCK);
     if constexpr (GLU) {
-        if (KB <= 4) return go<T, 2, 2, 1, GLU, 4>(a, tiles, st);
-        if (KB <= 8) return go<T, 2, 4, 1, GLU, 4>(a, tiles, st);
-        if (KB <= 16) return go<T, 4, 4, 1, GLU, 4>(a, tiles, st);
-        if (KB <= 32) return go<T, 8, 4, 1, GLU>(a, tiles, st);
-        if (KB <= 64) return go<T, 8, 8, 1, GLU>(a, tiles, st);
+        if (KB <= 4) return go<T, 2, 2, 1, GLU, EXACT, 4>(a, tiles, st);
+        if (KB <= 8) return go<T, 2, 4, 1, GLU, EXACT, 4>(a, tiles, st);
+        if (KB <= 16) return go<T, 4, 4, 1, GLU, EXACT, 4>(a, tiles, st);
+        if (KB <= 32) return go<T, 8, 4, 1, GLU, EXACT>(a, tiles, st);
+        if (KB <= 64) return go<T, 8, 8, 1, GLU, EXACT>(a, tiles, st);
     } else {
-        if (KB <= 2) return go<T, 2, 1, 4, GLU>(a, tiles, st);
-        if (KB <= 4) return go<T, 2, 2, 2, GLU>(a, tiles, st);
-        if (KB <= 8) return go<T, 2, 4, 1, GLU>(a, tiles, st);
-        if (KB <= 16) return go<T, 4, 4, 1, GLU>(a, tiles, st);
-        if (KB <= 32) return go<T, 8, 4, 1, GLU>(a, tiles, st);
-        if (KB <= 64) return go<T, 8, 8, 1, GLU>(a, tiles, st);
+        if (KB <= 2) return go<T, 2, 1, 4, GLU, EXACT>(a, tiles, st);
+        if (KB <= 4) return go<T, 2, 2, 2, GLU, EXACT>(a, tiles, st);
+        if (KB <= 8) return go<T, 2, 4, 1, GLU, EXACT>(a, tiles, st);
+        if (KB <= 16) return go<T, 4, 4, 1, GLU, EXACT>(a, tiles, st);
+        if (KB <= 32) return go<T, 8, 4, 1, GLU, EXACT>(a, tiles, st);
+        if (KB <= 64) return go<T, 8, 8, 1, GLU, EXACT>(a, tiles, st);
     }
-    if constexpr (!GLU) return go<T, 8, 16, 1, GLU>(a, tiles, st);
+    if constexpr (!EXACT) return go<T, 8, 16, 1, GLU, EXACT>(a, tiles, st);
     set_error("fp8: K=%lld for tiles of %d rows", (long long)a.K, a.tm);
     return EINVAL_ARG;
 }
 
 }  // namespace
 
-int64_t fp8_skinny_max_k(bool glu) { return glu ? 8192 : 16384; }
+int64_t fp8_skinny_max_k(bool block) { return block ? 8192 : 16384; }
 
-int launch_fp8_skinny(const F8Args& a, int dtype, bool glu, int64_t tiles, hipStream_t st) {
-    if (tiles <= 0 || tiles >= 65536 || a.tm < 1 || a.tm > 16 || (glu && dtype != BF16) || a.K > fp8_skinny_max_k(glu)) {
+int launch_fp8_skinny(const F8Args& a, int dtype, F8Use use, int64_t tiles, hipStream_t st) {
+    const bool block = use != F8_PRODUCT;
+    if (tiles <= 0 || tiles >= 65536 || a.tm < 1 || a.tm > 16 || (block && dtype != BF16) || a.K > fp8_skinny_max_k(block)) {
         set_error("fp8: %lld tiles of %d rows, K=%lld", (long long)tiles, a.tm, (long long)a.K);
         return EINVAL_ARG;
     }
-    if (glu) return parts<F8BF16, true>(a, tiles, st);
-    return dtype == BF16 ? parts<F8BF16, false>(a, tiles, st) : parts<F8F16, false>(a, tiles, st);
+    if (block) return use == F8_GLU ? parts<F8BF16, true, true>(a, tiles, st) : parts<F8BF16, false, true>(a, tiles, st);
+    return dtype == BF16 ? parts<F8BF16, false, false>(a, tiles, st) : parts<F8F16, false, false>(a, tiles, st);
 }
 
 bool fp8_combine_supported(int64_t K, int k) { return K <= CB_MAX_K && k <= CB_MAX_SLOTS; }
