@@ -327,6 +327,8 @@ int kmi_gather_qmm_fp8(const void* x, int64_t X, int64_t M, int64_t K, const uin
  * I % 128 == 0), w_down [E, H, I/4], H % 16 == 0, H and I <= 65536, k <= 64.  The activations
  * round(round(silu(gate)) * up) are quantized per row and 128 of I on their
  * way into the down product.  bf16.  out [T, k, H], or [T, H] with scores.
+ * gate and up, and down at decode sizes, are multiplied exactly (16-bit operands
+ * hold the codes); down's products of many rows are kmi_gather_qmm_fp8's.
  */
 size_t kmi_switch_glu_fp8_workspace_bytes(int64_t T, int64_t H, int64_t I, int k, int64_t E);
 int kmi_switch_glu_fp8(const void* x, int64_t T, int64_t H, int64_t I, int k, const int32_t* inds,

@@ -218,7 +218,8 @@ class SwitchGLU:
 
     def gathered(self, x: torch.Tensor, indices: torch.Tensor) -> torch.Tensor:
         """The same through separate gather_qmm calls (any layer mix, with the
-        layers' biases)."""
+        layers' biases).  Over fp8 layers the products are ``gather_qmm``'s, less
+        exact than the one call's (``switch_glu_fp8``)."""
         lead, H = x.shape[:-1], x.shape[-1]
         k = indices.shape[-1]
         T = math.prod(lead)

@@ -97,3 +97,58 @@ def test_few_rows_are_multiplied_exactly(dev, T, k, E, I, kind):
     out = bf(bf(bf(y) * to_numpy(scores)[..., None]).sum(1))
     off = (to_numpy(K.switch_glu_fp8(*args, scores.to(dev))) != out).mean()
     assert off < 1e-3, off
+
+
+def _separate_ref(x, inds, gate, up, down, dtype):
+    """float64 SwitchGLU of separate (codes, scales) with the roundings to
+    ``dtype`` of its steps, and how far separate products may be from it
+    (counted as for a single product; an activation, and its code, may round to
+    the neighbour)."""
+    rnd = lambda v: torch.from_numpy(np.asarray(v, np.float64)).to(torch.float32).to(dtype).double().numpy()
+    eps = torch.finfo(dtype).eps
+    act = lambda g, u: rnd(rnd(g / (1 + np.exp(-g))) * u)
+    T, k = inds.shape
+    H = down[0].shape[1]
+    y, far = np.zeros((T, k, H)), np.zeros((T, k, H))
+    for e in np.unique(inds):
+        t, j = np.nonzero(inds == e)
+        (g, gm, gc), (u, um, uc) = (R.product(x[t], w[e], s[e]) for w, s in (gate, up))
+        ge, ue = R.bound(0 * g, gm, gc, x.shape[1], 0), R.bound(0 * u, um, uc, x.shape[1], 0)
+        h, off = act(rnd(g), rnd(u)), 0
+        for a in (-1, 1):
+            for b in (-1, 1):
+                off = np.maximum(off, np.abs(R.rows(act(rnd(g + a * ge), rnd(u + b * ue))) - R.rows(h)))
+        d, mag, cut = R.product(h, down[0][e], down[1][e])
+        y[t, j] = rnd(d)
+        far[t, j] = R.bound(d, mag, cut, h.shape[1], eps) + eps / 2 * np.abs(d) + \
+            (1 + eps / 2) * off @ np.abs(R.weights(down[0][e], down[1][e])).T
+    return y, far
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, torch.float16])
+@pytest.mark.parametrize("T", [1, 20, 150])
+@pytest.mark.parametrize("I", [144, 256])
+def test_separate_products_against_float64(dev, dtype, T, I):
+    """What SwitchGLU runs where one call does not take it: I that is not whole
+    blocks, float16 rows; and gathered for what it does."""
+    E, H, k = 5, 272, 2
+    rng = np.random.default_rng(T + I)
+
+    def layer(n, m):
+        q = rng.integers(0, 256, (E, n, m), dtype=np.uint8) & 0xBF                     # below 2
+        s = (rng.random((E, -(-n // 128), -(-m // 128))) * 0.03 + 0.02).astype(np.float32)
+        up = torch.from_numpy(q.copy()).to(dev).view(torch.uint32)
+        return (q, s), nn.QuantizedSwitchLinear(up, torch.from_numpy(s).to(dev), None, None, 128, 8, "fp8")
+    (gate, lg), (up, lu), (down, ld) = layer(I, H), layer(I, H), layer(H, I)
+    glu = nn.SwitchGLU(lg, lu, ld)
+    assert (glu.fused is None) == (I == 144)
+    x = torch.randn(T, H, generator=torch.Generator().manual_seed(T)).to(dtype)
+    inds = np.stack([rng.permutation(E)[:k] for _ in range(T)])
+    y, far = _separate_ref(to_numpy(x), inds, gate, up, down, dtype)
+    ti = torch.from_numpy(inds).to(dev)
+    got = glu.gathered(x.to(dev), ti)
+    d = np.abs(to_numpy(got).astype(np.float64) - y)
+    assert got.dtype == dtype and (d <= far).all(), f"{np.max(d / far):.3g} of the bound"
+    if not glu._one_call_fp8(x, k):
+        assert torch.equal(glu(x.to(dev), ti), got)
