@@ -40,15 +40,23 @@ struct Plan {
 };
 
 //
-// Dense: the stream up to 16 rows ([4096, 4096] x 16 rows: 11 us, tiles 14.4;
-// [14336, 4096]: 19.3, 20.6), then the tiles with the least rounds x time of a
-// round.  A block of 128 inputs takes 0.5 us in tiles of 64 rows where each is
+// (Times at the rules: us per call in a captured graph over 600 MB of different
+// weights, so that none is in a cache.)
+//
+// Dense: the stream up to 16 rows, while each wave's part of x, which it quantizes
+// before its first product, is short: 9 rows or more up to K = 4096, 2 or more up to 9216,
+// one up to the most.  Stream and tiles at 16 rows: [4096, 4096] 11.6, 14.4;
+// [14336, 4096] 19.1, 20.6; [4096, 4352] 15.2, 15.3; [4096, 5120] 17.1, 15.6; [4096,
+// 8192] 19.2, 17.4; [4096, 14336] 31.9, 21.4; at 8: [4096, 8192] 15.2, 17.1; [4096, 9216]
+// 17.8, 17.8; [14336, 10240] 39.6, 36.6; [4096, 14336] 23.3, 21.0; at 2 the same within 1; at 1:
+// [4096, 8192] 11.8, 16.5; [4096, 14336] 17.3, 20.5; [8192, 16384] 32.8, 42.2; but [5120,
+// 12288] 23.4, 20.9.  Then the tiles with the least rounds x time of a round.  A block of 128 inputs takes 0.5 us in tiles of 64 rows where each is
 // alone on its CU, 0.8 two to a CU; 0.9 and 1.2 in tiles of 128; 1.5 in tiles of 256
 // x 256, one to a CU.  [4096, 4096], tiles of 64 / 128 / 256: 512 rows 23 / 35 / 59
 // us, 1024 35 / 38 / 60, 2048 63 / 50 / 65, 4096 117 / 94 / 75; [14336, 4096]: 256
 // rows 37 / 38 / 62, 512 64 / 49 / 64, 1024 106 / 90 / 67.
 Plan plan_dense(int64_t M, int64_t K, int64_t N) {
-    if (M <= 16 && K <= fp8_skinny_max_k(false)) return {false, 16};
+    if (M <= 16 && K <= (M == 1 ? fp8_skinny_max_k(false) : M <= 8 ? 9216 : 4096)) return {false, 16};
     const auto rounds = [&](int64_t tm, int64_t tn, int64_t at_once) {
         return ceil_div(ceil_div(M, tm) * ceil_div(N, tn), at_once);
     };

@@ -146,3 +146,15 @@ def test_loader_refuses_other_block_shapes():
         C.build({"a.weight": w.float(), "a.weight_scale_inv": torch.ones(2, 2)}, "a", device="cpu")
     with pytest.raises(ValueError, match="128 x 128"):
         C.build({"a.weight": w[:, :24], "a.weight_scale_inv": torch.ones(2, 1)}, "a", device="cpu")
+
+
+@pytest.mark.parametrize("M,K,stream", [(1, 4096, 1), (16, 4096, 1), (17, 4096, 0), (16, 4112, 0), (9, 4112, 0), (8, 4112, 1),
+                                        (8, 9216, 1), (8, 9232, 0), (2, 9232, 0), (2, 14336, 0), (16, 14336, 0),
+                                        (1, 16384, 1), (1, 16400, 0)])
+def test_few_rows_of_a_long_k_leave_the_stream(M, K, stream):
+    """The stream quantizes x in every workgroup before its first product: with
+    many inputs that costs more than the pass over x that the tiles take (which
+    need a workspace for it; the stream needs none)."""
+    for N in (64, 4096, 14336):
+        for dtype in (0, 1):
+            assert (_abi.load().kmi_qmm_fp8_workspace_bytes(M, K, N, dtype) == 0) == bool(stream)
