@@ -75,7 +75,12 @@ Plan plan_dense(int64_t M, int64_t K, int64_t N) {
 // [2048, 2048], 256 rows: 61.9, 58.8), or an expert's few rows are long (128 experts
 // [1536, 4096], 256 rows: 126, 156, 512 rows: 148, 184; 768: 186, 174; 256 experts
 // [2048, 4096], 256 rows, one each: 287, 253).  Tiles of 64 rows (gate|up's only
-// size) up to 64 rows to an expert, then 128: 64 experts [2048, 2048], 96 rows each:
+// size) up to 64 rows to an expert, then 128, as below.  Where the rule takes not the
+// best of the three: 128 experts [1536, 4096], 96 rows tiles 109 (stream 84), 128 rows
+// tiles 128 (pairs 112); 256 experts [2048, 4096], 96 rows pairs 147 (stream 121); 64
+// experts [2048, 2048], 48 rows tiles 40.5 (pairs 36.1); blocks of 32 experts 2048 -> 768, top
+// 4, 6 and 8 tokens: stream 37.4 and 41.6 (pairs 33.9 and 37.3): it counts rows to an
+// expert, not the bytes each way reads.  Tiles of 64 and 128: 64 experts [2048, 2048], 96 rows each:
 // 97 us, in tiles of 64 104; 8 experts [4096, 4096], 64 rows each: 54 both.
 Plan plan_grouped(int64_t rows, int64_t P, int64_t E, int64_t K, int64_t N, bool glu) {
     const int64_t experts = P < E ? P : E, per = ceil_div(rows, experts);

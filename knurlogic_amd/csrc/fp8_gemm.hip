@@ -12,13 +12,14 @@
 // D holds activation rows along its columns, so a lane has one row's scale per
 // 16 x 16 tile.
 //
-// Bound by the matrix instructions in full tiles: 4096 rows of [4096, 14336] 187 us
-// (2.57 PFLOP/s; the chip gives an 8-bit 16 x 16 x 128 every 32 cycles at 2.16 GHz,
-// 175 us) and 35 of the pass before; 2048 rows of [14336, 4096] are 448 tiles on
-// 256 CUs, 1.75 rounds: 132 us + 8.  Few rows are bound by a workgroup's chain of
-// latencies: 77 rows of [4100, 2064] 13.6 us, 2.7 of them the pass; rows of many
-// experts by the weights' stream: 128 rows of 128 experts [1536, 2048] 47 us in all
-// with the sort (255 MB at 5.4 TB/s).
+// Bound by the matrix instructions in full tiles: 4096 rows of [4096, 14336] 185 us
+// (2.6 PFLOP/s; the chip gives an 8-bit 16 x 16 x 128 every 32 cycles at 2.16 GHz,
+// 175 us) and 35 of the pass before, called now and then; call after call the same tiles
+// take 196-229.  2048 rows of [14336, 4096] are 448 tiles on 256 CUs, 1.75 rounds:
+// 131 us + 8.  Few rows are bound by a workgroup's chain of latencies: 77 rows of
+// [4100, 2064] 12 us + 3; rows of many experts by the weights' stream: 128 rows that
+// reach 62 of 128 experts [1536, 2048] (197 MB) 39-43 us, 4.6-5.0 TB/s, + 5 for the sort
+// and 3 for x.
 #include "fp8_tiles.hpp"
 
 namespace kmi {

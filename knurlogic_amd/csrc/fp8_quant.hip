@@ -1,6 +1,9 @@
 // E4M3 with one E8M0 scale per block of 128 x 128: weights into codes and
-// scales, and back.  Bound by HBM: bf16 [14336, 4096] 34.4 us, 5.1 TB/s read and
-// written (a large copy: 4.8).
+// scales, and back.  Codes from weights are bound by HBM: bf16 [14336, 4096] 30 us, 5.8
+// TB/s read and written; a few small experts (5 of [700, 1040], float32) by one
+// workgroup's read, maximum and write in sequence, 6.8 us (270 workgroups on 256
+// CUs).  The way back is a plain loop whose time nobody waits for at load: 147 us for
+// the same bf16 weight, 1.2 TB/s.
 #include "fp8.hpp"
 #include "../../include/knurlogic_amd.h"
 

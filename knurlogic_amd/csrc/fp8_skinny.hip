@@ -16,9 +16,10 @@
 // 0.00165 so; 1 token of 128 experts [2048, 768] 20.9 us with either, 4 tokens of top 2
 // of 8 [4096, 4096] 76.8 for 73.7).
 //
-// Bound by HBM where the weights are large (16 rows of [14336, 4096] 16.6 us, 3.6
-// TB/s: each wave quantizes its part of x before its first product), by the launch
-// and one chain of latencies where they are not (1 row of [4096, 4096] 7 us).
+// Bound by x's quantization, which each wave does for its part before its first
+// product, and the weights' stream after it (kernel trace, no weights in a cache: 16
+// rows of [14336, 4096] 18-19 us, 3.2 TB/s), and where the weights are small by the
+// launch and one chain of latencies (1 row of [4096, 4096] 7.0-7.9 us, 2.3 TB/s).
 #include "fp8.hpp"
 
 namespace kmi {
